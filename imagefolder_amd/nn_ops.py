@@ -313,3 +313,41 @@ def spatial_attention(q, k, v):
     qq = q.reshape(b, c, hh * ww).permute(0, 2, 1)
     w_ = F.softmax(torch.bmm(qq, k.reshape(b, c, hh * ww)) * (int(c) ** (-0.5)), dim=2)
     return torch.bmm(v.reshape(b, c, hh * ww), w_.permute(0, 2, 1)).reshape(b, c, hh, ww)
+
+
+def dropout(x, p=0.5, training=True, key=None, residual=None):
+    """Dropout [+ residual] with a counter-based generator: y = keep ? x / (1 - p) : 0 (+ residual), the mask a function of `key` and an element's place
+    in memory that the backward pass computes again (csrc/xq_drop.hip; nothing of the mask is stored).
+      x: bf16 or fp32, any shape and any dense memory order (the result keeps it; a tensor with holes is made contiguous first);
+      p: rounded to a multiple of 2^-16; 1 leaves zeros; not training or p = 0: x (+ residual) itself;
+      key: int64 tensor of two values (seed, stream) on x's device: the same key and memory order give the same mask.  It is read when the kernels run and
+           must not change before the backward pass has; None draws one from the device's default generator (torch.manual_seed, graph-safe);
+      residual: added in fp32 before the one rounding; x's shape, x's type or fp32 (the result has its type).
+    CPU tensors: F.dropout (no key there)."""
+    if not training or p == 0:
+        return x if residual is None else x + residual
+    if not x.is_cuda:
+        if key is not None:
+            from ._lib import XqError
+            raise XqError("dropout: a keyed mask is computed on an MI355X only (x lives on the CPU)")
+        IMPL["dropout"] = "library (CPU)"
+        y = F.dropout(x, p)
+        return y if residual is None else y + residual
+    from . import ops_seq
+    IMPL["dropout"] = "hip"
+    return ops_seq.dropout(x, p, key, residual)
+
+
+def embedding(idx, weight, scale=1.0, padding_idx=None, dtype=None):
+    """scale * weight[idx]: (*idx.shape, D) in `dtype` (default: the table's), one rounding; the gradient of the table is summed over tokens sorted by row,
+    in fp32, without atomics: the same bits from run to run (csrc/xq_embed.hip).
+      weight: (V, D) bf16 or fp32, V <= 2^20; idx: int64 or int32, any shape; padding_idx: a row that is looked up but receives no gradient.
+    An index outside [0, V) gives a row of NaN and no gradient (no host check: that would wait for the GPU).  CPU tensors: F.embedding."""
+    if not weight.is_cuda:
+        IMPL["embedding"] = "library (CPU)"
+        y = F.embedding(idx, weight, padding_idx)
+        y = y if scale == 1.0 else y * scale
+        return y if dtype is None else y.to(dtype)
+    from . import ops_seq
+    IMPL["embedding"] = "hip"
+    return ops_seq.embedding(idx, weight, scale, padding_idx, dtype)

@@ -560,6 +560,28 @@ int xq_gemm_bf16_batched(int op, const void *a, const void *b, int batch, int64_
 int xq_gemm_bf16_tn(const void *g_y, const void *x, int64_t R, int64_t P, int64_t Q, float *g_w, void *workspace,
                     size_t workspace_bytes, int impl, xq_stream_t stream);
 
+/* ---- operators of token models that read the tokenizer's codes: dropout, embedding, cross attention (no counterpart in the reference's
+ *      tokenizer path; nn.Dropout of its ResnetBlock / Mlp arguments, nn.Embedding of its level tables) ------------------------------------ */
+
+/* dropout whose mask is a function of (key, position), csrc/xq_drop.hip: with t = round(65536 p),
+ *   y[i] = u16(i) >= t ? x[i] * 65536 / (65536 - t) : 0   (+ residual[i], nullable, of y's type),
+ * u16(i) = half i % 2 (low first) of word (i % 8) / 2 of Philox4x32-10 at counter (i / 8 low, high, key[1] low, high) under the key
+ * (key[0] low, high); i counts elements in memory order.  The backward pass is the same call on the gradient (x = g, no residual).
+ *   x: x_bf16 ? bf16 : fp32, [n]; key: DEVICE int64 [2], read by the kernel; y: y_bf16 ? bf16 : fp32, [n], may be x where the types agree.
+ *   p in [0, 1].  Any alignment of the elements; 16-byte aligned pointers take the vector path. */
+int xq_dropout(const void *x, int x_bf16, const void *residual, int64_t n, double p, const int64_t *key, void *y, int y_bf16, xq_stream_t stream);
+
+/* embedding lookup, csrc/xq_embed.hip: y[n][D] = scale * w[idx[n]][D]; idx int64 (idx_i64) or int32 [N].  An index outside [0, V) reads nothing of the
+ * table: its row of y is NaN.  V <= 2^20, N < 2^31. */
+int xq_embedding_forward(const void *idx, int idx_i64, const void *w, int w_bf16, int64_t N, int64_t V, int D, float scale, void *y, int y_bf16,
+                         xq_stream_t stream);
+/* its gradient: dw[v] = scale * sum over n with idx[n] = v of g[n] (fp32 sums in a fixed order: ascending n in runs of the sorted tokens, no atomics on
+ * floats; bit-identical from run to run); every row of dw [V][D] is written.  skip: a row that receives no gradient (a padding id; -1 for none);
+ * indices outside [0, V) add nothing.  workspace: xq_embedding_backward_workspace_bytes (0 for sizes the call refuses and for N = 0). */
+size_t xq_embedding_backward_workspace_bytes(int64_t N, int64_t V, int D);
+int xq_embedding_backward(const void *idx, int idx_i64, const void *g, int g_bf16, int64_t N, int64_t V, int D, float scale, int64_t skip, void *dw,
+                          int dw_bf16, void *workspace, size_t workspace_bytes, xq_stream_t stream);
+
 /* ---- measurement hooks (bench.py): HIP events recorded around the instrumented hand-written kernels on the stream they
  *      are launched on.  xq_prof_enable(1) resets and arms, (0) disarms and keeps what was recorded, (2) arms without resetting; xq_prof_collect_kind synchronises the recorded events of one
  *      kernel kind and returns their summed duration, launch count and summed algorithmic work (flops) since arming;
