@@ -5,7 +5,7 @@
 // inside a row) and every row of dw is one fp32 chain, written once (rows without a token with zeros: no clearing pass).
 //
 // The sort is two launches, not a radix sort's pass per digit: (1) `embed_bin_kernel` — every block sorts its slice of the tokens by the row's high
-// bits (the bucket: up to 1024 buckets of 2^shift rows) in LDS and writes the slice's sorted list and its bucket starts; (2) `embed_sort_kernel` —
+// bits (the bucket: 256 or up to 1024 buckets of 2^shift rows) in LDS and writes the slice's sorted list and its bucket starts; (2) `embed_sort_kernel` —
 // one block per bucket gathers its pieces of every slice's list (they follow each other in token order) and places them by the row's low bits.  The
 // position of a bucket in the sorted whole needs no scan over buckets: it is the sum of the slices' starts of that bucket.
 // The sums are two more: (3) `embed_sum_kernel` — rows of up to `chunk` tokens whole, and of the longer ones (a frequent word, a padding id) the pieces
@@ -18,27 +18,47 @@
 
 namespace {
 
-constexpr int BIN_THREADS = 256, BIN_WAVES = BIN_THREADS / 64, BIN_ROUNDS = 8, BIN_TILE = BIN_THREADS * BIN_ROUNDS;
-constexpr int MAX_BUCKETS = 1024, MAX_LOCAL = 1024;      // rows <= 2^20
+constexpr int TILE = 2048;                               // tokens that a block of the first launch ranks at once
+constexpr int BIN_THREADS = 512;
+constexpr int MAX_BUCKETS = 1024;                        // of 1024 rows at most: rows <= 2^20
 
 // ---- forward ------------------------------------------------------------------------------------------------------------------------------
 
+// a / per_row from the host's floor(2^64 / per_row) + 1 (exact for whole numbers below 2^32; 0 stands for a divisor of one)
+__device__ __forceinline__ uint32_t quotient(uint32_t a, uint64_t reciprocal) { return reciprocal ? (uint32_t)__umul64hi((uint64_t)a, reciprocal) : a; }
+
+// One thread per VEC columns; `per_row` threads a row, a quotient by the host's reciprocal (a block of threads per row would idle a quarter of them at
+// a width of 768).  split = 8: XCD x (blocks go round-robin over the eight) takes the x-th eighth of the columns of every token, so that a table of up to
+// 32 MB, which no 4 MB L2 holds, is held by the eight together; the rows that many tokens share then come out of L2.
 template <typename TW, typename TY, typename TI, int VEC>
-__global__ __launch_bounds__(256) void embed_fwd_kernel(const TI *__restrict__ idx, const TW *__restrict__ w, long N, long V, int D, int lanes, float scale,
-                                                        TY *__restrict__ y) {
-    const int rows = 256 / lanes, lane = threadIdx.x % lanes;
-    for (long n = (long)blockIdx.x * rows + threadIdx.x / lanes; n < N; n += (long)gridDim.x * rows) {
-        const long v = (long)idx[n];
-        const bool ok = v >= 0 && v < V;
-        const TW *src = w + (ok ? v : 0) * (long)D;
-        TY *dst = y + n * (long)D;
-        for (int c = lane * VEC; c < D; c += lanes * VEC) {
-            float a[VEC];
-            load_vec<TW, VEC>(src + c, a);
+__global__ __launch_bounds__(256) void embed_fwd_kernel(const TI *__restrict__ idx, const TW *__restrict__ w, long V, int D, int split, uint32_t per_row, uint32_t total,
+                                                        uint64_t reciprocal, float scale, TY *__restrict__ y) {
+    constexpr int U = 4;
+    const uint32_t part = split == 1 ? 0 : blockIdx.x & 7, block = split == 1 ? blockIdx.x : blockIdx.x >> 3;
+    const uint32_t step = gridDim.x / split * 256u;
+    uint32_t at[U];
+    long v[U];
+    float a[U][VEC];
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) a[j] = ok ? a[j] * scale : __uint_as_float(0x7fc00000u);   // an index outside the table reads nothing of it
-            store_vec<TY, VEC>(dst + c, a);
-        }
+    for (int u = 0; u < U; ++u) {
+        at[u] = block * 256u + threadIdx.x + u * step;
+        v[u] = -1;
+        if (at[u] < total) v[u] = (long)idx[quotient(at[u], reciprocal)];
+    }
+    uint32_t n[U], c[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        n[u] = quotient(at[u], reciprocal);
+        c[u] = at[u] < total ? (at[u] - n[u] * per_row + part * per_row) * VEC : 0;
+        const long row = v[u] >= 0 && v[u] < V ? v[u] : 0;
+        load_vec<TW, VEC>(w + row * D + c[u], a[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const bool ok = v[u] >= 0 && v[u] < V;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) a[u][j] = ok ? a[u][j] * scale : __uint_as_float(0x7fc00000u);   // an index outside the table reads nothing of it
+        if (at[u] < total) store_vec<TY, VEC>(y + (long)n[u] * D + c[u], a[u]);
     }
 }
 
@@ -55,9 +75,10 @@ __device__ __forceinline__ uint64_t same_digit(uint32_t digit, int bits, bool li
 }
 
 // exclusive scan of count[0 .. n) in place by the whole block; `part` holds one value a wave.  Returns the total.
+template <int THREADS>
 __device__ __forceinline__ uint32_t block_scan(uint32_t *count, int n, uint32_t *part) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int per = (n + BIN_THREADS - 1) / BIN_THREADS;
+    const int per = (n + THREADS - 1) / THREADS;
     const int lo = min(tid * per, n), hi = min(lo + per, n);
     uint32_t mine = 0;
     for (int i = lo; i < hi; ++i) mine += count[i];
@@ -70,7 +91,8 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t *count, int n, uint32_t 
     if (lane == 63) part[wave] = incl;
     __syncthreads();
     uint32_t before = 0, total = 0;
-    for (int w = 0; w < BIN_WAVES; ++w) {
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w) {
         if (w < wave) before += part[w];
         total += part[w];
     }
@@ -84,252 +106,332 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t *count, int n, uint32_t 
     return total;
 }
 
-// The stable ranks of one tile of BIN_TILE items: wave w owns items [w * 512, (w + 1) * 512) of the tile in rounds of 64; at[w][digit] counts what the
-// wave has seen (own region of LDS: no two waves meet).  rank[r] = items of the same digit before this one in the wave.
-template <int ROUNDS>
-__device__ __forceinline__ void wave_ranks(const uint32_t (&digit)[ROUNDS], const bool (&live)[ROUNDS], int bits, uint32_t *at, uint32_t (&rank)[ROUNDS]) {
+// A stable counting sort of one tile by a whole block.  Every wave holds `rounds` x 64 items that follow each other in token order, round r's digit in
+// digit[r] (NONE: no item); seen[wave][digit] counts what a wave has met (no two waves share a counter, and the additions of one wave are in order).
+constexpr uint32_t NONE = 0xffffffffu;
+
+template <int ROUNDS, int DIGITS>
+__device__ __forceinline__ void tile_ranks(const uint32_t (&digit)[ROUNDS], int rounds, int bits, int digits, uint32_t (*seen)[DIGITS], uint32_t (&rank)[ROUNDS]) {
     const int lane = threadIdx.x & 63;
+    uint32_t *at = seen[threadIdx.x >> 6];
+    for (int i = lane; i < digits; i += 64) at[i] = 0;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
     for (int r = 0; r < ROUNDS; ++r) {
-        const uint64_t same = same_digit(digit[r], bits, live[r]);
+        if (r >= rounds) break;
+        const bool live = digit[r] != NONE;
+        const uint64_t same = same_digit(digit[r], bits, live);
         const uint32_t before = (uint32_t)__popcll(same & ((1ull << lane) - 1));
-        uint32_t seen = 0;
-        if (live[r]) seen = at[digit[r]];
-        rank[r] = seen + before;
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");       // every lane has read before the last one of the digit writes, and reads again after it
-        if (live[r] && (same >> lane) == 1ull) at[digit[r]] = seen + before + 1;
+        uint32_t met = 0;
+        if (live) met = at[digit[r]];
+        rank[r] = met + before;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");       // every lane has read before the last one of a digit writes, and reads again after it
+        if (live && (same >> lane) == 1ull) at[digit[r]] = met + before + 1;
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
+    __syncthreads();
 }
 
-// slices of `tiles` tiles; list (row low bits | token) in bucket order, starts[slice][bucket] relative to the slice, buckets + 1 entries
+// the tile's count of every digit -> count
+template <int WAVES>
+__device__ __forceinline__ void tile_counts(const uint32_t *seen, int pitch, int digits, uint32_t *count) {
+    for (int i = threadIdx.x; i < digits; i += WAVES * 64) {
+        uint32_t c = 0;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) c += seen[w * pitch + i];
+        count[i] = c;
+    }
+    __syncthreads();
+}
+
+// base: where each digit's next item goes -> seen[wave][digit]: where the wave's first one goes; base moves on behind the tile
+template <int WAVES>
+__device__ __forceinline__ void tile_places(uint32_t *seen, int pitch, int digits, uint32_t *base) {
+    for (int i = threadIdx.x; i < digits; i += WAVES * 64) {
+        uint32_t b = base[i];
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            const uint32_t c = seen[w * pitch + i];
+            seen[w * pitch + i] = b;
+            b += c;
+        }
+        base[i] = b;
+    }
+    __syncthreads();
+}
+
+// slices of `tiles` tiles; list (row low bits, token) in bucket order, starts[slice][bucket] relative to the slice, buckets + 1 entries
 template <typename TI>
 __global__ __launch_bounds__(BIN_THREADS) void embed_bin_kernel(const TI *__restrict__ idx, long N, long V, long skip, int shift, int buckets, int bits,
                                                                 int tiles, uint2 *__restrict__ list, uint32_t *__restrict__ starts) {
-    __shared__ uint32_t at[BIN_WAVES][MAX_BUCKETS];
+    constexpr int WAVES = BIN_THREADS / 64, ROUNDS = TILE / BIN_THREADS;
+    __shared__ uint32_t seen[WAVES][MAX_BUCKETS];
     __shared__ uint32_t base[MAX_BUCKETS];
-    __shared__ uint32_t part[BIN_WAVES];
+    __shared__ uint32_t part[WAVES];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const long first = (long)blockIdx.x * tiles * BIN_TILE, end = min(N, first + (long)tiles * BIN_TILE);
-    // the slice's bucket counts (a slice of one tile gets them from the ranking below)
-    for (int i = tid; i < buckets; i += BIN_THREADS) base[i] = 0;
-    __syncthreads();
-    for (long n = first + tid; n < end; n += BIN_THREADS) {
-        const long v = (long)idx[n];
-        if (v >= 0 && v < V && v != skip) atomicAdd(&base[v >> shift], 1u);      // whole numbers: the order of the adds does not matter
-    }
-    __syncthreads();
-    const uint32_t total = block_scan(base, buckets, part);
+    const long first = (long)blockIdx.x * tiles * TILE, end = min(N, first + (long)tiles * TILE);
     uint32_t *st = starts + (long)blockIdx.x * (buckets + 1);
-    for (int i = tid; i < buckets; i += BIN_THREADS) st[i] = base[i];
-    if (tid == 0) st[buckets] = total;
-    for (long t0 = first; t0 < end; t0 += BIN_TILE) {
-        for (int i = lane; i < buckets; i += 64) at[wave][i] = 0;
+    auto publish = [&] {
+        const uint32_t total = block_scan<BIN_THREADS>(base, buckets, part);
+        for (int i = tid; i < buckets; i += BIN_THREADS) st[i] = base[i];
+        if (tid == 0) st[buckets] = total;
+    };
+    if (tiles > 1) {            // the slice's counts first; a slice of one tile has them from its ranks
+        for (int i = tid; i < buckets; i += BIN_THREADS) base[i] = 0;
         __syncthreads();
-        uint32_t digit[BIN_ROUNDS], low[BIN_ROUNDS], rank[BIN_ROUNDS];
-        bool live[BIN_ROUNDS];
+        for (long n0 = first + wave * 64; n0 < end; n0 += BIN_THREADS) {
+            long v = -1;
+            if (n0 + lane < end) v = (long)idx[n0 + lane];
+            const bool live = v >= 0 && v < V && v != skip;
+            const uint64_t same = same_digit((uint32_t)(v >> shift), bits, live);
+            if (live && (same & ((1ull << lane) - 1)) == 0) atomicAdd(&base[v >> shift], (uint32_t)__popcll(same));   // whole numbers: any order
+        }
+        __syncthreads();
+        publish();
+        __syncthreads();
+    }
+    for (long t0 = first; t0 < end; t0 += TILE) {
+        uint32_t digit[ROUNDS], low[ROUNDS], rank[ROUNDS];
+        const long n0 = t0 + wave * (64 * ROUNDS) + lane;
 #pragma unroll
-        for (int r = 0; r < BIN_ROUNDS; ++r) {
-            const long n = t0 + wave * (64 * BIN_ROUNDS) + r * 64 + lane;
+        for (int r = 0; r < ROUNDS; ++r) {
+            const long n = n0 + r * 64;
             long v = -1;
             if (n < end) v = (long)idx[n];
-            live[r] = v >= 0 && v < V && v != skip;
-            digit[r] = live[r] ? (uint32_t)(v >> shift) : 0u;
+            const bool live = v >= 0 && v < V && v != skip;
+            digit[r] = live ? (uint32_t)(v >> shift) : NONE;
             low[r] = (uint32_t)v & ((1u << shift) - 1);
         }
-        wave_ranks<BIN_ROUNDS>(digit, live, bits, at[wave], rank);
-        __syncthreads();
-        for (int i = tid; i < buckets; i += BIN_THREADS) {      // where each wave's items of bucket i begin; base moves on to the next tile
-            uint32_t b = base[i];
-#pragma unroll
-            for (int w = 0; w < BIN_WAVES; ++w) {
-                const uint32_t c = at[w][i];
-                at[w][i] = b;
-                b += c;
-            }
-            base[i] = b;
+        tile_ranks<ROUNDS, MAX_BUCKETS>(digit, ROUNDS, bits, buckets, seen, rank);
+        if (tiles == 1) {
+            tile_counts<WAVES>(seen[0], MAX_BUCKETS, buckets, base);
+            publish();
         }
-        __syncthreads();
+        tile_places<WAVES>(seen[0], MAX_BUCKETS, buckets, base);
 #pragma unroll
-        for (int r = 0; r < BIN_ROUNDS; ++r) {
-            const long n = t0 + wave * (64 * BIN_ROUNDS) + r * 64 + lane;
-            if (live[r]) list[first + at[wave][digit[r]] + rank[r]] = make_uint2(low[r], (uint32_t)n);
-        }
+        for (int r = 0; r < ROUNDS; ++r)
+            if (digit[r] != NONE) list[first + seen[wave][digit[r]] + rank[r]] = make_uint2(low[r], (uint32_t)(n0 + r * 64));
         __syncthreads();
     }
 }
 
-// one block per bucket: row starts of the bucket's rows, its tokens in row order, and the rows of every chunk's first and last position
-__global__ __launch_bounds__(BIN_THREADS) void embed_sort_kernel(const uint2 *__restrict__ list, const uint32_t *__restrict__ starts, long V, int shift,
-                                                                 int buckets, int bits, int slices, long slice_tokens, uint32_t *__restrict__ row_start,
-                                                                 uint32_t *__restrict__ order, int chunk_bits, uint32_t *__restrict__ edge) {
+// One block per bucket: row starts of the bucket's rows, its tokens in row order, and the rows of every chunk's first and last position.  Every wave
+// counts the rows of its own eighth of the bucket, then places it: nothing but two meetings of the block between them, so that a bucket that one frequent
+// row fills (14000 of 100000 tokens) costs 40 us (in tiles that the whole block ranked: 100); 7 us where no row is frequent.
+template <int SORT_THREADS>
+__global__ __launch_bounds__(SORT_THREADS) void embed_sort_kernel(const uint2 *__restrict__ list, const uint32_t *__restrict__ starts, long V, int shift,
+                                                                  int buckets, int slices, int half, long slice_tokens, uint32_t *__restrict__ row_start,
+                                                                  uint32_t *__restrict__ order, int chunk_bits, uint32_t *__restrict__ edge) {
+    constexpr int WAVES = SORT_THREADS / 64, U = 4;
     extern __shared__ uint32_t lds[];
-    uint32_t *piece = lds;                       // [slices + 1] where a slice's piece begins in the bucket
-    __shared__ uint32_t at[BIN_WAVES][MAX_LOCAL];
-    __shared__ uint32_t base[MAX_LOCAL];
-    __shared__ uint32_t part[BIN_WAVES];
-    __shared__ uint32_t before;
+    uint32_t *piece = lds, *from = lds + slices;          // where a slice's piece begins in the bucket, and in the slice's list
+    uint32_t *seen = from + slices, *base = seen + (WAVES << shift);
+    __shared__ uint32_t part[WAVES];
+    __shared__ uint32_t ahead[WAVES];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, bucket = blockIdx.x;
     const int rows = 1 << shift;
-    if (tid == 0) before = 0;
-    __syncthreads();
-    uint32_t ahead = 0;
-    for (int s = tid; s < slices; s += BIN_THREADS) {
+    uint32_t *at = seen + (wave << shift);
+    uint32_t mine = 0;
+    for (int s = tid; s < slices; s += SORT_THREADS) {
         const uint32_t *st = starts + (long)s * (buckets + 1) + bucket;
         const uint32_t b = st[0];
-        ahead += b;
+        mine += b;
+        from[s] = b;
         piece[s] = st[1] - b;
     }
-    if (ahead) atomicAdd(&before, ahead);
-    for (int i = tid; i < rows; i += BIN_THREADS) base[i] = 0;
+    for (int i = lane; i < rows; i += 64) at[i] = 0;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) mine += __shfl_xor(mine, o);
+    if (lane == 0) ahead[wave] = mine;
     __syncthreads();
-    const uint32_t total = block_scan(piece, slices, part);
-    if (tid == 0) piece[slices] = total;
-    __syncthreads();
-    const uint32_t start = before;
-    // the item at position i of the bucket: the slice whose piece holds it
-    auto item = [&](uint32_t i) {
-        int lo = 0, hi = slices;                 // piece[lo] <= i < piece[hi]
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (piece[mid] <= i) lo = mid; else hi = mid;
+    const uint32_t total = block_scan<SORT_THREADS>(piece, slices, part);
+    uint32_t start = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) start += ahead[w];
+    // the items at positions i0 + 64 r of the bucket below `end`: the slice whose piece holds each, by halving, all of them abreast (one after another they
+    // would be six to nine dependent reads each)
+    auto items = [&](uint32_t i0, uint32_t end, uint2 (&it)[U]) {
+        int lo[U];
+#pragma unroll
+        for (int r = 0; r < U; ++r) lo[r] = 0;
+        for (int h = half; h > 0; h >>= 1) {
+#pragma unroll
+            for (int r = 0; r < U; ++r) {
+                const int m = lo[r] + h;
+                if (m < slices && piece[m] <= i0 + 64 * r) lo[r] = m;
+            }
         }
-        return list[(long)lo * slice_tokens + starts[(long)lo * (buckets + 1) + bucket] + (i - piece[lo])];
+#pragma unroll
+        for (int r = 0; r < U; ++r) {
+            it[r] = make_uint2(NONE, 0u);
+            const uint32_t i = i0 + 64 * r;
+            if (i < end) it[r] = list[(long)lo[r] * slice_tokens + from[lo[r]] + (i - piece[lo[r]])];
+        }
     };
-    for (uint32_t i = tid; i < total; i += BIN_THREADS) atomicAdd(&base[item(i).x], 1u);
+    const uint32_t per = (total + SORT_THREADS - 1) / SORT_THREADS * 64, first = wave * per, end = min(total, first + per);
+    uint2 it[U];
+    for (uint32_t i = first; i < end; i += 64 * U) {
+        items(i + lane, end, it);
+#pragma unroll
+        for (int r = 0; r < U; ++r) {
+            if (i + 64 * r >= end) break;
+            const uint64_t same = same_digit(it[r].x, shift, it[r].x != NONE);
+            if (it[r].x != NONE && (same >> lane) == 1ull) atomicAdd(&at[it[r].x], (uint32_t)__popcll(same));      // (one lane: nothing waits for it)
+        }
+    }
     __syncthreads();
-    block_scan(base, rows, part);
+    tile_counts<WAVES>(seen, rows, rows, base);
+    block_scan<SORT_THREADS>(base, rows, part);
     const long v0 = (long)bucket << shift;
-    for (int i = tid; i < rows; i += BIN_THREADS)
+    for (int i = tid; i < rows; i += SORT_THREADS)
         if (v0 + i < V) row_start[v0 + i] = start + base[i];
     if (bucket == buckets - 1 && tid == 0) row_start[V] = start + total;
-    for (uint32_t t0 = 0; t0 < total; t0 += BIN_TILE) {
-        for (int i = lane; i < rows; i += 64) at[wave][i] = 0;
-        __syncthreads();
-        uint32_t digit[BIN_ROUNDS], tok[BIN_ROUNDS], rank[BIN_ROUNDS];
-        bool live[BIN_ROUNDS];
+    tile_places<WAVES>(seen, rows, rows, base);
+    for (uint32_t i = first; i < end; i += 64 * U) {
+        if (end - first > 64 * U) items(i + lane, end, it);       // up to U rounds are still here
 #pragma unroll
-        for (int r = 0; r < BIN_ROUNDS; ++r) {
-            const uint32_t i = t0 + wave * (64 * BIN_ROUNDS) + r * 64 + lane;
-            live[r] = i < total;
-            uint2 it = make_uint2(0u, 0u);
-            if (live[r]) it = item(i);
-            digit[r] = it.x;
-            tok[r] = it.y;
-        }
-        wave_ranks<BIN_ROUNDS>(digit, live, bits, at[wave], rank);
-        __syncthreads();
-        for (int i = tid; i < rows; i += BIN_THREADS) {
-            uint32_t b = base[i];
-#pragma unroll
-            for (int w = 0; w < BIN_WAVES; ++w) {
-                const uint32_t c = at[w][i];
-                at[w][i] = b;
-                b += c;
+        for (int r = 0; r < U; ++r) {
+            if (i + 64 * r >= end) break;
+            const uint32_t digit = it[r].x;
+            const bool live = digit != NONE;
+            const uint64_t same = same_digit(digit, shift, live);
+            uint32_t met = 0;
+            if (live) met = at[digit];
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            if (live && (same >> lane) == 1ull) at[digit] = met + (uint32_t)__popcll(same);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            if (live) {
+                const uint32_t pos = start + met + (uint32_t)__popcll(same & ((1ull << lane) - 1)), in = pos & ((1u << chunk_bits) - 1);
+                order[pos] = it[r].y;
+                if (in == 0) edge[2 * (pos >> chunk_bits)] = (uint32_t)v0 + digit;
+                if (in == (1u << chunk_bits) - 1) edge[2 * (pos >> chunk_bits) + 1] = (uint32_t)v0 + digit;
             }
-            base[i] = b;
         }
-        __syncthreads();
-#pragma unroll
-        for (int r = 0; r < BIN_ROUNDS; ++r) {
-            if (!live[r]) continue;
-            const uint32_t pos = start + at[wave][digit[r]] + rank[r], in = pos & ((1u << chunk_bits) - 1);
-            order[pos] = tok[r];
-            if (in == 0) edge[2 * (pos >> chunk_bits)] = (uint32_t)v0 + digit[r];
-            if (in == (1u << chunk_bits) - 1) edge[2 * (pos >> chunk_bits) + 1] = (uint32_t)v0 + digit[r];
-        }
-        __syncthreads();
     }
 }
 
 // ---- gradient: the sums ---------------------------------------------------------------------------------------------------------------------
 
-// sum of g over the sorted positions [lo, hi) at columns c .. c + VEC
+// Sum of g over the sorted positions [lo, hi) at columns c .. c + VEC.  Eight rows of g in flight, the next eight tokens' numbers fetched behind them: what a
+// row takes are its trips to memory.  The last ones in pieces of four, two and one, so that a short row (four tokens, at a codebook's sizes) loads no more than it has.
 template <typename TG, int VEC>
 __device__ __forceinline__ void sum_rows(const TG *__restrict__ g, const uint32_t *__restrict__ order, uint32_t lo, uint32_t hi, int D, int c, float (&acc)[VEC]) {
+    constexpr int U = 8;
 #pragma unroll
     for (int j = 0; j < VEC; ++j) acc[j] = 0.0f;
+    if (lo >= hi) return;
+    const uint32_t last = hi - 1;
+    uint32_t n[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k) n[k] = order[min(lo + k, last)];
     uint32_t i = lo;
-    for (; i + 4 <= hi; i += 4) {
-        float a[4][VEC];
+    for (; i + U <= hi; i += U) {
+        float a[U][VEC];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) load_vec<TG, VEC>(g + (long)order[i + k] * D + c, a[k]);
+        for (int k = 0; k < U; ++k) load_vec<TG, VEC>(g + (long)n[k] * D + c, a[k]);
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
+        for (int k = 0; k < U; ++k) n[k] = order[min(i + U + k, last)];
+#pragma unroll
+        for (int k = 0; k < U; ++k)
 #pragma unroll
             for (int j = 0; j < VEC; ++j) acc[j] += a[k][j];
     }
-    for (; i < hi; ++i) {
-        float a[VEC];
-        load_vec<TG, VEC>(g + (long)order[i] * D + c, a);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) acc[j] += a[j];
+    const uint32_t left = hi - i;
+#define XQ_PIECE(COUNT, FROM)                                                                                     \
+    {                                                                                                             \
+        float a[COUNT][VEC];                                                                                      \
+        _Pragma("unroll") for (int k = 0; k < COUNT; ++k) load_vec<TG, VEC>(g + (long)(FROM)[k] * D + c, a[k]);   \
+        _Pragma("unroll") for (int k = 0; k < COUNT; ++k)                                                         \
+            _Pragma("unroll") for (int j = 0; j < VEC; ++j) acc[j] += a[k][j];                                    \
     }
+    if (left & 4) {
+        XQ_PIECE(4, n)
+#pragma unroll
+        for (int k = 0; k < 3; ++k) n[k] = n[k + 4];
+    }
+    if (left & 2) {
+        XQ_PIECE(2, n)
+        n[0] = n[2];
+    }
+    if (left & 1) XQ_PIECE(1, n)
+#undef XQ_PIECE
 }
 
-// blocks [0, row_blocks): rows of at most `chunk` tokens; the others: chunk `b` of the sorted positions, pieces of longer rows -> part[b][head | tail][D]
+// Groups of `lanes` threads.  Blocks [0, row_blocks): one row of at most `chunk` tokens each; the others: pieces of longer rows, piece 2 b (+ 1) being the
+// head (tail) of chunk b of the sorted positions -> part[piece][D].
 template <typename TG, typename TW, int VEC>
 __global__ __launch_bounds__(256) void embed_sum_kernel(const TG *__restrict__ g, const uint32_t *__restrict__ order, const uint32_t *__restrict__ row_start,
-                                                        const uint32_t *__restrict__ edge, long V, int D, int lanes, float scale, uint32_t chunk, long row_blocks, TW *__restrict__ dw,
-                                                        float *__restrict__ part) {
-    const int lane = threadIdx.x % lanes, sub = threadIdx.x / lanes, rows = 256 / lanes;
-    if ((long)blockIdx.x < row_blocks) {
-        const long v = (long)blockIdx.x * rows + sub;
-        if (v >= V) return;
-        const uint32_t lo = row_start[v], hi = row_start[v + 1];
-        if (hi - lo > chunk) return;
+                                                        const uint32_t *__restrict__ edge, long V, int D, int lanes, float scale, uint32_t chunk, long chunks,
+                                                        long row_blocks, TW *__restrict__ dw, float *__restrict__ part) {
+    const int lane = threadIdx.x % lanes, sub = threadIdx.x / lanes, groups = 256 / lanes;
+    if ((long)blockIdx.x >= row_blocks) {
+        const long id = ((long)blockIdx.x - row_blocks) * groups + sub, b = id >> 1;
+        if (b >= chunks) return;
+        const uint32_t valid = row_start[V];
+        const uint64_t p0_ = (uint64_t)b * chunk;
+        if (p0_ >= valid) return;
+        const bool full = p0_ + chunk <= valid, tail = id & 1;
+        const uint32_t p0 = (uint32_t)p0_, p1 = full ? p0 + chunk : valid;
+        if (tail && !full) return;                 // a tail goes on behind its chunk's end
+        const uint32_t v = edge[2 * b + tail];
+        const uint32_t s = row_start[v], e = row_start[v + 1];
+        // a long row that began in an earlier chunk, or one that begins here and goes on behind the chunk's end
+        if (!(e - s > chunk && (tail ? s >= p0 : s < p0))) return;
+        const uint32_t lo = tail ? s : p0, hi = tail ? p1 : min(e, p1);
+        float *dst = part + id * (long)D;
         for (int c = lane * VEC; c < D; c += lanes * VEC) {
             float acc[VEC];
             sum_rows<TG, VEC>(g, order, lo, hi, D, c, acc);
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) acc[j] *= scale;
-            store_vec<TW, VEC>(dw + v * D + c, acc);
+            store_vec<float, VEC>(dst + c, acc);
         }
         return;
     }
-    const uint32_t valid = row_start[V];
-    const long b = (long)blockIdx.x - row_blocks;
-    const uint64_t p0_ = (uint64_t)b * chunk;
-    if (p0_ >= valid) return;
-    const bool full = p0_ + chunk <= valid;
-    const uint32_t p0 = (uint32_t)p0_, p1 = full ? p0 + chunk : valid;
-    const uint32_t vh = edge[2 * b], vt = full ? edge[2 * b + 1] : vh;
-    const uint32_t hs = row_start[vh], he = row_start[vh + 1], ts = row_start[vt], te = row_start[vt + 1];
-    if (sub >= 2) return;
-    // head: a long row that began in an earlier chunk; tail: one that begins here and goes on behind the chunk's end
-    uint32_t lo, hi;
-    if (sub == 0) {
-        if (!(he - hs > chunk && hs < p0)) return;
-        lo = p0; hi = min(he, p1);
-    } else {
-        if (!(full && te - ts > chunk && ts >= p0)) return;
-        lo = ts; hi = p1;
-    }
-    float *dst = part + (2 * b + sub) * (long)D;
+    const long v = (long)blockIdx.x * groups + sub;
+    if (v >= V) return;
+    const uint32_t lo = row_start[v], hi = row_start[v + 1];
+    if (hi - lo > chunk) return;
     for (int c = lane * VEC; c < D; c += lanes * VEC) {
         float acc[VEC];
         sum_rows<TG, VEC>(g, order, lo, hi, D, c, acc);
-        store_vec<float, VEC>(dst + c, acc);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) acc[j] *= scale;
+        store_vec<TW, VEC>(dw + v * D + c, acc);
     }
 }
 
-// block b: the long row that begins in chunk b (there is at most one: it goes on behind the chunk's end), its pieces in order
+// block b: the long row that begins in chunk b (there is at most one: it goes on behind the chunk's end).  Its pieces are shared out over the waves in order
+// (each a chain of its own), the waves' sums meet in order.
 template <typename TW>
-__global__ __launch_bounds__(256) void embed_long_kernel(const float *__restrict__ part, const uint32_t *__restrict__ row_start,
+__global__ __launch_bounds__(512) void embed_long_kernel(const float *__restrict__ part, const uint32_t *__restrict__ row_start,
                                                          const uint32_t *__restrict__ edge, long V, int D, float scale, uint32_t chunk,
                                                          TW *__restrict__ dw) {
+    __shared__ float sums[8][64];
     const uint32_t valid = row_start[V];
     const uint64_t p0 = (uint64_t)blockIdx.x * chunk;
     if (p0 + chunk >= valid) return;             // nothing goes on behind the last chunk
-    const long lo = edge[2 * (long)blockIdx.x + 1];
-    const uint32_t s = row_start[lo], e = row_start[lo + 1];
+    const long v = edge[2 * (long)blockIdx.x + 1];
+    const uint32_t s = row_start[v], e = row_start[v + 1];
     if (!(e - s > chunk && s >= p0)) return;
-    const long b0 = blockIdx.x, b1 = (long)((e - 1) / chunk);
-    for (int c = blockIdx.y * 256 + threadIdx.x; c < D; c += 256 * gridDim.y) {
-        float acc = part[(2 * b0 + 1) * (long)D + c];
-#pragma unroll 4
-        for (long b = b0 + 1; b <= b1; ++b) acc += part[2 * b * (long)D + c];
-        dw[lo * D + c] = from_f<TW>(acc * scale);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    // piece 0: the tail of this chunk; piece k: the head of chunk blockIdx.x + k
+    const long b0 = blockIdx.x, pieces = (long)((e - 1) / chunk) - b0 + 1, per = (pieces + 7) / 8;
+    const long k0 = wave * per, k1 = min(pieces, k0 + per);
+    for (int c0 = blockIdx.y * 64; c0 < D; c0 += 64 * gridDim.y) {
+        const int c = c0 + lane;
+        float acc = 0.0f;
+        if (c < D) {
+#pragma unroll 8
+            for (long k = k0; k < k1; ++k) acc += part[(2 * (b0 + k) + (k == 0)) * (long)D + c];
+        }
+        sums[wave][lane] = acc;
+        __syncthreads();
+        if (wave == 0 && c < D) {
+            float t = 0.0f;
+#pragma unroll
+            for (int w = 0; w < 8; ++w) t += sums[w][lane];
+            dw[v * D + c] = from_f<TW>(t * scale);
+        }
+        __syncthreads();
     }
 }
 
@@ -348,15 +450,16 @@ struct Plan {
 Plan make_plan(long N, long V, int D) {
     Plan p;
     const int bits = log2_up(V);
-    // a table of up to 256 rows: one row a bucket; above, 512 or 1024 buckets of few rows (a codebook of 16384: 1024 of 16)
-    p.shift = bits <= 8 ? 0 : std::max(bits - 10, (bits - 7) / 2);
+    // a table of up to 256 rows: one row a bucket.  Above, 256 buckets (one block of sixteen waves a CU; with 1024 buckets the second launch took 14 us
+    // instead of 7) while a bucket's counters fit a block's LDS, then 1024 of them.
+    p.shift = bits <= 8 ? 0 : bits <= 17 ? bits - 8 : bits - 10;
     p.buckets = (int)((V + (1L << p.shift) - 1) >> p.shift);
     p.bucket_bits = log2_up(p.buckets);
-    const long tiles = (N + BIN_TILE - 1) / BIN_TILE;
+    const long tiles = (N + TILE - 1) / TILE;
     p.tiles = (int)((tiles + 511) / 512);
     p.slices = (int)((tiles + p.tiles - 1) / p.tiles);
-    // pieces long enough that a row's own sum (one fp32 each) is little work, short enough that the rows' longest chain stays near the mean's cost
-    p.chunk_bits = std::max(7, log2_up((N + 2047) / 2048));
+    // 64 tokens: eight trips to memory for a row or a piece of one, and one fp32 row of partial sums written for 64 read
+    p.chunk_bits = std::max(6, log2_up((N + 4095) / 4096));
     p.chunks = (N + (1L << p.chunk_bits) - 1) >> p.chunk_bits;
     size_t off = 0;
     auto take = [&](size_t b) { size_t o = off; off = xq::align_up(off + b, 256); return o; };
@@ -378,19 +481,29 @@ int check(const char *fn, int64_t N, int64_t V, int D) {
 }
 
 template <typename TW, typename TY, typename TI>
-void launch_fwd(const void *idx, const void *w, long N, long V, int D, float scale, void *y, hipStream_t s) {
-    const bool a16 = (((uintptr_t)w | (uintptr_t)y) & 15) == 0;
-#define XQ_EMB(VEC)                                                                                                                          \
-    {                                                                                                                                        \
-        const int lanes = pow2_lanes(D, VEC);                                                                                                \
-        const long blocks = std::min<long>((N + 256 / lanes - 1) / (256 / lanes), (long)num_cus() * 32);                                     \
-        hipLaunchKernelGGL((embed_fwd_kernel<TW, TY, TI, VEC>), dim3((unsigned)blocks), dim3(256), 0, s, (const TI *)idx, (const TW *)w, N, V, D, \
-                           lanes, scale, (TY *)y);                                                                                           \
-    }
-    if (a16 && D % 8 == 0) XQ_EMB(8)
-    else if (a16 && D % 4 == 0 && sizeof(TW) == 4 && sizeof(TY) == 4) XQ_EMB(4)
-    else XQ_EMB(1)
+void launch_fwd(const void *idx_, const void *w, long N, long V, int D, float scale, void *y_, hipStream_t s) {
+    const bool a16 = (((uintptr_t)w | (uintptr_t)y_) & 15) == 0;
+    // 16 bytes of the wider side a thread: two 16-byte loads of one thread (eight fp32) lie 32 bytes apart over the wave and cost twice the lines
+    const int vec = a16 && D % 8 == 0 && sizeof(TW) == 2 && sizeof(TY) == 2 ? 8 : a16 && D % 4 == 0 ? 4 : 1;
+    // by columns where a table that one L2 does not hold is read more than once over and an eighth of a row is a 64-byte piece at least
+    const size_t table = (size_t)V * D * sizeof(TW);
+    const int split = N > 2 * V && table > (4u << 20) && table <= (32u << 20) && D % (8 * vec) == 0 && D * sizeof(TY) >= 512 ? 8 : 1;
+    const uint32_t per_row = (uint32_t)(D / vec / split);
+    const uint64_t reciprocal = per_row == 1 ? 0 : ~0ull / per_row + 1;
+    const long most = per_row > 0x40000000u ? 1 : 0x40000000L / per_row;      // rows a launch: places count in 32 bits
+    for (long n0 = 0; n0 < N; n0 += most) {
+        const long n = std::min(most, N - n0);
+        const uint32_t total = (uint32_t)(n * per_row);
+        const unsigned blocks = (total + 1023) / 1024 * split;
+        const TI *idx = (const TI *)idx_ + n0;
+        TY *y = (TY *)y_ + n0 * D;
+#define XQ_EMB(VEC) \
+    hipLaunchKernelGGL((embed_fwd_kernel<TW, TY, TI, VEC>), dim3(blocks), dim3(256), 0, s, idx, (const TW *)w, V, D, split, per_row, total, reciprocal, scale, y)
+        if (vec == 8) XQ_EMB(8);
+        else if (vec == 4) XQ_EMB(4);
+        else XQ_EMB(1);
 #undef XQ_EMB
+    }
 }
 
 template <typename TG, typename TW>
@@ -399,16 +512,16 @@ void launch_sums(const void *g, long V, int D, float scale, const Plan &p, const
     const bool a16 = (((uintptr_t)g | (uintptr_t)dw) & 15) == 0;
 #define XQ_SUM(VEC)                                                                                                                          \
     {                                                                                                                                        \
-        const int lanes = std::min(128, pow2_lanes(D, VEC));                                                                                 \
-        const long rb = (V + 256 / lanes - 1) / (256 / lanes);                                                                               \
-        hipLaunchKernelGGL((embed_sum_kernel<TG, TW, VEC>), dim3((unsigned)(rb + p.chunks)), dim3(256), 0, s, (const TG *)g, order, rows, edge, V, D, lanes, \
-                           scale, 1u << p.chunk_bits, rb, (TW *)dw, part);                                                                              \
+        const int lanes = pow2_lanes(D, VEC), groups = 256 / lanes;                                                                          \
+        const long rb = (V + groups - 1) / groups, pb = (2 * p.chunks + groups - 1) / groups;                                                \
+        hipLaunchKernelGGL((embed_sum_kernel<TG, TW, VEC>), dim3((unsigned)(rb + pb)), dim3(256), 0, s, (const TG *)g, order, rows, edge, V, D, \
+                           lanes, scale, 1u << p.chunk_bits, p.chunks, rb, (TW *)dw, part);                                                  \
     }
     if (a16 && D % 8 == 0 && sizeof(TG) == 2) XQ_SUM(8)
     else if (a16 && D % 4 == 0 && sizeof(TG) == 4) XQ_SUM(4)
     else XQ_SUM(1)
 #undef XQ_SUM
-    hipLaunchKernelGGL((embed_long_kernel<TW>), dim3((unsigned)p.chunks, (unsigned)std::min(8, (D + 255) / 256)), dim3(256), 0, s, part, rows, edge, V, D,
+    hipLaunchKernelGGL((embed_long_kernel<TW>), dim3((unsigned)p.chunks, (unsigned)std::min(8, (D + 63) / 64)), dim3(512), 0, s, part, rows, edge, V, D,
                        scale, 1u << p.chunk_bits, (TW *)dw);
 }
 
@@ -472,8 +585,13 @@ extern "C" int xq_embedding_backward(const void *idx, int idx_i64, const void *g
     else
         hipLaunchKernelGGL((embed_bin_kernel<int32_t>), dim3(p.slices), dim3(BIN_THREADS), 0, s, (const int32_t *)idx, (long)N, (long)V, (long)skip, p.shift,
                            p.buckets, p.bucket_bits, p.tiles, list, starts);
-    hipLaunchKernelGGL(embed_sort_kernel, dim3(p.buckets), dim3(BIN_THREADS), (size_t)(p.slices + 1) * 4, s, list, starts, (long)V, p.shift, p.buckets, p.shift,
-                       p.slices, (long)p.tiles * BIN_TILE, rows, order, p.chunk_bits, edge);
+#define XQ_SORT(THREADS)                                                                                                                       \
+    hipLaunchKernelGGL((embed_sort_kernel<THREADS>), dim3(p.buckets), dim3(THREADS), (size_t)p.slices * 8 + ((THREADS / 64 + 1) << p.shift) * 4, s, list, \
+                       starts, (long)V, p.shift, p.buckets, p.slices, p.slices > 1 ? 1 << (log2_up(p.slices) - 1) : 0, (long)p.tiles * TILE, rows, order, \
+                       p.chunk_bits, edge)
+    if (p.shift <= 9) XQ_SORT(1024);
+    else XQ_SORT(512);           // 1024 rows a bucket: sixteen waves' counters would not fit the 64 KB of a launch
+#undef XQ_SORT
     if (g_bf16 && dw_bf16) launch_sums<bf16, bf16>(g, V, D, scale, p, order, rows, edge, part, dw, s);
     else if (g_bf16) launch_sums<bf16, float>(g, V, D, scale, p, order, rows, edge, part, dw, s);
     else if (dw_bf16) launch_sums<float, bf16>(g, V, D, scale, p, order, rows, edge, part, dw, s);

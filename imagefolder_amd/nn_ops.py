@@ -12,6 +12,8 @@ ATen implementation of the same op (tests/test_dense_ops_gpu.py).
 import torch
 import torch.nn.functional as F
 
+from . import ops_seq
+
 # op name -> what ran last ("hip": hand-written gfx950 kernel; "library": PyTorch-ROCm op = hipBLASLt / MIOpen / ATen).
 # Filled in by the dispatchers below as they execute, so bench.py reports what the timed step actually used.
 IMPL = {}
@@ -333,7 +335,6 @@ def dropout(x, p=0.5, training=True, key=None, residual=None):
         IMPL["dropout"] = "library (CPU)"
         y = F.dropout(x, p)
         return y if residual is None else y + residual
-    from . import ops_seq
     IMPL["dropout"] = "hip"
     return ops_seq.dropout(x, p, key, residual)
 
@@ -348,6 +349,5 @@ def embedding(idx, weight, scale=1.0, padding_idx=None, dtype=None):
         y = F.embedding(idx, weight, padding_idx)
         y = y if scale == 1.0 else y * scale
         return y if dtype is None else y.to(dtype)
-    from . import ops_seq
     IMPL["embedding"] = "hip"
     return ops_seq.embedding(idx, weight, scale, padding_idx, dtype)

@@ -1,34 +1,31 @@
 """Autograd Functions over csrc/xq_drop.hip and csrc/xq_embed.hip: the operators of a token model that reads the tokenizer's codes (dropout with a
 counter-based generator, embedding with a sorted gradient).  The public entry points are nn_ops.dropout / nn_ops.embedding; everything here takes
 tensors that live on an MI355X.  Every call enqueues on the current stream of its tensors' device and allocates its outputs and workspace there."""
-import ctypes
-
 import torch
 
 from . import _lib
-from ._lib import XqError, check, ptr
+from ._lib import XqError, check
 
 _TYPES = (torch.bfloat16, torch.float32)
+_raw_stream = torch._C._cuda_getCurrentRawStream       # the handle alone: torch.cuda.current_stream builds an object, 4 us of a 5 us call
+_current_device = torch._C._cuda_getDevice
 
 
-def _stream(t):
-    return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+def _launch(name, device, *args):
+    """one C entry point on the current stream of `device`, which is made the current device only where it is not"""
+    fn = getattr(_lib.lib(), name)
+    i = device.index
+    if _current_device() == i:
+        rc = fn(*args, _raw_stream(i))
+    else:
+        with torch.cuda.device(i):
+            rc = fn(*args, _raw_stream(i))
+    if rc:
+        check(rc, name)
 
 
-def _on(t):
-    """the launching thread's current device has to be the tensors' one; entering the context costs more than a small kernel, so only where it is not"""
-    return _SAME if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
-
-
-class _Same:
-    def __enter__(self):
-        return self
-
-    def __exit__(self, *a):
-        return False
-
-
-_SAME = _Same()
+def _at(t):
+    return None if t is None else t.data_ptr()
 
 
 def _same_device(name, first, *others):
@@ -62,11 +59,8 @@ def _like(t, ref):
 
 def _dropout(x, residual, p, key, out_dtype):
     y = torch.empty_like(x, dtype=out_dtype)          # keeps the strides of a dense x
-    with _on(x):
-        rc = _lib.lib().xq_dropout(ptr(x), int(x.dtype == torch.bfloat16), ptr(residual), x.numel(), p, ptr(key), ptr(y),
-                                   int(out_dtype == torch.bfloat16), _stream(x))
-    if rc:
-        check(rc, "xq_dropout")
+    _launch("xq_dropout", x.device, x.data_ptr(), x.dtype == torch.bfloat16, _at(residual), x.numel(), p, key.data_ptr(), y.data_ptr(),
+            out_dtype == torch.bfloat16)
     return y
 
 
@@ -125,11 +119,8 @@ class EmbeddingFn(torch.autograd.Function):
         ic, w = idx.contiguous(), weight.detach().contiguous()
         V, D = w.shape
         y = torch.empty(*idx.shape, D, dtype=dtype, device=w.device)
-        with _on(w):
-            rc = _lib.lib().xq_embedding_forward(ptr(ic), int(ic.dtype == torch.int64), ptr(w), int(w.dtype == torch.bfloat16), ic.numel(), V, D, scale,
-                                                 ptr(y), int(dtype == torch.bfloat16), _stream(w))
-        if rc:
-            check(rc, "xq_embedding_forward")
+        _launch("xq_embedding_forward", w.device, ic.data_ptr(), ic.dtype == torch.int64, w.data_ptr(), w.dtype == torch.bfloat16, ic.numel(), V, D, scale,
+                y.data_ptr(), dtype == torch.bfloat16)
         if ctx.needs_input_grad[1]:
             ctx.save_for_backward(ic)
             ctx.cfg = (V, D, scale, skip, w.dtype)
@@ -141,15 +132,11 @@ class EmbeddingFn(torch.autograd.Function):
         V, D, scale, skip, wdtype = ctx.cfg
         gc = g.detach().contiguous()
         dw = torch.empty(V, D, dtype=wdtype, device=g.device)
-        l = _lib.lib()
         N = ic.numel()
-        nbytes = l.xq_embedding_backward_workspace_bytes(N, V, D)
+        nbytes = _lib.lib().xq_embedding_backward_workspace_bytes(N, V, D)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=g.device) if nbytes else None
-        with _on(gc):
-            rc = l.xq_embedding_backward(ptr(ic), int(ic.dtype == torch.int64), ptr(gc), int(gc.dtype == torch.bfloat16), N, V, D, scale, skip, ptr(dw),
-                                         int(wdtype == torch.bfloat16), ptr(ws), nbytes, _stream(gc))
-        if rc:
-            check(rc, "xq_embedding_backward")
+        _launch("xq_embedding_backward", gc.device, ic.data_ptr(), ic.dtype == torch.int64, gc.data_ptr(), gc.dtype == torch.bfloat16, N, V, D, scale, skip,
+                dw.data_ptr(), wdtype == torch.bfloat16, _at(ws), nbytes)
         return None, dw, None, None, None
 
 

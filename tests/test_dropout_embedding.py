@@ -273,8 +273,14 @@ def check_gradient(idx, g, V, scale, dw, skip=None):
     if skip is not None:
         ok &= i != skip
     i, g64 = i[ok], g64[ok]
-    want = torch.zeros(V, D, dtype=torch.float64, device="cuda").index_add_(0, i, g64) * scale
-    size = torch.zeros(V, D, dtype=torch.float64, device="cuda").index_add_(0, i, g64.abs()) * abs(scale)
+    # on the host: 64-bit sums of runs of the sorted tokens
+    order = np.argsort(i.cpu().numpy(), kind="stable")
+    rows, first = np.unique(i.cpu().numpy()[order], return_index=True)
+    want, size = np.zeros((V, D)), np.zeros((V, D))
+    if len(rows):
+        sorted64 = g64.cpu().numpy()[order]
+        want[rows], size[rows] = np.add.reduceat(sorted64, first), np.add.reduceat(np.abs(sorted64), first)
+    want, size = torch.from_numpy(want * scale).cuda(), torch.from_numpy(size * abs(scale)).cuda()
     count = torch.bincount(i, minlength=V).double()[:, None]
     tol = (count + 2) * 2.0 ** -24 * size + want.abs() * HALF[dw.dtype] * (1 + 2.0 ** -7) + 1e-38
     off = (dw.double() - want).abs()
