@@ -145,6 +145,11 @@ SIGNATURES = {
     "xq_embedding_backward_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int]),
     "xq_embedding_backward": (ctypes.c_int, [vp, ctypes.c_int, vp, ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_int, ctypes.c_float,
                                              ctypes.c_int64, vp, ctypes.c_int, vp, ctypes.c_size_t, vp]),
+    "xq_xattn_forward_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int] * 6),
+    "xq_xattn_forward": (ctypes.c_int, [vp, vp, vp] + [ctypes.c_int] * 6 + [c_i64p, vp, ctypes.c_int, vp, ctypes.c_float, vp, vp, vp, ctypes.c_size_t, vp]),
+    "xq_xattn_backward_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int] * 6),
+    "xq_xattn_backward": (ctypes.c_int, [vp] * 6 + [ctypes.c_int] * 6 + [c_i64p, vp, ctypes.c_int, vp, ctypes.c_float, vp, vp, vp, c_i64p, vp,
+                                                                         ctypes.c_size_t, vp]),
     "xq_prof_enable": (ctypes.c_int, [ctypes.c_int]),
     "xq_prof_collect": (ctypes.c_int, [ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_int)]),
     "xq_prof_collect_kind": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_int),

@@ -1,0 +1,813 @@
+// xq_xattn.hip — attention of one sequence to another one: queries (B, Nq, H, D), keys and values (B, Nk, Hk, D) of another length and with their own
+// strides, H = G Hk (query head h reads kv head h / G), the valid keys of a sample given by a length and / or a mask; forward and backward, bf16 MFMA with fp32
+// softmax statistics and sums (gfx950).
+//
+//   S = scale q k^T;  P = exp(S - lse) on valid keys, 0 elsewhere;  O = P v;  a sample without a valid key: O = 0, gradients 0, lse = -inf.
+//   dv = P^T dO;  delta = sum_d dO O;  dS = P (dO v^T - delta);  dq = scale dS k;  dk = scale dS^T q  (dk, dv over the G heads that share them).
+//
+// The rows of one kv head are its G Nq (query, head) pairs, query-major: shared heads fill a tile's rows like more queries do, and their sum in dk / dv is the
+// contraction over rows itself.  D is any multiple of 8 up to 128, computed in the next multiple of 32 (DT) with zeros behind it.
+//
+// Layouts (v_mfma_f32_32x32x16_bf16: A[i][k] lane = i, 8 consecutive k per lane half; B[k][j] lane = j; D[i][j] column = lane & 31, row = (r & 3) +
+// 8 (r >> 2) + 4 (lane >> 5)): the forward and the dq kernel hold one row per lane (S^T = K Q^T, P stays in registers and is the B operand of O^T = V^T P^T;
+// V^T comes from the row-major LDS tile through ds_read_b64_tr_b16), the dk / dv kernel one key per lane.
+// Masked keys are zero rows in LDS and -inf in S: what lies in memory there (infinities, NaN) reaches nothing.
+// Roundings to bf16: P and dS before their products (they are MFMA operands), the results once; everything else is fp32.
+#include "xq_common.hpp"
+#include "xq_internal.hpp"
+#include "../../include/xq_ops.h"
+#include <algorithm>
+#include <math.h>
+
+using namespace xq;
+
+namespace {
+
+typedef short bf16x8 __attribute__((ext_vector_type(8)));
+typedef short bf16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bfv2 __attribute__((ext_vector_type(2)));
+typedef float fv2 __attribute__((ext_vector_type(2)));
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+struct View {                      // a (B, N, heads, D) bf16 tensor: element strides, the last one is 1
+    short *p;
+    long sb, sn, sh;
+};
+
+struct Args {
+    View q, k, v, dq, dk, dv;
+    const short *out_in, *dout;    // (B, Nq, H, D) contiguous
+    short *out;
+    float *lse, *delta;            // (B, Hk, G Nq)
+    float *part, *stat;            // split over keys / rows: fp32 slabs [split][...], running (maximum, sum) [split][B Hk][R][2]
+    const void *lens;              // valid keys of a sample, or null
+    const unsigned char *mask;     // (B, Nk), or null
+    int lens_i64, B, Nq, Nk, H, Hk, G, D, R;
+    unsigned long long g_reciprocal;   // of G (0: one)
+    float scale;
+    int nper, groups, swizzle, splits;
+};
+
+__device__ __forceinline__ unsigned pack_bf16(float a, float b) {
+    fv2 v = {a, b};
+    bfv2 r = __builtin_convertvector(v, bfv2);   // v_cvt_pk_bf16_f32 (RNE)
+    return __builtin_bit_cast(unsigned, r);
+}
+__device__ __forceinline__ bf16x8 pack8(const float *s) {
+    uint4 u = make_uint4(pack_bf16(s[0], s[1]), pack_bf16(s[2], s[3]), pack_bf16(s[4], s[5]), pack_bf16(s[6], s[7]));
+    return __builtin_bit_cast(bf16x8, u);
+}
+__device__ __forceinline__ float bf_lo(unsigned u) { return __uint_as_float(u << 16); }
+__device__ __forceinline__ float bf_hi(unsigned u) { return __uint_as_float(u & 0xffff0000u); }
+
+typedef short s4lds __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ bf16x4 lds_tr4(const short *p) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((s4lds __attribute__((address_space(3))) *)p);
+}
+// A fragment of T^T for a row-major tile T of pitch P: contraction rows ROW0 + {4 hh .. + 3, 8 + 4 hh ..}, output rows = columns COL0 + (lane & 31);
+// the pointer carries the lane's part (trp below)
+template <int P>
+__device__ __forceinline__ bf16x8 tr_frag(const short *trp, int row0, int col0) {
+    const bf16x4 lo = lds_tr4(trp + row0 * P + col0), hi = lds_tr4(trp + (row0 + 8) * P + col0);
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// v_max3_f32 without the operand canonicalisation that fmaxf() carries under IEEE mode
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
+    return d;
+}
+
+#define XA_MFMA(A, B, C) __builtin_amdgcn_mfma_f32_32x32x16_bf16((A), (B), (C), 0, 0, 0)
+
+__device__ __forceinline__ uint32_t quotient(uint32_t a, uint64_t reciprocal) { return reciprocal ? (uint32_t)__umul64hi((uint64_t)a, reciprocal) : a; }
+
+// (b, kv head) and the tile of a block.  Where the (batch, kv head) pairs divide over the eight XCDs, the blocks of one pair share an XCD (round-robin: block id
+// mod 8), whose L2 then holds its keys and values (or rows) once; otherwise they run on in order, so that no XCD idles.
+__device__ __forceinline__ bool map_block(const Args &a, int &g, int &i) {
+    const int L = blockIdx.x;
+    if (a.swizzle) {
+        const int slot = L >> 3, gl = slot / a.nper;
+        i = slot - gl * a.nper;
+        g = gl * 8 + (L & 7);
+    } else {
+        g = L / a.nper;
+        i = L - g * a.nper;
+    }
+    return g < a.groups;
+}
+
+__device__ __forceinline__ int keys_of(const Args &a, int b) {
+    if (!a.lens) return a.Nk;
+    const long n = a.lens_i64 ? (long)((const int64_t *)a.lens)[b] : (long)((const int32_t *)a.lens)[b];
+    return (int)(n < 0 ? 0 : n > a.Nk ? a.Nk : n);
+}
+
+// the valid ones of the 64 keys from kv0, one bit each (the same in every lane)
+__device__ __forceinline__ uint64_t valid_bits(const Args &a, const unsigned char *mask_row, int len, int kv0) {
+    const int left = len - kv0;
+    uint64_t bits = left >= 64 ? ~0ull : left <= 0 ? 0ull : (1ull << left) - 1;
+    if (mask_row) {
+        const int key = kv0 + (int)(threadIdx.x & 63);
+        bool on = false;
+        if (key < len) on = mask_row[key] != 0;
+        bits &= __ballot(on);
+    }
+    return bits;
+}
+
+__device__ __forceinline__ uint4 zero_unless(uint4 v, bool ok) {
+    if (!ok) v = make_uint4(0u, 0u, 0u, 0u);
+    return v;
+}
+
+// element offset of row r of kv head hk in a query-sided view
+__device__ __forceinline__ long row_offset(const Args &a, const View &t, int b, int hk, int r) {
+    const uint32_t tok = quotient((uint32_t)r, a.g_reciprocal), g = (uint32_t)r - tok * a.G;
+    return b * t.sb + (long)tok * t.sn + (long)(hk * a.G + (int)g) * t.sh;
+}
+
+// 64 rows of a key-sided view into registers (CH 16-byte chunks a thread), then into the LDS tile with the invalid ones zeroed
+template <int DT, int ROWS>
+struct Stage {
+    static constexpr int PER_ROW = DT / 8, CH = ROWS * PER_ROW / 256, P = DT + 8;
+    uint4 r[CH];
+    __device__ __forceinline__ void load(const short *base, long sn, int row0, int last, int D) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int id = threadIdx.x + 256 * c, row = id / PER_ROW, part = id % PER_ROW;
+            const int n = row0 + row <= last ? row0 + row : last;
+            const uint4 x = *reinterpret_cast<const uint4 *>(base + (long)n * sn + (8 * part < D ? 8 * part : 0));
+            r[c] = zero_unless(x, 8 * part < D);
+        }
+    }
+    __device__ __forceinline__ void store(short *tile, uint64_t bits) const {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int id = threadIdx.x + 256 * c, row = id / PER_ROW, part = id % PER_ROW;
+            *reinterpret_cast<uint4 *>(tile + row * P + 8 * part) = zero_unless(r[c], (bits >> row) & 1);
+        }
+    }
+};
+
+// one lane's 8-element chunks of a row: the B operand over the head dimension
+template <int DT>
+__device__ __forceinline__ void load_row(const short *row, int D, int hh, bf16x8 (&f)[DT / 16]) {
+#pragma unroll
+    for (int s = 0; s < DT / 16; ++s) {
+        const int col = 16 * s + 8 * hh;
+        const uint4 x = *reinterpret_cast<const uint4 *>(row + (col < D ? col : 0));
+        f[s] = __builtin_bit_cast(bf16x8, zero_unless(x, col < D));
+    }
+}
+
+// a lane's column of an (output row, lane) accumulator block, rounded: 16 bytes a lane, the lane halves exchanging register quads.  Every lane takes part.
+template <int DT>
+__device__ __forceinline__ void store_row(short *row, int D, int hh, const f32x16 (&acc)[DT / 32], float factor, bool ok) {
+#pragma unroll
+    for (int t = 0; t < DT / 32; ++t)
+#pragma unroll
+        for (int q = 0; q < 4; q += 2) {
+            const uint2 x = make_uint2(pack_bf16(acc[t][4 * q] * factor, acc[t][4 * q + 1] * factor), pack_bf16(acc[t][4 * q + 2] * factor, acc[t][4 * q + 3] * factor));
+            const uint2 y = make_uint2(pack_bf16(acc[t][4 * q + 4] * factor, acc[t][4 * q + 5] * factor),
+                                       pack_bf16(acc[t][4 * q + 6] * factor, acc[t][4 * q + 7] * factor));
+            const auto e = __builtin_amdgcn_permlane32_swap(x.x, y.x, false, false);
+            const auto f = __builtin_amdgcn_permlane32_swap(x.y, y.y, false, false);
+            const int col = 32 * t + 8 * q + 8 * hh;
+            if (ok && col < D) *reinterpret_cast<uint4 *>(row + col) = make_uint4(e[0], f[0], e[1], f[1]);
+        }
+}
+
+// the same into an fp32 slab
+template <int DT>
+__device__ __forceinline__ void store_part(float *row, int D, int hh, const f32x16 (&acc)[DT / 32], bool ok) {
+#pragma unroll
+    for (int t = 0; t < DT / 32; ++t)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int col = 32 * t + 8 * q + 4 * hh;
+            if (ok && col < D) *reinterpret_cast<float4 *>(row + col) = make_float4(acc[t][4 * q], acc[t][4 * q + 1], acc[t][4 * q + 2], acc[t][4 * q + 3]);
+        }
+}
+
+// lse in log2 units; that of a row without a finite score stands for P = 0 (exp2(-inf - 0)), not for NaN
+__device__ __forceinline__ float log2_of(float lse) { return lse == -INFINITY ? 0.0f : lse * LOG2E; }
+
+// share `part` of `parts` of n tiles
+__device__ __forceinline__ void share(int n, int part, int parts, int &from, int &to) {
+    from = (int)((long)n * part / parts);
+    to = (int)((long)n * (part + 1) / parts);
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------------------------
+// forward: 128 rows of one (sample, kv head) a block, 32 a wave; 64-key tiles of K and V in two LDS buffers
+// ---------------------------------------------------------------------------------------------------------------------------------------------
+template <int DT, bool SPLIT>
+__global__ __launch_bounds__(256, 2) void xattn_fwd_kernel(Args a) {
+    constexpr int P = DT + 8, KS = DT / 16, OT = DT / 32;
+    __shared__ __attribute__((aligned(16))) short Ks[2][64 * P];
+    __shared__ __attribute__((aligned(16))) short Vs[2][64 * P];
+    int g, i;
+    if (!map_block(a, g, i)) return;
+    const int split = SPLIT ? i % a.splits : 0, rb = SPLIT ? i / a.splits : i;
+    const int b = g / a.Hk, hk = g - b * a.Hk;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 31, hh = lane >> 5;
+    const int trp = (4 * hh + ((lane & 15) >> 2)) * P + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+    const int len = keys_of(a, b);
+    const unsigned char *mask = a.mask ? a.mask + (long)b * a.Nk : nullptr;
+    const short *kb = a.k.p + b * a.k.sb + hk * a.k.sh, *vb = a.v.p + b * a.v.sb + hk * a.v.sh;
+    const float c = a.scale * LOG2E;
+
+    const int r = rb * 128 + wave * 32 + li, rc = r < a.R ? r : a.R - 1;
+    const bool wave_live = rb * 128 + wave * 32 < a.R;
+    bf16x8 qf[KS];
+    load_row<DT>(a.q.p + row_offset(a, a.q, b, hk, rc), a.D, hh, qf);
+
+    f32x16 o[OT];
+#pragma unroll
+    for (int t = 0; t < OT; ++t)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[t][j] = 0.0f;
+    // m is the reference exponent (log2 units), moved only when a tile's maximum passes it by more than 2^8: P <= 2^8 loses nothing in bf16 / fp32, and the
+    // rescale becomes a rare branch; the row sums come from the matrix pipe (ones x P^T), of the rounded P that the product with V sees
+    float m = -INFINITY, l = 0.0f;
+    const bf16x8 ones = {0x3F80, 0x3F80, 0x3F80, 0x3F80, 0x3F80, 0x3F80, 0x3F80, 0x3F80};
+    const f32x16 zero16 = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+
+    int t0, t1;
+    share((len + 63) / 64, split, SPLIT ? a.splits : 1, t0, t1);
+    Stage<DT, 64> sk, sv;
+    uint64_t bits = 0, next = 0;
+    if (t0 < t1) {
+        bits = valid_bits(a, mask, len, t0 * 64);
+        sk.load(kb, a.k.sn, t0 * 64, a.Nk - 1, a.D);
+        sv.load(vb, a.v.sn, t0 * 64, a.Nk - 1, a.D);
+        sk.store(Ks[0], bits);
+        sv.store(Vs[0], bits);
+    }
+    __syncthreads();
+    for (int t = t0; t < t1; ++t) {
+        const int cur = (t - t0) & 1;
+        if (t + 1 < t1) {
+            next = valid_bits(a, mask, len, t * 64 + 64);
+            sk.load(kb, a.k.sn, t * 64 + 64, a.Nk - 1, a.D);
+            sv.load(vb, a.v.sn, t * 64 + 64, a.Nk - 1, a.D);
+        }
+        if (wave_live && bits) {
+            const short *K = Ks[cur] + li * P + 8 * hh, *V = Vs[cur] + trp;
+            f32x16 s[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                s[h] = zero16;
+#pragma unroll
+                for (int k = 0; k < KS; ++k) s[h] = XA_MFMA(*reinterpret_cast<const bf16x8 *>(K + 32 * h * P + 16 * k), qf[k], s[h]);
+            }
+            if (~bits) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t w = (uint32_t)(bits >> (32 * h)) >> (4 * hh);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j)
+                        if (!((w >> ((j & 3) + 8 * (j >> 2))) & 1u)) s[h][j] = -INFINITY;
+                }
+            }
+            float mx = max3(s[0][0], s[0][1], s[0][2]);
+#pragma unroll
+            for (int j = 3; j < 15; j += 2) mx = max3(mx, s[0][j], s[0][j + 1]);
+            mx = max3(mx, s[0][15], s[1][0]);
+#pragma unroll
+            for (int j = 1; j < 15; j += 2) mx = max3(mx, s[1][j], s[1][j + 1]);
+            mx = max3(mx, s[1][15], s[1][15]);
+            mx = max3(mx, __shfl_xor(mx, 32), mx);
+            const float cand = mx * c;
+            if (__any(cand > m + 8.0f)) {
+                const float mn = fmaxf(m, cand);
+                const float alpha = m == mn ? 1.0f : __builtin_amdgcn_exp2f(m - mn);      // (a row without a key so far: m = mn = -inf)
+                m = mn;
+                l *= alpha;
+#pragma unroll
+                for (int q = 0; q < OT; ++q)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) o[q][j] *= alpha;
+            }
+            const float mref = m == -INFINITY ? 0.0f : m;      // (every score so far -inf: P is 0, not NaN)
+            f32x16 ls = zero16;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float p[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) p[j] = __builtin_amdgcn_exp2f(fmaf(s[h][j], c, -mref));
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const bf16x8 pk = pack8(p + 8 * k);
+#pragma unroll
+                    for (int q = 0; q < OT; ++q) o[q] = XA_MFMA(tr_frag<P>(V, 32 * h + 16 * k, 32 * q), pk, o[q]);
+                    ls = XA_MFMA(ones, pk, ls);
+                }
+            }
+            l += ls[0];            // every row of ones x P^T is the sum over the tile's keys of this lane's row
+        }
+        if (t + 1 < t1) {
+            sk.store(Ks[cur ^ 1], next);
+            sv.store(Vs[cur ^ 1], next);
+            bits = next;
+        }
+        __syncthreads();
+    }
+    const bool ok = r < a.R;
+    if (SPLIT) {
+        const long slot = ((long)split * a.groups + g) * a.R + (ok ? r : 0);
+        store_part<DT>(a.part + slot * a.D, a.D, hh, o, ok);
+        if (ok && hh == 0) *reinterpret_cast<float2 *>(a.stat + 2 * slot) = make_float2(m, l);
+    } else {
+        const uint32_t tok = quotient((uint32_t)rc, a.g_reciprocal), gg = (uint32_t)rc - tok * a.G;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        store_row<DT>(a.out + (((long)b * a.Nq + tok) * a.H + hk * a.G + gg) * a.D, a.D, hh, o, inv, ok);
+        if (a.lse && ok && hh == 0) a.lse[(long)g * a.R + r] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * LN2;
+    }
+}
+
+// the slabs of a split over keys: O = sum_s w_s O_s / sum_s w_s l_s, w_s = 2^(m_s - max m); four columns a thread
+__global__ __launch_bounds__(256) void xattn_join_kernel(Args a, int per_row, unsigned long long row_reciprocal, long total) {
+    const long id = (long)blockIdx.x * 256 + threadIdx.x;
+    if (id >= total) return;
+    const uint32_t row = quotient((uint32_t)id, row_reciprocal);          // g R + r (the host keeps total below 2^32)
+    const int col = ((uint32_t)id - row * per_row) * 4;
+    const long rows = (long)a.groups * a.R;
+    float M = -INFINITY;
+    for (int s = 0; s < a.splits; ++s) M = fmaxf(M, a.stat[2 * (s * rows + row)]);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    float l = 0.0f;
+#pragma unroll 4
+    for (int s = 0; s < a.splits; ++s) {
+        const float2 ml = *reinterpret_cast<const float2 *>(a.stat + 2 * (s * rows + row));
+        const float4 x = *reinterpret_cast<const float4 *>(a.part + (s * rows + row) * a.D + col);
+        const float w = ml.x == M ? 1.0f : __builtin_amdgcn_exp2f(ml.x - M);
+        l = fmaf(ml.y, w, l);
+        o.x = fmaf(x.x, w, o.x); o.y = fmaf(x.y, w, o.y); o.z = fmaf(x.z, w, o.z); o.w = fmaf(x.w, w, o.w);
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const int g = row / a.R, r = row - (long)g * a.R, b = g / a.Hk, hk = g - b * a.Hk;
+    const uint32_t tok = quotient((uint32_t)r, a.g_reciprocal), gg = (uint32_t)r - tok * a.G;
+    *reinterpret_cast<uint2 *>(a.out + (((long)b * a.Nq + tok) * a.H + hk * a.G + gg) * a.D + col) =
+        make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+    if (a.lse && col == 0) a.lse[row] = l == 0.0f ? -INFINITY : (M + __builtin_amdgcn_logf(l)) * LN2;
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------------------------
+// dq: one row per lane as the forward; delta in the prologue, written for the dk / dv kernel behind it
+// ---------------------------------------------------------------------------------------------------------------------------------------------
+template <int DT, bool SPLIT>
+__global__ __launch_bounds__(256, DT > 64 ? 1 : 2) void xattn_dq_kernel(Args a) {
+    constexpr int P = DT + 8, KS = DT / 16, OT = DT / 32;
+    __shared__ __attribute__((aligned(16))) short Ks[2][64 * P];
+    __shared__ __attribute__((aligned(16))) short Vs[2][64 * P];
+    int g, i;
+    if (!map_block(a, g, i)) return;
+    const int split = SPLIT ? i % a.splits : 0, rb = SPLIT ? i / a.splits : i;
+    const int b = g / a.Hk, hk = g - b * a.Hk;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 31, hh = lane >> 5;
+    const int trp = (4 * hh + ((lane & 15) >> 2)) * P + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+    const int len = keys_of(a, b);
+    const unsigned char *mask = a.mask ? a.mask + (long)b * a.Nk : nullptr;
+    const short *kb = a.k.p + b * a.k.sb + hk * a.k.sh, *vb = a.v.p + b * a.v.sb + hk * a.v.sh;
+    const float c = a.scale * LOG2E;
+
+    const int r = rb * 128 + wave * 32 + li, rc = r < a.R ? r : a.R - 1;
+    const bool wave_live = rb * 128 + wave * 32 < a.R, ok = r < a.R;
+    bf16x8 qf[KS], df[KS];
+    load_row<DT>(a.q.p + row_offset(a, a.q, b, hk, rc), a.D, hh, qf);
+    const uint32_t tok = quotient((uint32_t)rc, a.g_reciprocal), gg = (uint32_t)rc - tok * a.G;
+    const long orow = (((long)b * a.Nq + tok) * a.H + hk * a.G + gg) * a.D;
+    load_row<DT>(a.dout + orow, a.D, hh, df);
+    float delta = 0.0f;
+    {
+        bf16x8 of[KS];
+        load_row<DT>(a.out_in + orow, a.D, hh, of);
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            const uint4 x = __builtin_bit_cast(uint4, of[k]), y = __builtin_bit_cast(uint4, df[k]);
+            delta = fmaf(bf_lo(x.x), bf_lo(y.x), delta); delta = fmaf(bf_hi(x.x), bf_hi(y.x), delta);
+            delta = fmaf(bf_lo(x.y), bf_lo(y.y), delta); delta = fmaf(bf_hi(x.y), bf_hi(y.y), delta);
+            delta = fmaf(bf_lo(x.z), bf_lo(y.z), delta); delta = fmaf(bf_hi(x.z), bf_hi(y.z), delta);
+            delta = fmaf(bf_lo(x.w), bf_lo(y.w), delta); delta = fmaf(bf_hi(x.w), bf_hi(y.w), delta);
+        }
+        delta += __shfl_xor(delta, 32);
+        if (hh == 0 && ok && split == 0) a.delta[(long)g * a.R + r] = delta;
+    }
+    const float lse2 = log2_of(a.lse[(long)g * a.R + rc]);
+
+    f32x16 acc[OT];
+#pragma unroll
+    for (int t = 0; t < OT; ++t)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) acc[t][j] = 0.0f;
+
+    int t0, t1;
+    share((len + 63) / 64, split, SPLIT ? a.splits : 1, t0, t1);
+    Stage<DT, 64> sk, sv;
+    uint64_t bits = 0, next = 0;
+    if (t0 < t1) {
+        bits = valid_bits(a, mask, len, t0 * 64);
+        sk.load(kb, a.k.sn, t0 * 64, a.Nk - 1, a.D);
+        sv.load(vb, a.v.sn, t0 * 64, a.Nk - 1, a.D);
+        sk.store(Ks[0], bits);
+        sv.store(Vs[0], bits);
+    }
+    __syncthreads();
+    for (int t = t0; t < t1; ++t) {
+        const int cur = (t - t0) & 1;
+        if (t + 1 < t1) {
+            next = valid_bits(a, mask, len, t * 64 + 64);
+            sk.load(kb, a.k.sn, t * 64 + 64, a.Nk - 1, a.D);
+            sv.load(vb, a.v.sn, t * 64 + 64, a.Nk - 1, a.D);
+        }
+        if (wave_live && bits) {
+            const short *K = Ks[cur] + li * P + 8 * hh, *V = Vs[cur] + li * P + 8 * hh, *T = Ks[cur] + trp;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                f32x16 s, p;
+#pragma unroll
+                for (int j = 0; j < 16; ++j) { s[j] = 0.0f; p[j] = 0.0f; }
+#pragma unroll
+                for (int k = 0; k < KS; ++k) {
+                    s = XA_MFMA(*reinterpret_cast<const bf16x8 *>(K + 32 * h * P + 16 * k), qf[k], s);
+                    p = XA_MFMA(*reinterpret_cast<const bf16x8 *>(V + 32 * h * P + 16 * k), df[k], p);
+                }
+                const uint32_t w = (uint32_t)(bits >> (32 * h)) >> (4 * hh);
+                float d[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) d[j] = __builtin_amdgcn_exp2f(fmaf(s[j], c, -lse2)) * (p[j] - delta);      // scale: once, in the end
+                if (~bits) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j)
+                        if (!((w >> ((j & 3) + 8 * (j >> 2))) & 1u)) d[j] = 0.0f;
+                }
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const bf16x8 dk = pack8(d + 8 * k);
+#pragma unroll
+                    for (int q = 0; q < OT; ++q) acc[q] = XA_MFMA(tr_frag<P>(T, 32 * h + 16 * k, 32 * q), dk, acc[q]);
+                }
+            }
+        }
+        if (t + 1 < t1) {
+            sk.store(Ks[cur ^ 1], next);
+            sv.store(Vs[cur ^ 1], next);
+            bits = next;
+        }
+        __syncthreads();
+    }
+    if (SPLIT) {
+        const long slot = ((long)split * a.groups + g) * a.R + (ok ? r : 0);
+        store_part<DT>(a.part + slot * a.D, a.D, hh, acc, ok);
+    } else {
+        store_row<DT>(a.dq.p + row_offset(a, a.dq, b, hk, rc), a.D, hh, acc, a.scale, ok);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------------------------
+// dk, dv: one key per lane, 128 keys of one (sample, kv head) a block; 32-row tiles of q and dO (and lse, delta) in two LDS buffers
+// ---------------------------------------------------------------------------------------------------------------------------------------------
+template <int DT, bool SPLIT>
+__global__ __launch_bounds__(256, DT > 64 ? 1 : 2) void xattn_dkdv_kernel(Args a) {
+    constexpr int P = DT + 8, KS = DT / 16, OT = DT / 32, PER_ROW = DT / 8, CH = (32 * PER_ROW + 255) / 256;
+    __shared__ __attribute__((aligned(16))) short Qs[2][32 * P];
+    __shared__ __attribute__((aligned(16))) short Os[2][32 * P];
+    __shared__ __attribute__((aligned(16))) float Ls[2][32];
+    __shared__ __attribute__((aligned(16))) float Ds[2][32];
+    int g, i;
+    if (!map_block(a, g, i)) return;
+    const int split = SPLIT ? i % a.splits : 0, kbk = SPLIT ? i / a.splits : i;
+    const int b = g / a.Hk, hk = g - b * a.Hk;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, hh = lane >> 5;
+    const int trp = (4 * hh + ((lane & 15) >> 2)) * P + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+    const int len = keys_of(a, b);
+    const float c = a.scale * LOG2E;
+    const float *lse = a.lse + (long)g * a.R, *dlt = a.delta + (long)g * a.R;
+
+    const int n = kbk * 128 + wave * 32 + li, nc = n < a.Nk ? n : a.Nk - 1;
+    bool valid = n < len;
+    if (a.mask && valid) valid = a.mask[(long)b * a.Nk + n] != 0;
+    const bool wave_live = __any(valid);      // a wave without a valid key only helps to stage
+    bf16x8 kf[KS], vf[KS];
+    load_row<DT>(a.k.p + b * a.k.sb + hk * a.k.sh + (long)nc * a.k.sn, a.D, hh, kf);
+    load_row<DT>(a.v.p + b * a.v.sb + hk * a.v.sh + (long)nc * a.v.sn, a.D, hh, vf);
+
+    f32x16 dk[OT], dv[OT];
+#pragma unroll
+    for (int t = 0; t < OT; ++t)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) { dk[t][j] = 0.0f; dv[t][j] = 0.0f; }
+
+    uint4 rq[CH], ro[CH];
+    float rl = 0.0f;
+    auto load = [&](int r0) {
+#pragma unroll
+        for (int ch = 0; ch < CH; ++ch) {
+            const int id = tid + 256 * ch, row = id / PER_ROW, part = id % PER_ROW;
+            const int r = r0 + row;
+            const bool ok = row < 32 && r < a.R && 8 * part < a.D;
+            const int rr = ok ? r : 0, col = ok ? 8 * part : 0;
+            const uint32_t tok = quotient((uint32_t)rr, a.g_reciprocal), gg = (uint32_t)rr - tok * a.G;
+            rq[ch] = zero_unless(*reinterpret_cast<const uint4 *>(a.q.p + row_offset(a, a.q, b, hk, rr) + col), ok);
+            ro[ch] = zero_unless(*reinterpret_cast<const uint4 *>(a.dout + (((long)b * a.Nq + tok) * a.H + hk * a.G + gg) * a.D + col), ok);
+        }
+        if (tid < 64) {
+            const int r = r0 + li;
+            rl = r < a.R ? (hh == 0 ? log2_of(lse[r]) : dlt[r]) : 0.0f;
+        }
+    };
+    auto store = [&](int buf) {
+#pragma unroll
+        for (int ch = 0; ch < CH; ++ch) {
+            const int id = tid + 256 * ch, row = id / PER_ROW, part = id % PER_ROW;
+            if (row < 32) {
+                *reinterpret_cast<uint4 *>(Qs[buf] + row * P + 8 * part) = rq[ch];
+                *reinterpret_cast<uint4 *>(Os[buf] + row * P + 8 * part) = ro[ch];
+            }
+        }
+        if (tid < 32) Ls[buf][li] = rl;
+        else if (tid < 64) Ds[buf][li] = rl;
+    };
+
+    int t0, t1;
+    share(kbk * 128 < len ? (a.R + 31) / 32 : 0, split, SPLIT ? a.splits : 1, t0, t1);
+    if (t0 < t1) {
+        load(t0 * 32);
+        store(0);
+    }
+    __syncthreads();
+    for (int t = t0; t < t1; ++t) {
+        const int cur = (t - t0) & 1;
+        if (t + 1 < t1) load(t * 32 + 32);
+        if (wave_live) {
+            const short *Q = Qs[cur] + li * P + 8 * hh, *O = Os[cur] + li * P + 8 * hh;
+            f32x16 s, p;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) { s[j] = 0.0f; p[j] = 0.0f; }
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                s = XA_MFMA(*reinterpret_cast<const bf16x8 *>(Q + 16 * k), kf[k], s);
+                p = XA_MFMA(*reinterpret_cast<const bf16x8 *>(O + 16 * k), vf[k], p);
+            }
+            // register j <-> row (j & 3) + 8 (j >> 2) + 4 hh of the tile; rows behind the last have q = dO = 0 and lse = delta = 0: P is 1 there, dS 0
+            float e[16], d[16];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const float4 l4 = *reinterpret_cast<const float4 *>(&Ls[cur][8 * q + 4 * hh]);
+                const float4 d4 = *reinterpret_cast<const float4 *>(&Ds[cur][8 * q + 4 * hh]);
+                const float lv[4] = {l4.x, l4.y, l4.z, l4.w}, dl[4] = {d4.x, d4.y, d4.z, d4.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    e[4 * q + j] = __builtin_amdgcn_exp2f(fmaf(s[4 * q + j], c, -lv[j]));
+                    d[4 * q + j] = e[4 * q + j] * (p[4 * q + j] - dl[j]);
+                }
+            }
+            const short *ot = Os[cur] + trp, *qt = Qs[cur] + trp;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const bf16x8 pb = pack8(e + 8 * k), db = pack8(d + 8 * k);
+#pragma unroll
+                for (int q = 0; q < OT; ++q) {
+                    dv[q] = XA_MFMA(tr_frag<P>(ot, 16 * k, 32 * q), pb, dv[q]);
+                    dk[q] = XA_MFMA(tr_frag<P>(qt, 16 * k, 32 * q), db, dk[q]);
+                }
+            }
+        }
+        if (t + 1 < t1) store(cur ^ 1);
+        __syncthreads();
+    }
+    // a masked key's column holds what its bytes gave: zero goes out for it
+    if (!valid) {
+#pragma unroll
+        for (int t = 0; t < OT; ++t)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) { dk[t][j] = 0.0f; dv[t][j] = 0.0f; }
+    }
+    const bool ok = n < a.Nk;
+    if (SPLIT) {
+        const long slots = (long)a.groups * a.Nk, slot = (long)g * a.Nk + nc;
+        float *pk = a.part + (2 * split * slots + slot) * a.D, *pv = a.part + ((2 * split + 1) * slots + slot) * a.D;
+        store_part<DT>(pk, a.D, hh, dk, ok);
+        store_part<DT>(pv, a.D, hh, dv, ok);
+    } else {
+        store_row<DT>(a.dk.p + b * a.dk.sb + hk * a.dk.sh + (long)nc * a.dk.sn, a.D, hh, dk, a.scale, ok);
+        store_row<DT>(a.dv.p + b * a.dv.sb + hk * a.dv.sh + (long)nc * a.dv.sn, a.D, hh, dv, 1.0f, ok);
+    }
+}
+
+// slabs of a split gradient, added in order: KIND 0 dq rows (g R + r), 1 dk and dv keys (2 x (g Nk + n)); four columns a thread
+template <int KIND>
+__global__ __launch_bounds__(256) void xattn_sum_kernel(Args a, int per_row, unsigned long long row_reciprocal, long total) {
+    const long id = (long)blockIdx.x * 256 + threadIdx.x;
+    if (id >= total) return;
+    const uint32_t row = quotient((uint32_t)id, row_reciprocal);
+    const int col = ((uint32_t)id - row * per_row) * 4;
+    const long rows = KIND == 0 ? (long)a.groups * a.R : 2L * a.groups * a.Nk;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int s = 0; s < a.splits; ++s) {
+        const float4 y = *reinterpret_cast<const float4 *>(a.part + (s * rows + row) * a.D + col);
+        x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+    }
+    short *dst;
+    float f = a.scale;
+    if (KIND == 0) {
+        const int g = row / a.R, b = g / a.Hk;
+        dst = a.dq.p + row_offset(a, a.dq, b, g - b * a.Hk, row - (long)g * a.R);
+    } else {
+        const long key = row < (uint32_t)(a.groups * (long)a.Nk) ? row : row - (long)a.groups * a.Nk;
+        const View &t = key == row ? a.dk : a.dv;
+        if (key != row) f = 1.0f;
+        const int g = (int)(key / a.Nk), b = g / a.Hk;
+        dst = t.p + b * t.sb + (g - b * a.Hk) * t.sh + (key - (long)g * a.Nk) * t.sn;
+    }
+    *reinterpret_cast<uint2 *>(dst + col) = make_uint2(pack_bf16(x.x * f, x.y * f), pack_bf16(x.z * f, x.w * f));
+}
+
+// ---- host -----------------------------------------------------------------------------------------------------------------------------------
+
+unsigned long long reciprocal_of(long d) { return d <= 1 ? 0 : ~0ull / (unsigned long long)d + 1; }
+
+// blocks of `tile` rows (or keys) for each (sample, kv head)
+long tiles_of(long n, int tile) { return (n + tile - 1) / tile; }
+
+// shares of the contracted axis (`steps` tiles long) so that about two blocks run on every CU; a share has at least `least` tiles
+int splits_for(long blocks, long steps, int least) {
+    const long want = 2L * num_cus();
+    if (blocks >= want || steps < 2 * least) return 1;
+    return (int)std::max<long>(1, std::min(steps / least, (want + blocks - 1) / blocks));
+}
+
+struct Sizes {
+    long groups, R;
+    int fwd_splits, dq_splits, kv_splits;
+    size_t fwd_part, fwd_bytes, delta_bytes, bwd_bytes;
+};
+
+Sizes sizes_of(int B, int Nq, int Nk, int H, int Hk, int D) {
+    Sizes z;
+    z.groups = (long)B * Hk;
+    z.R = (long)Nq * (H / Hk);
+    const long rb = z.groups * tiles_of(z.R, 128), kb = z.groups * tiles_of(Nk, 128);
+    z.fwd_splits = splits_for(rb, tiles_of(Nk, 64), 4);
+    z.dq_splits = splits_for(rb, tiles_of(Nk, 64), 4);
+    z.kv_splits = splits_for(kb, tiles_of(z.R, 32), 8);
+    const size_t rows = (size_t)z.groups * z.R;
+    z.fwd_part = align_up(z.fwd_splits > 1 ? rows * z.fwd_splits * D * 4 : 0, 256);
+    z.fwd_bytes = z.fwd_splits > 1 ? z.fwd_part + rows * z.fwd_splits * 8 : 0;
+    z.delta_bytes = align_up(rows * 4, 256);
+    const size_t dq = z.dq_splits > 1 ? rows * z.dq_splits * D * 4 : 0, kv = z.kv_splits > 1 ? 2 * (size_t)z.groups * Nk * z.kv_splits * D * 4 : 0;
+    z.bwd_bytes = z.delta_bytes + std::max(dq, kv);
+    return z;
+}
+
+int check_sizes(const char *fn, int B, int Nq, int Nk, int H, int Hk, int D, float scale) {
+    if (B < 0 || Nq < 0 || Nk < 0 || H < 1 || Hk < 1) return xq_set_error(XQ_EINVAL, "%s: bad sizes (H=%ld, Hk=%ld)", fn, (long)H, (long)Hk);
+    if (H % Hk) return xq_set_error(XQ_EINVAL, "%s: %ld query heads do not share %ld kv heads evenly", fn, (long)H, (long)Hk);
+    if (D < 8 || D > 128 || D % 8) return xq_set_error(XQ_EINVAL, "%s: head dim %ld is not a multiple of 8 up to 128", fn, (long)D);
+    if (!(scale > 0.0f) || !(scale < INFINITY)) return xq_set_error(XQ_EINVAL, "%s: scale has to be positive and finite", fn);
+    if ((long)B * Hk * (tiles_of((long)Nq * (H / Hk), 128) + 8) > (1L << 22) || (long)B * Hk * (tiles_of(Nk, 128) + 8) > (1L << 22) ||
+        (long)Nq * (H / Hk) > 0x7fffff00L || (long)B * H * Nq > 0x7fffffffL || (long)B * Hk * Nk > 0x3fffffffL)
+        return xq_set_error(XQ_EINVAL, "%s: too many rows (%ld) or keys (%ld) for one call", fn, (long)B * H * Nq, (long)B * Hk * Nk);
+    return XQ_OK;
+}
+
+int check_view(const char *fn, const char *what, const void *p, const int64_t *s) {
+    if (((uintptr_t)p & 15) || s[0] % 8 || s[1] % 8 || s[2] % 8) {
+        snprintf(g_err, sizeof(g_err), "%s: %s has to be 16-byte aligned in every row (pointer and strides in multiples of 8 elements)", fn, what);
+        return XQ_EINVAL;
+    }
+    return XQ_OK;
+}
+
+View view_of(const void *p, const int64_t *s) { return View{(short *)p, (long)s[0], (long)s[1], (long)s[2]}; }
+
+void plan_blocks(Args &a, long tiles, int splits, unsigned &blocks) {
+    a.splits = splits;
+    a.nper = (int)(tiles * splits);
+    a.swizzle = a.groups % 8 == 0 || a.groups >= 64;
+    blocks = (unsigned)((a.swizzle ? (a.groups + 7) / 8 * 8 : a.groups) * (long)a.nper);
+}
+
+#define XA_BY_WIDTH(D, CALL)          \
+    do {                              \
+        if ((D) <= 32) CALL(32);      \
+        else if ((D) <= 64) CALL(64); \
+        else if ((D) <= 96) CALL(96); \
+        else CALL(128);               \
+    } while (0)
+
+}  // namespace
+
+extern "C" size_t xq_xattn_forward_workspace_bytes(int B, int Nq, int Nk, int H, int Hk, int D) {
+    if (check_sizes("xq_xattn_forward_workspace_bytes", B, Nq, Nk, H, Hk, D, 1.0f)) return 0;
+    return sizes_of(B, Nq, Nk, H, Hk, D).fwd_bytes;
+}
+
+extern "C" size_t xq_xattn_backward_workspace_bytes(int B, int Nq, int Nk, int H, int Hk, int D) {
+    if (check_sizes("xq_xattn_backward_workspace_bytes", B, Nq, Nk, H, Hk, D, 1.0f)) return 0;
+    return sizes_of(B, Nq, Nk, H, Hk, D).bwd_bytes;
+}
+
+extern "C" int xq_xattn_forward(const void *q, const void *k, const void *v, int B, int Nq, int Nk, int H, int Hk, int D, const int64_t *strides,
+                                const void *kv_lens, int lens_i64, const void *key_mask, float scale, void *out, float *lse, void *workspace,
+                                size_t workspace_bytes, xq_stream_t stream) {
+    const char *fn = "xq_xattn_forward";
+    if (int rc = check_sizes(fn, B, Nq, Nk, H, Hk, D, scale)) return rc;
+    if (B == 0 || Nq == 0) return XQ_OK;
+    if (!q || !out || !strides || (Nk > 0 && (!k || !v))) return xq_set_error(XQ_EINVAL, "%s: null pointer", fn);
+    if (int rc = check_view(fn, "q", q, strides)) return rc;
+    if (int rc = check_view(fn, "k", k, strides + 3)) return rc;
+    if (int rc = check_view(fn, "v", v, strides + 6)) return rc;
+    if ((uintptr_t)out & 15) return xq_set_error(XQ_EINVAL, "%s: out has to be 16-byte aligned", fn);
+    const Sizes z = sizes_of(B, Nq, Nk, H, Hk, D);
+    if (z.fwd_bytes && (!workspace || workspace_bytes < z.fwd_bytes))
+        return xq_set_error(XQ_ENOSPACE, "%s: workspace too small (need %ld bytes, got %ld)", fn, (long)z.fwd_bytes, (long)workspace_bytes);
+    hipStream_t s = (hipStream_t)stream;
+    Args a = {};
+    a.q = view_of(q, strides); a.k = view_of(k, strides + 3); a.v = view_of(v, strides + 6);
+    a.out = (short *)out; a.lse = lse;
+    a.lens = kv_lens; a.lens_i64 = lens_i64; a.mask = (const unsigned char *)key_mask;
+    a.B = B; a.Nq = Nq; a.Nk = Nk; a.H = H; a.Hk = Hk; a.G = H / Hk; a.D = D; a.R = (int)z.R;
+    a.g_reciprocal = reciprocal_of(a.G);
+    a.scale = scale; a.groups = (int)z.groups;
+    a.part = (float *)workspace; a.stat = (float *)((char *)workspace + z.fwd_part);
+    unsigned blocks;
+    plan_blocks(a, tiles_of(z.R, 128), z.fwd_splits, blocks);
+    if (z.fwd_splits > 1) {
+#define XA_CALL(DT) hipLaunchKernelGGL((xattn_fwd_kernel<DT, true>), dim3(blocks), dim3(256), 0, s, a)
+        XA_BY_WIDTH(D, XA_CALL);
+#undef XA_CALL
+        const long total = z.groups * z.R * (D / 4);
+        hipLaunchKernelGGL(xattn_join_kernel, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, s, a, D / 4, reciprocal_of(D / 4), total);
+    } else {
+#define XA_CALL(DT) hipLaunchKernelGGL((xattn_fwd_kernel<DT, false>), dim3(blocks), dim3(256), 0, s, a)
+        XA_BY_WIDTH(D, XA_CALL);
+#undef XA_CALL
+    }
+    return xq_check_launch(fn);
+}
+
+extern "C" int xq_xattn_backward(const void *q, const void *k, const void *v, const void *out, const void *dout, const float *lse, int B, int Nq, int Nk, int H,
+                                 int Hk, int D, const int64_t *strides, const void *kv_lens, int lens_i64, const void *key_mask, float scale, void *dq, void *dk,
+                                 void *dv, const int64_t *grad_strides, void *workspace, size_t workspace_bytes, xq_stream_t stream) {
+    const char *fn = "xq_xattn_backward";
+    if (int rc = check_sizes(fn, B, Nq, Nk, H, Hk, D, scale)) return rc;
+    if (B == 0 || (Nq == 0 && Nk == 0)) return XQ_OK;
+    if (!strides || !grad_strides || (Nq > 0 && (!q || !out || !dout || !lse || !dq)) || (Nk > 0 && (!k || !v || !dk || !dv)))
+        return xq_set_error(XQ_EINVAL, "%s: null pointer", fn);
+    const void *in[3] = {q, k, v}, *gr[3] = {dq, dk, dv};
+    const char *names[6] = {"q", "k", "v", "dq", "dk", "dv"};
+    for (int i = 0; i < 3; ++i) {
+        if (int rc = check_view(fn, names[i], in[i], strides + 3 * i)) return rc;
+        if (int rc = check_view(fn, names[3 + i], gr[i], grad_strides + 3 * i)) return rc;
+    }
+    if (((uintptr_t)out | (uintptr_t)dout) & 15) return xq_set_error(XQ_EINVAL, "%s: out and dout have to be 16-byte aligned", fn);
+    const Sizes z = sizes_of(B, Nq, Nk, H, Hk, D);
+    if (z.bwd_bytes && (!workspace || workspace_bytes < z.bwd_bytes))
+        return xq_set_error(XQ_ENOSPACE, "%s: workspace too small (need %ld bytes, got %ld)", fn, (long)z.bwd_bytes, (long)workspace_bytes);
+    hipStream_t s = (hipStream_t)stream;
+    Args a = {};
+    a.q = view_of(q, strides); a.k = view_of(k, strides + 3); a.v = view_of(v, strides + 6);
+    a.dq = view_of(dq, grad_strides); a.dk = view_of(dk, grad_strides + 3); a.dv = view_of(dv, grad_strides + 6);
+    a.out_in = (const short *)out; a.dout = (const short *)dout; a.lse = (float *)lse;
+    a.lens = kv_lens; a.lens_i64 = lens_i64; a.mask = (const unsigned char *)key_mask;
+    a.B = B; a.Nq = Nq; a.Nk = Nk; a.H = H; a.Hk = Hk; a.G = H / Hk; a.D = D; a.R = (int)z.R;
+    a.g_reciprocal = reciprocal_of(a.G);
+    a.scale = scale; a.groups = (int)z.groups;
+    a.delta = (float *)workspace; a.part = (float *)((char *)workspace + z.delta_bytes);
+    unsigned blocks;
+    if (Nq > 0) {
+        plan_blocks(a, tiles_of(z.R, 128), z.dq_splits, blocks);
+        if (z.dq_splits > 1) {
+#define XA_CALL(DT) hipLaunchKernelGGL((xattn_dq_kernel<DT, true>), dim3(blocks), dim3(256), 0, s, a)
+            XA_BY_WIDTH(D, XA_CALL);
+#undef XA_CALL
+            const long total = z.groups * z.R * (D / 4);
+            hipLaunchKernelGGL((xattn_sum_kernel<0>), dim3((unsigned)((total + 255) / 256)), dim3(256), 0, s, a, D / 4, reciprocal_of(D / 4), total);
+        } else {
+#define XA_CALL(DT) hipLaunchKernelGGL((xattn_dq_kernel<DT, false>), dim3(blocks), dim3(256), 0, s, a)
+            XA_BY_WIDTH(D, XA_CALL);
+#undef XA_CALL
+        }
+    }
+    if (Nk > 0) {
+        plan_blocks(a, tiles_of(Nk, 128), z.kv_splits, blocks);
+        if (z.kv_splits > 1) {
+#define XA_CALL(DT) hipLaunchKernelGGL((xattn_dkdv_kernel<DT, true>), dim3(blocks), dim3(256), 0, s, a)
+            XA_BY_WIDTH(D, XA_CALL);
+#undef XA_CALL
+            const long total = 2 * z.groups * (long)Nk * (D / 4);
+            hipLaunchKernelGGL((xattn_sum_kernel<1>), dim3((unsigned)((total + 255) / 256)), dim3(256), 0, s, a, D / 4, reciprocal_of(D / 4), total);
+        } else {
+#define XA_CALL(DT) hipLaunchKernelGGL((xattn_dkdv_kernel<DT, false>), dim3(blocks), dim3(256), 0, s, a)
+            XA_BY_WIDTH(D, XA_CALL);
+#undef XA_CALL
+        }
+    }
+    return xq_check_launch(fn);
+}

@@ -120,11 +120,14 @@ def attention_qkvpacked(qkv, num_heads):
             _f32_train_note()
             IMPL["attention_fp32_training"] = "hip (xq_attention_f32_lse / xq_attention_f32_backward)"
             return ops_f32.AttentionF32Fn.apply(qkv, num_heads)
+        if ops_seq.packed_attention_supported(qkv, num_heads):
+            IMPL["attention"] = "hip (xq_xattn_forward / xq_xattn_backward)"
+            return ops_seq.PackedAttentionFn.apply(qkv, num_heads)
     B, N, C3 = qkv.shape
     C = C3 // 3
     q, k, v = qkv.reshape(B, N, 3, num_heads, C // num_heads).permute(2, 0, 3, 1, 4).unbind(0)
     if qkv.is_cuda:
-        _lib_ran("attention_library", "library (SDPA: head_dim != 64 or fp32 training)")
+        _lib_ran("attention_library", "library (SDPA: head_dim no multiple of 8 up to 128, or fp32 training)")
     x = F.scaled_dot_product_attention(q, k, v)
     return x.transpose(1, 2).reshape(B, N, C)
 
@@ -351,3 +354,32 @@ def embedding(idx, weight, scale=1.0, padding_idx=None, dtype=None):
         return y if dtype is None else y.to(dtype)
     IMPL["embedding"] = "hip"
     return ops_seq.embedding(idx, weight, scale, padding_idx, dtype)
+
+
+def cross_attention(q, k, v, kv_lens=None, key_mask=None, scale=None):
+    """Attention of one sequence to another: softmax(scale q k^T over the valid keys) v -> (B, Nq, H, D); one token (Nq = 1, serving) to thousands, gradients
+    for q, k and v (csrc/xq_xattn.hip; no N x N buffer, no atomics).
+      q: (B, Nq, H, D); k, v: (B, Nk, Hk, D) with H a multiple of Hk (head h reads kv head h // (H // Hk)); bf16, or cast to it by bf16 autocast; D a multiple of 8
+         up to 128; any strides (a packed k / v projection is read in place; rows that are not 16-byte aligned are copied first);
+      kv_lens: int32 / int64 (B,), how many of a sample's keys are valid (clamped to 0 .. Nk: no host check); key_mask: bool (B, Nk), True = valid.  Both on the
+         device; a key is valid where both say so.  What lies in masked places (infinities, NaN) reaches nothing; a sample without a valid key gives zeros;
+      scale: positive; default D ** -0.5.
+    CPU tensors: the same in plain fp32 operations."""
+    if q.is_cuda:
+        if torch.is_autocast_enabled("cuda"):
+            act = torch.get_autocast_dtype("cuda")
+            q, k, v = q.to(act), k.to(act), v.to(act)
+        IMPL["cross_attention"] = "hip"
+        return ops_seq.cross_attention(q, k, v, kv_lens, key_mask, scale)
+    scale = ops_seq.check_cross_attention(q, k, v, kv_lens, key_mask, scale)
+    IMPL["cross_attention"] = "library (CPU)"
+    B, Nq, H, D = q.shape
+    Nk, G = k.shape[1], q.shape[2] // k.shape[2]
+    valid = torch.ones(B, Nk, dtype=torch.bool) if key_mask is None else key_mask
+    if kv_lens is not None:
+        valid = valid & (torch.arange(Nk) < kv_lens[:, None])
+    valid = valid[:, None, None]
+    kk, vv = (t.float().repeat_interleave(G, dim=2).transpose(1, 2).masked_fill(~valid.transpose(2, 3), 0.0) for t in (k, v))
+    s = (torch.matmul(q.float().transpose(1, 2), kk.transpose(2, 3)) * scale).masked_fill(~valid, float("-inf"))
+    p = torch.softmax(s.masked_fill(~valid.any(-1, keepdim=True), 0.0), dim=-1).masked_fill(~valid, 0.0) if Nk else s
+    return torch.matmul(p, vv).transpose(1, 2).to(q.dtype)

@@ -569,9 +569,9 @@ def attention_supported(qkv, num_heads):
 
 
 def attention_qkvpacked(qkv, num_heads):
-    """(B, N, 3*C) -> (B, N, C).  bf16 with head_dim 64: the hand-written kernels on the packed projection; anything else
-    (the fp32 parity path): library SDPA on strided q/k/v views."""
-    from . import nn_ops, ops_f32
+    """(B, N, 3*C) -> (B, N, C).  bf16 with head_dim 64: the hand-written kernels on the packed projection; bf16 with another multiple of 8 up to 128:
+    the cross-attention kernels on its views; anything else (the fp32 parity path): library SDPA on strided q/k/v views."""
+    from . import nn_ops, ops_f32, ops_seq
     if attention_supported(qkv, num_heads):
         nn_ops.IMPL["attention"] = "hip"
         return AttentionFn.apply(qkv, num_heads)
@@ -582,6 +582,9 @@ def attention_qkvpacked(qkv, num_heads):
         nn_ops._f32_train_note()
         nn_ops.IMPL["attention_fp32_training"] = "hip (xq_attention_f32_lse / xq_attention_f32_backward)"
         return ops_f32.AttentionF32Fn.apply(qkv, num_heads)
+    if ops_seq.packed_attention_supported(qkv, num_heads):
+        nn_ops.IMPL["attention"] = "hip (xq_xattn_forward / xq_xattn_backward)"
+        return ops_seq.PackedAttentionFn.apply(qkv, num_heads)
     nn_ops.IMPL["attention"] = "library (SDPA)"
     B, N, C3 = qkv.shape
     C = C3 // 3

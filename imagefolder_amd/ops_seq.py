@@ -1,6 +1,9 @@
-"""Autograd Functions over csrc/xq_drop.hip and csrc/xq_embed.hip: the operators of a token model that reads the tokenizer's codes (dropout with a
-counter-based generator, embedding with a sorted gradient).  The public entry points are nn_ops.dropout / nn_ops.embedding; everything here takes
-tensors that live on an MI355X.  Every call enqueues on the current stream of its tensors' device and allocates its outputs and workspace there."""
+"""Autograd Functions over csrc/xq_drop.hip, csrc/xq_embed.hip and csrc/xq_xattn.hip: the operators of a token model that reads the tokenizer's codes
+(dropout with a counter-based generator, embedding with a sorted gradient, attention to another sequence).  The public entry points are nn_ops.dropout,
+nn_ops.embedding and nn_ops.cross_attention; everything here takes tensors that live on an MI355X.  Every call enqueues on the current stream of its
+tensors' device and allocates its outputs and workspace there."""
+import ctypes
+
 import torch
 
 from . import _lib
@@ -155,3 +158,130 @@ def embedding(idx, weight, scale=1.0, padding_idx=None, dtype=None):
         skip = padding_idx % weight.shape[0]
     _same_device("embedding", weight, idx)
     return EmbeddingFn.apply(idx, weight, float(scale), skip, dtype)
+
+
+# ---- attention to another sequence ---------------------------------------------------------------------------------------------------------
+
+_NINE = ctypes.c_int64 * 9
+
+
+def _rows(t):
+    """t (B, N, heads, D) as the kernels read it: elements of a row side by side, rows 16-byte aligned; a copy where it is not"""
+    s = t.stride()
+    if (s[3] == 1 or t.shape[3] == 1) and not (s[0] | s[1] | s[2]) & 7 and not t.data_ptr() & 15:
+        return t
+    if t.is_contiguous() and not t.data_ptr() & 15:
+        return t                                       # (strides of dimensions of one element may be anything: see _strides)
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _strides(*views):
+    return _NINE(*[0 if n == 1 else st for t in views for n, st in zip(t.shape[:3], t.stride()[:3])])
+
+
+def _xattn_forward(q, k, v, lens, mask, scale, want_lse):
+    B, Nq, H, D = q.shape
+    Nk, Hk = k.shape[1], k.shape[2]
+    out = torch.empty(B, Nq, H, D, dtype=q.dtype, device=q.device)
+    lse = torch.empty(B, Hk, Nq * (H // Hk), dtype=torch.float32, device=q.device) if want_lse else None
+    nbytes = _lib.lib().xq_xattn_forward_workspace_bytes(B, Nq, Nk, H, Hk, D)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    _launch("xq_xattn_forward", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), B, Nq, Nk, H, Hk, D, _strides(q, k, v), _at(lens),
+            lens is not None and lens.dtype == torch.int64, _at(mask), scale, out.data_ptr(), _at(lse), _at(ws), nbytes)
+    return out, lse
+
+
+def _xattn_backward(q, k, v, out, g, lse, lens, mask, scale, dq, dk, dv):
+    B, Nq, H, D = q.shape
+    Nk, Hk = k.shape[1], k.shape[2]
+    g = _rows(g) if g.is_contiguous() else g.contiguous()
+    nbytes = _lib.lib().xq_xattn_backward_workspace_bytes(B, Nq, Nk, H, Hk, D)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    _launch("xq_xattn_backward", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), g.data_ptr(), lse.data_ptr(), B, Nq, Nk, H, Hk, D,
+            _strides(q, k, v), _at(lens), lens is not None and lens.dtype == torch.int64, _at(mask), scale, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+            _strides(dq, dk, dv), _at(ws), nbytes)
+
+
+class CrossAttentionFn(torch.autograd.Function):
+    """softmax(scale q k^T over valid keys) v: xq_xattn_forward / xq_xattn_backward"""
+
+    @staticmethod
+    def forward(ctx, q, k, v, lens, mask, scale):
+        q, k, v = _rows(q.detach()), _rows(k.detach()), _rows(v.detach())
+        grad = any(ctx.needs_input_grad)
+        out, lse = _xattn_forward(q, k, v, lens, mask, scale, grad)
+        if grad:
+            ctx.save_for_backward(q, k, v, out, lse, lens, mask)
+            ctx.scale = scale
+        return out
+
+    @staticmethod
+    def backward(ctx, g):
+        q, k, v, out, lse, lens, mask = ctx.saved_tensors
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        _xattn_backward(q, k, v, out, g.detach(), lse, lens, mask, ctx.scale, dq, dk, dv)
+        return dq, dk, dv, None, None, None
+
+
+class PackedAttentionFn(torch.autograd.Function):
+    """self-attention on the packed (B, N, 3, H, D) projection through the same kernels, for the head widths that csrc/xq_attn.hip (64) does not take"""
+
+    @staticmethod
+    def forward(ctx, qkv, num_heads):
+        B, N, C3 = qkv.shape
+        x = qkv.detach().contiguous()
+        if x.data_ptr() & 15:
+            x = x.clone()
+        q, k, v = x.view(B, N, 3, num_heads, -1).unbind(2)
+        scale = float(q.shape[3]) ** -0.5
+        out, lse = _xattn_forward(q, k, v, None, None, scale, True)
+        ctx.save_for_backward(x, out, lse)
+        ctx.scale = scale
+        return out.view(B, N, C3 // 3)
+
+    @staticmethod
+    def backward(ctx, g):
+        x, out, lse = ctx.saved_tensors
+        B, N, H, D = out.shape
+        dx = torch.empty_like(x)
+        _xattn_backward(*x.view(B, N, 3, H, D).unbind(2), out, g.detach().to(x.dtype).reshape(B, N, H, D), lse, None, None, ctx.scale,
+                        *dx.view(B, N, 3, H, D).unbind(2))
+        return dx, None
+
+
+def packed_attention_supported(qkv, num_heads):
+    D = qkv.shape[-1] // (3 * num_heads)
+    return qkv.is_cuda and qkv.dtype == torch.bfloat16 and qkv.dim() == 3 and qkv.shape[-1] == 3 * num_heads * D and D % 8 == 0 and 8 <= D <= 128
+
+
+def check_cross_attention(q, k, v, kv_lens, key_mask, scale):
+    """shapes and types, on whatever device -> the scale"""
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if t.dim() != 4:
+            raise XqError(f"cross_attention: {name} is (batch, tokens, heads, head dim) (got shape {tuple(t.shape)})")
+    B, Nq, H, D = q.shape
+    Nk, Hk = k.shape[1], k.shape[2]
+    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
+        raise XqError(f"cross_attention: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not go together")
+    if H < 1 or Hk < 1 or H % Hk:
+        raise XqError(f"cross_attention: {H} query heads do not share {Hk} key / value heads evenly")
+    if D < 1:
+        raise XqError("cross_attention: a head dim of 0")
+    if kv_lens is not None and (tuple(kv_lens.shape) != (B,) or kv_lens.dtype not in (torch.int32, torch.int64)):
+        raise XqError(f"cross_attention: kv_lens is an int32 or int64 tensor of {B} lengths (got {kv_lens.dtype}, shape {tuple(kv_lens.shape)})")
+    if key_mask is not None and (tuple(key_mask.shape) != (B, Nk) or key_mask.dtype != torch.bool):
+        raise XqError(f"cross_attention: key_mask is a bool tensor of shape {(B, Nk)} (got {key_mask.dtype}, shape {tuple(key_mask.shape)})")
+    scale = float(D) ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < float("inf"):
+        raise XqError(f"cross_attention: scale = {scale} is not positive and finite")
+    return scale
+
+
+def cross_attention(q, k, v, kv_lens=None, key_mask=None, scale=None):
+    scale = check_cross_attention(q, k, v, kv_lens, key_mask, scale)
+    if q.dtype != torch.bfloat16 or k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
+        raise XqError(f"cross_attention: q, k, v of types {q.dtype}, {k.dtype}, {v.dtype} (bf16; other types under bf16 autocast)")
+    if q.shape[3] % 8 or q.shape[3] > 128:
+        raise XqError(f"cross_attention: head dim {q.shape[3]} is not a multiple of 8 up to 128")
+    _same_device("cross_attention", q, k, v, kv_lens, key_mask)
+    return CrossAttentionFn.apply(q, k, v, None if kv_lens is None else kv_lens.contiguous(), None if key_mask is None else key_mask.contiguous(), scale)

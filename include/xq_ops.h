@@ -582,6 +582,24 @@ size_t xq_embedding_backward_workspace_bytes(int64_t N, int64_t V, int D);
 int xq_embedding_backward(const void *idx, int idx_i64, const void *g, int g_bf16, int64_t N, int64_t V, int D, float scale, int64_t skip, void *dw,
                           int dw_bf16, void *workspace, size_t workspace_bytes, xq_stream_t stream);
 
+/* attention of one sequence to another, csrc/xq_xattn.hip: O = softmax(scale q k^T over the valid keys) v.
+ *   q [B][Nq][H][D], k, v [B][Nk][Hk][D] bf16 with any strides: `strides` is a HOST array of nine element strides (q batch, token, head; k ...; v ...), the last
+ *   dimension has stride 1, pointers are 16-byte aligned, strides multiples of 8 (0 for a broadcast dimension).  Head h reads kv head h / (H / Hk).
+ *   D a multiple of 8, 8 .. 128.  Nq, Nk from 0 on.
+ *   kv_lens (nullable): DEVICE int32 or int64 (lens_i64) [B], valid keys of a sample (clamped to 0 .. Nk); key_mask (nullable): DEVICE bytes [B][Nk], 0 = masked.
+ *   What lies in masked places reaches nothing.  A sample without a valid key: rows of zeros, lse = -inf, zero gradients.  scale > 0.
+ *   out [B][Nq][H][D] bf16 contiguous; lse (nullable) fp32 [B][Hk][Nq * H / Hk] (row = token * (H / Hk) + head of the group), what the backward reads.
+ *   workspace: xq_xattn_forward_workspace_bytes (0 where the keys are not split over blocks). */
+size_t xq_xattn_forward_workspace_bytes(int B, int Nq, int Nk, int H, int Hk, int D);
+int xq_xattn_forward(const void *q, const void *k, const void *v, int B, int Nq, int Nk, int H, int Hk, int D, const int64_t *strides, const void *kv_lens,
+                     int lens_i64, const void *key_mask, float scale, void *out, float *lse, void *workspace, size_t workspace_bytes, xq_stream_t stream);
+/* its gradients: dq, dk, dv bf16 with `grad_strides` (HOST, nine, as above); out, dout contiguous; every row of dq, dk, dv is written (masked keys with zeros).
+ * No atomics: the same bits from run to run.  workspace: xq_xattn_backward_workspace_bytes. */
+size_t xq_xattn_backward_workspace_bytes(int B, int Nq, int Nk, int H, int Hk, int D);
+int xq_xattn_backward(const void *q, const void *k, const void *v, const void *out, const void *dout, const float *lse, int B, int Nq, int Nk, int H, int Hk,
+                      int D, const int64_t *strides, const void *kv_lens, int lens_i64, const void *key_mask, float scale, void *dq, void *dk, void *dv,
+                      const int64_t *grad_strides, void *workspace, size_t workspace_bytes, xq_stream_t stream);
+
 /* ---- measurement hooks (bench.py): HIP events recorded around the instrumented hand-written kernels on the stream they
  *      are launched on.  xq_prof_enable(1) resets and arms, (0) disarms and keeps what was recorded, (2) arms without resetting; xq_prof_collect_kind synchronises the recorded events of one
  *      kernel kind and returns their summed duration, launch count and summed algorithmic work (flops) since arming;
