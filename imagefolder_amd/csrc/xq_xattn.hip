@@ -105,22 +105,35 @@ __device__ __forceinline__ int keys_of(const Args &a, int b) {
     return (int)(n < 0 ? 0 : n > a.Nk ? a.Nk : n);
 }
 
-// the valid ones of the 64 keys from kv0, one bit each (the same in every lane)
-__device__ __forceinline__ uint64_t valid_bits(const Args &a, const unsigned char *mask_row, int len, int kv0) {
-    const int left = len - kv0;
-    uint64_t bits = left >= 64 ? ~0ull : left <= 0 ? 0ull : (1ull << left) - 1;
-    if (mask_row) {
+// The valid ones of 64 keys, one bit each (the same in every lane).  A mask's bytes are fetched a tile ahead of the tile's own loads, which wait for them.
+struct KeyBits {
+    const unsigned char *mask;
+    int len, on;
+    __device__ __forceinline__ void fetch(int kv0) {
+        if (!mask) return;
         const int key = kv0 + (int)(threadIdx.x & 63);
-        bool on = false;
-        if (key < len) on = mask_row[key] != 0;
-        bits &= __ballot(on);
+        on = 0;
+        if (key < len) on = mask[key];
     }
-    return bits;
-}
+    __device__ __forceinline__ uint64_t take(int kv0) const {
+        const int left = len - kv0;
+        const uint64_t bits = left >= 64 ? ~0ull : left <= 0 ? 0ull : (1ull << left) - 1;
+        return mask ? bits & __ballot(on != 0) : bits;
+    }
+};
 
 __device__ __forceinline__ uint4 zero_unless(uint4 v, bool ok) {
     if (!ok) v = make_uint4(0u, 0u, 0u, 0u);
     return v;
+}
+
+// 16 bytes at a byte offset of up to 2^31 behind a wave-uniform base; FAR reads zeros (a buffer's bounds check), so that what is masked or behind the head
+// dimension costs an offset and no select on the data, and is never touched
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+constexpr uint32_t FAR = 0x80000000u;
+__device__ __forceinline__ uint4 load16(const short *base, uint32_t off) {
+    const auto rs = __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, 0x7fffffff, 0x00020000);
+    return __builtin_bit_cast(uint4, (u32x4)__builtin_amdgcn_raw_buffer_load_b128(rs, (int)off, 0, 0));
 }
 
 // element offset of row r of kv head hk in a query-sided view
@@ -129,26 +142,32 @@ __device__ __forceinline__ long row_offset(const Args &a, const View &t, int b, 
     return b * t.sb + (long)tok * t.sn + (long)(hk * a.G + (int)g) * t.sh;
 }
 
-// 64 rows of a key-sided view into registers (CH 16-byte chunks a thread), then into the LDS tile with the invalid ones zeroed
-template <int DT, int ROWS>
+// ROWS rows into registers (CH 16-byte chunks a thread), then into a row-major LDS tile; a row whose bit is clear arrives as zeros
+template <int DT, int ROWS, int THREADS>
 struct Stage {
-    static constexpr int PER_ROW = DT / 8, CH = ROWS * PER_ROW / 256, P = DT + 8;
+    static constexpr int PER_ROW = DT / 8, CH = (ROWS * PER_ROW + THREADS - 1) / THREADS, P = DT + 8;
+    static constexpr bool EVEN = ROWS * PER_ROW % THREADS == 0;
+    uint32_t off[CH];
     uint4 r[CH];
-    __device__ __forceinline__ void load(const short *base, long sn, int row0, int last, int D) {
+    static __device__ __forceinline__ int row(int c) { return (int)(threadIdx.x + THREADS * c) / PER_ROW; }
+    static __device__ __forceinline__ int col(int c) { return (int)(threadIdx.x + THREADS * c) % PER_ROW * 8; }
+    __device__ __forceinline__ void places(long sn, int D) {
 #pragma unroll
-        for (int c = 0; c < CH; ++c) {
-            const int id = threadIdx.x + 256 * c, row = id / PER_ROW, part = id % PER_ROW;
-            const int n = row0 + row <= last ? row0 + row : last;
-            const uint4 x = *reinterpret_cast<const uint4 *>(base + (long)n * sn + (8 * part < D ? 8 * part : 0));
-            r[c] = zero_unless(x, 8 * part < D);
+        for (int c = 0; c < CH; ++c) off[c] = col(c) < D && (EVEN || row(c) < ROWS) ? (uint32_t)(row(c) * (int)sn + col(c)) * 2 : FAR;
+    }
+    __device__ __forceinline__ void load(const short *base, uint64_t bits) {
+        if (~bits) {
+#pragma unroll
+            for (int c = 0; c < CH; ++c) r[c] = load16(base, (bits >> (row(c) & 63)) & 1 ? off[c] : FAR);
+        } else {
+#pragma unroll
+            for (int c = 0; c < CH; ++c) r[c] = load16(base, off[c]);
         }
     }
-    __device__ __forceinline__ void store(short *tile, uint64_t bits) const {
+    __device__ __forceinline__ void store(short *tile) const {
 #pragma unroll
-        for (int c = 0; c < CH; ++c) {
-            const int id = threadIdx.x + 256 * c, row = id / PER_ROW, part = id % PER_ROW;
-            *reinterpret_cast<uint4 *>(tile + row * P + 8 * part) = zero_unless(r[c], (bits >> row) & 1);
-        }
+        for (int c = 0; c < CH; ++c)
+            if (EVEN || row(c) < ROWS) *reinterpret_cast<uint4 *>(tile + row(c) * P + col(c)) = r[c];
     }
 };
 
@@ -216,7 +235,6 @@ __global__ __launch_bounds__(256, 2) void xattn_fwd_kernel(Args a) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 31, hh = lane >> 5;
     const int trp = (4 * hh + ((lane & 15) >> 2)) * P + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
     const int len = keys_of(a, b);
-    const unsigned char *mask = a.mask ? a.mask + (long)b * a.Nk : nullptr;
     const short *kb = a.k.p + b * a.k.sb + hk * a.k.sh, *vb = a.v.p + b * a.v.sb + hk * a.v.sh;
     const float c = a.scale * LOG2E;
 
@@ -238,29 +256,37 @@ __global__ __launch_bounds__(256, 2) void xattn_fwd_kernel(Args a) {
 
     int t0, t1;
     share((len + 63) / 64, split, SPLIT ? a.splits : 1, t0, t1);
-    Stage<DT, 64> sk, sv;
+    Stage<DT, 64, 256> sk, sv;
+    sk.places(a.k.sn, a.D);
+    sv.places(a.v.sn, a.D);
+    KeyBits keys = {a.mask ? a.mask + (long)b * a.Nk : nullptr, len, 0};
     uint64_t bits = 0, next = 0;
     if (t0 < t1) {
-        bits = valid_bits(a, mask, len, t0 * 64);
-        sk.load(kb, a.k.sn, t0 * 64, a.Nk - 1, a.D);
-        sv.load(vb, a.v.sn, t0 * 64, a.Nk - 1, a.D);
-        sk.store(Ks[0], bits);
-        sv.store(Vs[0], bits);
+        keys.fetch(t0 * 64);
+        bits = keys.take(t0 * 64);
+        sk.load(kb + t0 * 64L * a.k.sn, bits);
+        sv.load(vb + t0 * 64L * a.v.sn, bits);
+        keys.fetch(t0 * 64 + 64);
+        sk.store(Ks[0]);
+        sv.store(Vs[0]);
     }
     __syncthreads();
     for (int t = t0; t < t1; ++t) {
         const int cur = (t - t0) & 1;
         if (t + 1 < t1) {
-            next = valid_bits(a, mask, len, t * 64 + 64);
-            sk.load(kb, a.k.sn, t * 64 + 64, a.Nk - 1, a.D);
-            sv.load(vb, a.v.sn, t * 64 + 64, a.Nk - 1, a.D);
+            next = keys.take(t * 64 + 64);
+            sk.load(kb + (t + 1) * 64L * a.k.sn, next);
+            sv.load(vb + (t + 1) * 64L * a.v.sn, next);
+            keys.fetch(t * 64 + 128);
         }
         if (wave_live && bits) {
             const short *K = Ks[cur] + li * P + 8 * hh, *V = Vs[cur] + trp;
+            const bool wide = (bits >> 32) != 0;           // the second 32 keys of the tile hold one at least
             f32x16 s[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 s[h] = zero16;
+                if (h == 1 && !wide) continue;
 #pragma unroll
                 for (int k = 0; k < KS; ++k) s[h] = XA_MFMA(*reinterpret_cast<const bf16x8 *>(K + 32 * h * P + 16 * k), qf[k], s[h]);
             }
@@ -296,6 +322,7 @@ __global__ __launch_bounds__(256, 2) void xattn_fwd_kernel(Args a) {
             f32x16 ls = zero16;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
+                if (h == 1 && !wide) continue;
                 float p[16];
 #pragma unroll
                 for (int j = 0; j < 16; ++j) p[j] = __builtin_amdgcn_exp2f(fmaf(s[h][j], c, -mref));
@@ -310,8 +337,8 @@ __global__ __launch_bounds__(256, 2) void xattn_fwd_kernel(Args a) {
             l += ls[0];            // every row of ones x P^T is the sum over the tile's keys of this lane's row
         }
         if (t + 1 < t1) {
-            sk.store(Ks[cur ^ 1], next);
-            sv.store(Vs[cur ^ 1], next);
+            sk.store(Ks[cur ^ 1]);
+            sv.store(Vs[cur ^ 1]);
             bits = next;
         }
         __syncthreads();
@@ -360,7 +387,7 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(Args a, int per_row, un
 // dq: one row per lane as the forward; delta in the prologue, written for the dk / dv kernel behind it
 // ---------------------------------------------------------------------------------------------------------------------------------------------
 template <int DT, bool SPLIT>
-__global__ __launch_bounds__(256, DT > 64 ? 1 : 2) void xattn_dq_kernel(Args a) {
+__global__ __launch_bounds__(256, 2) void xattn_dq_kernel(Args a) {
     constexpr int P = DT + 8, KS = DT / 16, OT = DT / 32;
     __shared__ __attribute__((aligned(16))) short Ks[2][64 * P];
     __shared__ __attribute__((aligned(16))) short Vs[2][64 * P];
@@ -371,7 +398,6 @@ __global__ __launch_bounds__(256, DT > 64 ? 1 : 2) void xattn_dq_kernel(Args a) 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 31, hh = lane >> 5;
     const int trp = (4 * hh + ((lane & 15) >> 2)) * P + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
     const int len = keys_of(a, b);
-    const unsigned char *mask = a.mask ? a.mask + (long)b * a.Nk : nullptr;
     const short *kb = a.k.p + b * a.k.sb + hk * a.k.sh, *vb = a.v.p + b * a.v.sb + hk * a.v.sh;
     const float c = a.scale * LOG2E;
 
@@ -407,27 +433,34 @@ __global__ __launch_bounds__(256, DT > 64 ? 1 : 2) void xattn_dq_kernel(Args a) 
 
     int t0, t1;
     share((len + 63) / 64, split, SPLIT ? a.splits : 1, t0, t1);
-    Stage<DT, 64> sk, sv;
+    Stage<DT, 64, 256> sk, sv;
+    sk.places(a.k.sn, a.D);
+    sv.places(a.v.sn, a.D);
+    KeyBits keys = {a.mask ? a.mask + (long)b * a.Nk : nullptr, len, 0};
     uint64_t bits = 0, next = 0;
     if (t0 < t1) {
-        bits = valid_bits(a, mask, len, t0 * 64);
-        sk.load(kb, a.k.sn, t0 * 64, a.Nk - 1, a.D);
-        sv.load(vb, a.v.sn, t0 * 64, a.Nk - 1, a.D);
-        sk.store(Ks[0], bits);
-        sv.store(Vs[0], bits);
+        keys.fetch(t0 * 64);
+        bits = keys.take(t0 * 64);
+        sk.load(kb + t0 * 64L * a.k.sn, bits);
+        sv.load(vb + t0 * 64L * a.v.sn, bits);
+        keys.fetch(t0 * 64 + 64);
+        sk.store(Ks[0]);
+        sv.store(Vs[0]);
     }
     __syncthreads();
     for (int t = t0; t < t1; ++t) {
         const int cur = (t - t0) & 1;
         if (t + 1 < t1) {
-            next = valid_bits(a, mask, len, t * 64 + 64);
-            sk.load(kb, a.k.sn, t * 64 + 64, a.Nk - 1, a.D);
-            sv.load(vb, a.v.sn, t * 64 + 64, a.Nk - 1, a.D);
+            next = keys.take(t * 64 + 64);
+            sk.load(kb + (t + 1) * 64L * a.k.sn, next);
+            sv.load(vb + (t + 1) * 64L * a.v.sn, next);
+            keys.fetch(t * 64 + 128);
         }
         if (wave_live && bits) {
             const short *K = Ks[cur] + li * P + 8 * hh, *V = Vs[cur] + li * P + 8 * hh, *T = Ks[cur] + trp;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
+                if (h == 1 && !(bits >> 32)) continue;         // no valid key among the second 32
                 f32x16 s, p;
 #pragma unroll
                 for (int j = 0; j < 16; ++j) { s[j] = 0.0f; p[j] = 0.0f; }
@@ -454,8 +487,8 @@ __global__ __launch_bounds__(256, DT > 64 ? 1 : 2) void xattn_dq_kernel(Args a) 
             }
         }
         if (t + 1 < t1) {
-            sk.store(Ks[cur ^ 1], next);
-            sv.store(Vs[cur ^ 1], next);
+            sk.store(Ks[cur ^ 1]);
+            sv.store(Vs[cur ^ 1]);
             bits = next;
         }
         __syncthreads();
@@ -472,10 +505,13 @@ __global__ __launch_bounds__(256, DT > 64 ? 1 : 2) void xattn_dq_kernel(Args a) 
 // dk, dv: one key per lane, 128 keys of one (sample, kv head) a block; 32-row tiles of q and dO (and lse, delta) in two LDS buffers
 // ---------------------------------------------------------------------------------------------------------------------------------------------
 template <int DT, bool SPLIT>
-__global__ __launch_bounds__(256, DT > 64 ? 1 : 2) void xattn_dkdv_kernel(Args a) {
-    constexpr int P = DT + 8, KS = DT / 16, OT = DT / 32, PER_ROW = DT / 8, CH = (32 * PER_ROW + 255) / 256;
+__global__ __launch_bounds__(256, 2) void xattn_dkdv_kernel(Args a) {
+    constexpr int P = DT + 8, KS = DT / 16, OT = DT / 32;
     __shared__ __attribute__((aligned(16))) short Qs[2][32 * P];
     __shared__ __attribute__((aligned(16))) short Os[2][32 * P];
+    // a wave's own 32 rows of V: at 128 columns its fragments do not fit beside the accumulators in 256 registers (two waves a SIMD)
+    constexpr bool V_IN_LDS = DT > 96;
+    __shared__ __attribute__((aligned(16))) short Vs[V_IN_LDS ? 128 * P : 8];
     __shared__ __attribute__((aligned(16))) float Ls[2][32];
     __shared__ __attribute__((aligned(16))) float Ds[2][32];
     int g, i;
@@ -495,6 +531,10 @@ __global__ __launch_bounds__(256, DT > 64 ? 1 : 2) void xattn_dkdv_kernel(Args a
     bf16x8 kf[KS], vf[KS];
     load_row<DT>(a.k.p + b * a.k.sb + hk * a.k.sh + (long)nc * a.k.sn, a.D, hh, kf);
     load_row<DT>(a.v.p + b * a.v.sb + hk * a.v.sh + (long)nc * a.v.sn, a.D, hh, vf);
+    if (V_IN_LDS) {
+#pragma unroll
+        for (int k = 0; k < KS; ++k) *reinterpret_cast<bf16x8 *>(Vs + (wave * 32 + li) * P + 8 * hh + 16 * k) = vf[k];
+    }
 
     f32x16 dk[OT], dv[OT];
 #pragma unroll
@@ -502,33 +542,35 @@ __global__ __launch_bounds__(256, DT > 64 ? 1 : 2) void xattn_dkdv_kernel(Args a
 #pragma unroll
         for (int j = 0; j < 16; ++j) { dk[t][j] = 0.0f; dv[t][j] = 0.0f; }
 
-    uint4 rq[CH], ro[CH];
+    // row r0 + i of a 32-row tile: token (r0 + i) / G.  Where G divides 32 its offset from the tile's first token is the same in every tile
+    Stage<DT, 32, 256> sq, so;
+    const long on = (long)a.H * a.D, oh = a.D;
     float rl = 0.0f;
-    auto load = [&](int r0) {
+    auto places = [&](int g0) {
 #pragma unroll
-        for (int ch = 0; ch < CH; ++ch) {
-            const int id = tid + 256 * ch, row = id / PER_ROW, part = id % PER_ROW;
-            const int r = r0 + row;
-            const bool ok = row < 32 && r < a.R && 8 * part < a.D;
-            const int rr = ok ? r : 0, col = ok ? 8 * part : 0;
-            const uint32_t tok = quotient((uint32_t)rr, a.g_reciprocal), gg = (uint32_t)rr - tok * a.G;
-            rq[ch] = zero_unless(*reinterpret_cast<const uint4 *>(a.q.p + row_offset(a, a.q, b, hk, rr) + col), ok);
-            ro[ch] = zero_unless(*reinterpret_cast<const uint4 *>(a.dout + (((long)b * a.Nq + tok) * a.H + hk * a.G + gg) * a.D + col), ok);
+        for (int ch = 0; ch < sq.CH; ++ch) {
+            const uint32_t rr = g0 + sq.row(ch), tok = quotient(rr, a.g_reciprocal), gg = rr - tok * a.G;
+            const bool ok = sq.col(ch) < a.D && (sq.EVEN || sq.row(ch) < 32);
+            sq.off[ch] = ok ? (tok * (uint32_t)a.q.sn + gg * (uint32_t)a.q.sh + sq.col(ch)) * 2 : FAR;
+            so.off[ch] = ok ? (tok * (uint32_t)on + gg * (uint32_t)oh + sq.col(ch)) * 2 : FAR;
         }
+    };
+    const bool same_places = 32 % a.G == 0;
+    places(0);
+    auto load = [&](int r0) {
+        const int tok0 = (int)quotient((uint32_t)r0, a.g_reciprocal), left = a.R - r0;
+        if (!same_places) places(r0 - tok0 * a.G);
+        const uint64_t bits = left >= 32 ? ~0ull : (1ull << left) - 1;
+        sq.load(a.q.p + b * a.q.sb + tok0 * a.q.sn + (long)hk * a.G * a.q.sh, bits);
+        so.load(a.dout + ((long)b * a.Nq + tok0) * on + (long)hk * a.G * oh, bits);
         if (tid < 64) {
             const int r = r0 + li;
             rl = r < a.R ? (hh == 0 ? log2_of(lse[r]) : dlt[r]) : 0.0f;
         }
     };
     auto store = [&](int buf) {
-#pragma unroll
-        for (int ch = 0; ch < CH; ++ch) {
-            const int id = tid + 256 * ch, row = id / PER_ROW, part = id % PER_ROW;
-            if (row < 32) {
-                *reinterpret_cast<uint4 *>(Qs[buf] + row * P + 8 * part) = rq[ch];
-                *reinterpret_cast<uint4 *>(Os[buf] + row * P + 8 * part) = ro[ch];
-            }
-        }
+        sq.store(Qs[buf]);
+        so.store(Os[buf]);
         if (tid < 32) Ls[buf][li] = rl;
         else if (tid < 64) Ds[buf][li] = rl;
     };
@@ -544,14 +586,14 @@ __global__ __launch_bounds__(256, DT > 64 ? 1 : 2) void xattn_dkdv_kernel(Args a
         const int cur = (t - t0) & 1;
         if (t + 1 < t1) load(t * 32 + 32);
         if (wave_live) {
-            const short *Q = Qs[cur] + li * P + 8 * hh, *O = Os[cur] + li * P + 8 * hh;
+            const short *Q = Qs[cur] + li * P + 8 * hh, *O = Os[cur] + li * P + 8 * hh, *Vw = Vs + (V_IN_LDS ? (wave * 32 + li) * P + 8 * hh : 0);
             f32x16 s, p;
 #pragma unroll
             for (int j = 0; j < 16; ++j) { s[j] = 0.0f; p[j] = 0.0f; }
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
                 s = XA_MFMA(*reinterpret_cast<const bf16x8 *>(Q + 16 * k), kf[k], s);
-                p = XA_MFMA(*reinterpret_cast<const bf16x8 *>(O + 16 * k), vf[k], p);
+                p = XA_MFMA(*reinterpret_cast<const bf16x8 *>(O + 16 * k), V_IN_LDS ? *reinterpret_cast<const bf16x8 *>(Vw + 16 * k) : vf[k], p);
             }
             // register j <-> row (j & 3) + 8 (j >> 2) + 4 hh of the tile; rows behind the last have q = dO = 0 and lse = delta = 0: P is 1 there, dS 0
             float e[16], d[16];
@@ -676,7 +718,12 @@ int check_sizes(const char *fn, int B, int Nq, int Nk, int H, int Hk, int D, flo
     return XQ_OK;
 }
 
-int check_view(const char *fn, const char *what, const void *p, const int64_t *s) {
+// reach: heads that a tile of rows passes over (G for a query-sided view, 1 for a key-sided one)
+int check_view(const char *fn, const char *what, const void *p, const int64_t *s, int reach) {
+    if (s[0] < 0 || s[1] < 0 || s[2] < 0 || s[1] >= (1L << 24) || s[2] >= (1L << 24) || 64 * s[1] + reach * s[2] > (1L << 30)) {
+        snprintf(g_err, sizeof(g_err), "%s: token or head stride of %s out of range (64 tokens within 2^30 elements)", fn, what);
+        return XQ_EINVAL;
+    }
     if (((uintptr_t)p & 15) || s[0] % 8 || s[1] % 8 || s[2] % 8) {
         snprintf(g_err, sizeof(g_err), "%s: %s has to be 16-byte aligned in every row (pointer and strides in multiples of 8 elements)", fn, what);
         return XQ_EINVAL;
@@ -720,9 +767,9 @@ extern "C" int xq_xattn_forward(const void *q, const void *k, const void *v, int
     if (int rc = check_sizes(fn, B, Nq, Nk, H, Hk, D, scale)) return rc;
     if (B == 0 || Nq == 0) return XQ_OK;
     if (!q || !out || !strides || (Nk > 0 && (!k || !v))) return xq_set_error(XQ_EINVAL, "%s: null pointer", fn);
-    if (int rc = check_view(fn, "q", q, strides)) return rc;
-    if (int rc = check_view(fn, "k", k, strides + 3)) return rc;
-    if (int rc = check_view(fn, "v", v, strides + 6)) return rc;
+    if (int rc = check_view(fn, "q", q, strides, H / Hk)) return rc;
+    if (int rc = check_view(fn, "k", k, strides + 3, 1)) return rc;
+    if (int rc = check_view(fn, "v", v, strides + 6, 1)) return rc;
     if ((uintptr_t)out & 15) return xq_set_error(XQ_EINVAL, "%s: out has to be 16-byte aligned", fn);
     const Sizes z = sizes_of(B, Nq, Nk, H, Hk, D);
     if (z.fwd_bytes && (!workspace || workspace_bytes < z.fwd_bytes))
@@ -763,8 +810,8 @@ extern "C" int xq_xattn_backward(const void *q, const void *k, const void *v, co
     const void *in[3] = {q, k, v}, *gr[3] = {dq, dk, dv};
     const char *names[6] = {"q", "k", "v", "dq", "dk", "dv"};
     for (int i = 0; i < 3; ++i) {
-        if (int rc = check_view(fn, names[i], in[i], strides + 3 * i)) return rc;
-        if (int rc = check_view(fn, names[3 + i], gr[i], grad_strides + 3 * i)) return rc;
+        if (int rc = check_view(fn, names[i], in[i], strides + 3 * i, i ? 1 : H / Hk)) return rc;
+        if (int rc = check_view(fn, names[3 + i], gr[i], grad_strides + 3 * i, i ? 1 : H / Hk)) return rc;
     }
     if (((uintptr_t)out | (uintptr_t)dout) & 15) return xq_set_error(XQ_EINVAL, "%s: out and dout have to be 16-byte aligned", fn);
     const Sizes z = sizes_of(B, Nq, Nk, H, Hk, D);

@@ -168,7 +168,7 @@ _NINE = ctypes.c_int64 * 9
 def _rows(t):
     """t (B, N, heads, D) as the kernels read it: elements of a row side by side, rows 16-byte aligned; a copy where it is not"""
     s = t.stride()
-    if (s[3] == 1 or t.shape[3] == 1) and not (s[0] | s[1] | s[2]) & 7 and not t.data_ptr() & 15:
+    if (s[3] == 1 or t.shape[3] == 1) and not (s[0] | s[1] | s[2]) & 7 and not t.data_ptr() & 15 and s[1] <= 1 << 23 and s[2] <= 1 << 22:
         return t
     if t.is_contiguous() and not t.data_ptr() & 15:
         return t                                       # (strides of dimensions of one element may be anything: see _strides)

@@ -584,7 +584,7 @@ int xq_embedding_backward(const void *idx, int idx_i64, const void *g, int g_bf1
 
 /* attention of one sequence to another, csrc/xq_xattn.hip: O = softmax(scale q k^T over the valid keys) v.
  *   q [B][Nq][H][D], k, v [B][Nk][Hk][D] bf16 with any strides: `strides` is a HOST array of nine element strides (q batch, token, head; k ...; v ...), the last
- *   dimension has stride 1, pointers are 16-byte aligned, strides multiples of 8 (0 for a broadcast dimension).  Head h reads kv head h / (H / Hk).
+ *   dimension has stride 1, pointers are 16-byte aligned, strides multiples of 8 (0 for a broadcast dimension), 64 tokens within 2^30 elements.  Head h reads kv head h / (H / Hk).
  *   D a multiple of 8, 8 .. 128.  Nq, Nk from 0 on.
  *   kv_lens (nullable): DEVICE int32 or int64 (lens_i64) [B], valid keys of a sample (clamped to 0 .. Nk); key_mask (nullable): DEVICE bytes [B][Nk], 0 = masked.
  *   What lies in masked places reaches nothing.  A sample without a valid key: rows of zeros, lse = -inf, zero gradients.  scale > 0.
