@@ -502,18 +502,18 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(Args a) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------------------------
-// dk, dv: one key per lane, 128 keys of one (sample, kv head) a block; 32-row tiles of q and dO (and lse, delta) in two LDS buffers
+// dk, dv: one key per lane, 128 keys of one (sample, kv head) a block; tiles of QT rows of q and dO (and lse, delta) in two LDS buffers
 // ---------------------------------------------------------------------------------------------------------------------------------------------
-template <int DT, bool SPLIT>
-__global__ __launch_bounds__(256, 2) void xattn_dkdv_kernel(Args a) {
-    constexpr int P = DT + 8, KS = DT / 16, OT = DT / 32;
-    __shared__ __attribute__((aligned(16))) short Qs[2][32 * P];
-    __shared__ __attribute__((aligned(16))) short Os[2][32 * P];
+template <int DT, int W, bool SPLIT>
+__global__ __launch_bounds__(64 * W, DT > 64 ? 2 : 3) void xattn_dkdv_kernel(Args a) {
+    constexpr int QT = 32, P = DT + 8, KS = DT / 16, OT = DT / 32;
+    __shared__ __attribute__((aligned(16))) short Qs[2][QT * P];
+    __shared__ __attribute__((aligned(16))) short Os[2][QT * P];
     // a wave's own 32 rows of V: at 128 columns its fragments do not fit beside the accumulators in 256 registers (two waves a SIMD)
-    constexpr bool V_IN_LDS = DT > 96;
-    __shared__ __attribute__((aligned(16))) short Vs[V_IN_LDS ? 128 * P : 8];
-    __shared__ __attribute__((aligned(16))) float Ls[2][32];
-    __shared__ __attribute__((aligned(16))) float Ds[2][32];
+    constexpr bool V_IN_LDS = DT != 96;
+    __shared__ __attribute__((aligned(16))) short Vs[V_IN_LDS ? 32 * W * P : 8];
+    __shared__ __attribute__((aligned(16))) float Ls[2][QT];
+    __shared__ __attribute__((aligned(16))) float Ds[2][QT];
     int g, i;
     if (!map_block(a, g, i)) return;
     const int split = SPLIT ? i % a.splits : 0, kbk = SPLIT ? i / a.splits : i;
@@ -524,7 +524,7 @@ __global__ __launch_bounds__(256, 2) void xattn_dkdv_kernel(Args a) {
     const float c = a.scale * LOG2E;
     const float *lse = a.lse + (long)g * a.R, *dlt = a.delta + (long)g * a.R;
 
-    const int n = kbk * 128 + wave * 32 + li, nc = n < a.Nk ? n : a.Nk - 1;
+    const int n = (kbk * W + wave) * 32 + li, nc = n < a.Nk ? n : a.Nk - 1;
     bool valid = n < len;
     if (a.mask && valid) valid = a.mask[(long)b * a.Nk + n] != 0;
     const bool wave_live = __any(valid);      // a wave without a valid key only helps to stage
@@ -542,51 +542,54 @@ __global__ __launch_bounds__(256, 2) void xattn_dkdv_kernel(Args a) {
 #pragma unroll
         for (int j = 0; j < 16; ++j) { dk[t][j] = 0.0f; dv[t][j] = 0.0f; }
 
-    // row r0 + i of a 32-row tile: token (r0 + i) / G.  Where G divides 32 its offset from the tile's first token is the same in every tile
-    Stage<DT, 32, 256> sq, so;
+    // row r0 + i of a tile: token (r0 + i) / G.  Where G divides QT its offset from the tile's first token is the same in every tile
+    Stage<DT, QT, 64 * W> sq, so;
     const long on = (long)a.H * a.D, oh = a.D;
     float rl = 0.0f;
     auto places = [&](int g0) {
 #pragma unroll
         for (int ch = 0; ch < sq.CH; ++ch) {
             const uint32_t rr = g0 + sq.row(ch), tok = quotient(rr, a.g_reciprocal), gg = rr - tok * a.G;
-            const bool ok = sq.col(ch) < a.D && (sq.EVEN || sq.row(ch) < 32);
+            const bool ok = sq.col(ch) < a.D && (sq.EVEN || sq.row(ch) < QT);
             sq.off[ch] = ok ? (tok * (uint32_t)a.q.sn + gg * (uint32_t)a.q.sh + sq.col(ch)) * 2 : FAR;
             so.off[ch] = ok ? (tok * (uint32_t)on + gg * (uint32_t)oh + sq.col(ch)) * 2 : FAR;
         }
     };
-    const bool same_places = 32 % a.G == 0;
+    const bool same_places = QT % a.G == 0;
     places(0);
     auto load = [&](int r0) {
         const int tok0 = (int)quotient((uint32_t)r0, a.g_reciprocal), left = a.R - r0;
         if (!same_places) places(r0 - tok0 * a.G);
-        const uint64_t bits = left >= 32 ? ~0ull : (1ull << left) - 1;
+        const uint64_t bits = left >= QT ? ~0ull : (1ull << left) - 1;
         sq.load(a.q.p + b * a.q.sb + tok0 * a.q.sn + (long)hk * a.G * a.q.sh, bits);
         so.load(a.dout + ((long)b * a.Nq + tok0) * on + (long)hk * a.G * oh, bits);
-        if (tid < 64) {
-            const int r = r0 + li;
-            rl = r < a.R ? (hh == 0 ? log2_of(lse[r]) : dlt[r]) : 0.0f;
+        if (tid < 2 * QT) {
+            const int r = r0 + tid % QT;
+            rl = r < a.R ? (tid < QT ? log2_of(lse[r]) : dlt[r]) : 0.0f;
         }
     };
     auto store = [&](int buf) {
         sq.store(Qs[buf]);
         so.store(Os[buf]);
-        if (tid < 32) Ls[buf][li] = rl;
-        else if (tid < 64) Ds[buf][li] = rl;
+        if (tid < QT) Ls[buf][tid] = rl;
+        else if (tid < 2 * QT) Ds[buf][tid - QT] = rl;
     };
 
     int t0, t1;
-    share(kbk * 128 < len ? (a.R + 31) / 32 : 0, split, SPLIT ? a.splits : 1, t0, t1);
+    share(kbk * 32 * W < len ? (a.R + QT - 1) / QT : 0, split, SPLIT ? a.splits : 1, t0, t1);
     if (t0 < t1) {
-        load(t0 * 32);
+        load(t0 * QT);
         store(0);
     }
     __syncthreads();
     for (int t = t0; t < t1; ++t) {
         const int cur = (t - t0) & 1;
-        if (t + 1 < t1) load(t * 32 + 32);
+        if (t + 1 < t1) load(t * QT + QT);
         if (wave_live) {
-            const short *Q = Qs[cur] + li * P + 8 * hh, *O = Os[cur] + li * P + 8 * hh, *Vw = Vs + (V_IN_LDS ? (wave * 32 + li) * P + 8 * hh : 0);
+#pragma unroll
+        for (int h = 0; h < QT / 32; ++h) {
+            if (h && t * QT + 32 * h >= a.R) break;
+            const short *Q = Qs[cur] + (32 * h + li) * P + 8 * hh, *O = Os[cur] + (32 * h + li) * P + 8 * hh, *Vw = Vs + (V_IN_LDS ? (wave * 32 + li) * P + 8 * hh : 0);
             f32x16 s, p;
 #pragma unroll
             for (int j = 0; j < 16; ++j) { s[j] = 0.0f; p[j] = 0.0f; }
@@ -599,8 +602,8 @@ __global__ __launch_bounds__(256, 2) void xattn_dkdv_kernel(Args a) {
             float e[16], d[16];
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                const float4 l4 = *reinterpret_cast<const float4 *>(&Ls[cur][8 * q + 4 * hh]);
-                const float4 d4 = *reinterpret_cast<const float4 *>(&Ds[cur][8 * q + 4 * hh]);
+                const float4 l4 = *reinterpret_cast<const float4 *>(&Ls[cur][32 * h + 8 * q + 4 * hh]);
+                const float4 d4 = *reinterpret_cast<const float4 *>(&Ds[cur][32 * h + 8 * q + 4 * hh]);
                 const float lv[4] = {l4.x, l4.y, l4.z, l4.w}, dl[4] = {d4.x, d4.y, d4.z, d4.w};
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -614,10 +617,11 @@ __global__ __launch_bounds__(256, 2) void xattn_dkdv_kernel(Args a) {
                 const bf16x8 pb = pack8(e + 8 * k), db = pack8(d + 8 * k);
 #pragma unroll
                 for (int q = 0; q < OT; ++q) {
-                    dv[q] = XA_MFMA(tr_frag<P>(ot, 16 * k, 32 * q), pb, dv[q]);
-                    dk[q] = XA_MFMA(tr_frag<P>(qt, 16 * k, 32 * q), db, dk[q]);
+                    dv[q] = XA_MFMA(tr_frag<P>(ot, 32 * h + 16 * k, 32 * q), pb, dv[q]);
+                    dk[q] = XA_MFMA(tr_frag<P>(qt, 32 * h + 16 * k, 32 * q), db, dk[q]);
                 }
             }
+        }
         }
         if (t + 1 < t1) store(cur ^ 1);
         __syncthreads();
@@ -686,7 +690,7 @@ int splits_for(long blocks, long steps, int least) {
 
 struct Sizes {
     long groups, R;
-    int fwd_splits, dq_splits, kv_splits;
+    int fwd_splits, dq_splits, kv_splits, kv_waves;
     size_t fwd_part, fwd_bytes, delta_bytes, bwd_bytes;
 };
 
@@ -694,7 +698,8 @@ Sizes sizes_of(int B, int Nq, int Nk, int H, int Hk, int D) {
     Sizes z;
     z.groups = (long)B * Hk;
     z.R = (long)Nq * (H / Hk);
-    const long rb = z.groups * tiles_of(z.R, 128), kb = z.groups * tiles_of(Nk, 128);
+    z.kv_waves = D > 96 && Nk > 128 ? 8 : 4;
+    const long rb = z.groups * tiles_of(z.R, 128), kb = z.groups * tiles_of(Nk, 32 * z.kv_waves);
     z.fwd_splits = splits_for(rb, tiles_of(Nk, 64), 4);
     z.dq_splits = splits_for(rb, tiles_of(Nk, 64), 4);
     z.kv_splits = splits_for(kb, tiles_of(z.R, 32), 8);
@@ -843,17 +848,22 @@ extern "C" int xq_xattn_backward(const void *q, const void *k, const void *v, co
         }
     }
     if (Nk > 0) {
-        plan_blocks(a, tiles_of(Nk, 128), z.kv_splits, blocks);
-        if (z.kv_splits > 1) {
-#define XA_CALL(DT) hipLaunchKernelGGL((xattn_dkdv_kernel<DT, true>), dim3(blocks), dim3(256), 0, s, a)
+        plan_blocks(a, tiles_of(Nk, 32 * z.kv_waves), z.kv_splits, blocks);
+#define XA_GO(DT, W)                                                                                                                  \
+    do {                                                                                                                              \
+        if (z.kv_splits > 1) hipLaunchKernelGGL((xattn_dkdv_kernel<DT, W, true>), dim3(blocks), dim3(64 * W), 0, s, a);               \
+        else hipLaunchKernelGGL((xattn_dkdv_kernel<DT, W, false>), dim3(blocks), dim3(64 * W), 0, s, a);                              \
+    } while (0)
+        if (z.kv_waves == 8) XA_GO(128, 8);
+        else {
+#define XA_CALL(DT) XA_GO(DT, 4)
             XA_BY_WIDTH(D, XA_CALL);
 #undef XA_CALL
+        }
+#undef XA_GO
+        if (z.kv_splits > 1) {
             const long total = 2 * z.groups * (long)Nk * (D / 4);
             hipLaunchKernelGGL((xattn_sum_kernel<1>), dim3((unsigned)((total + 255) / 256)), dim3(256), 0, s, a, D / 4, reciprocal_of(D / 4), total);
-        } else {
-#define XA_CALL(DT) hipLaunchKernelGGL((xattn_dkdv_kernel<DT, false>), dim3(blocks), dim3(256), 0, s, a)
-            XA_BY_WIDTH(D, XA_CALL);
-#undef XA_CALL
         }
     }
     return xq_check_launch(fn);
