@@ -61,17 +61,37 @@ __device__ __forceinline__ bf16x8 pack8(const float *s) {
 __device__ __forceinline__ float bf_lo(unsigned u) { return __uint_as_float(u << 16); }
 __device__ __forceinline__ float bf_hi(unsigned u) { return __uint_as_float(u & 0xffff0000u); }
 
-typedef short s4lds __attribute__((ext_vector_type(4)));
-__device__ __forceinline__ bf16x4 lds_tr4(const short *p) {
-    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((s4lds __attribute__((address_space(3))) *)p);
-}
-// A fragment of T^T for a row-major tile T of pitch P: contraction rows ROW0 + {4 hh .. + 3, 8 + 4 hh ..}, output rows = columns COL0 + (lane & 31);
-// the pointer carries the lane's part (trp below)
-template <int P>
-__device__ __forceinline__ bf16x8 tr_frag(const short *trp, int row0, int col0) {
-    const bf16x4 lo = lds_tr4(trp + row0 * P + col0), hi = lds_tr4(trp + (row0 + 8) * P + col0);
-    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-}
+// LDS by byte address (the swizzle below is a XOR on it)
+template <typename T> using lds_ptr = T __attribute__((address_space(3))) *;
+__device__ __forceinline__ uint32_t lds_address(const void *p) { return (uint32_t)(uintptr_t)(lds_ptr<const char>)p; }
+__device__ __forceinline__ bf16x8 lds_16(uint32_t at) { return *(lds_ptr<const bf16x8>)(uintptr_t)at; }
+__device__ __forceinline__ bf16x4 lds_tr(uint32_t at) { return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr<bf16x4>)(uintptr_t)at); }
+
+// A row-major bf16 tile in LDS, rows of 64, 128 or 256 bytes (96 columns lie in 256).  Chunk c (16 bytes) of row R is kept at chunk c ^ twist(R), so that both
+// ways of reading meet all 64 banks: 16 rows at one chunk (the operands over the head dimension) and 4 rows x 4 chunks (the transpose reads).  A pitch of
+// DT + 8 instead serves the first way only: half of the LDS cycles were conflicts (forward at 128 columns 536 us, now 483).
+template <int DT>
+struct Tile {
+    static constexpr int PITCH = DT > 64 ? 128 : DT, ROW = 2 * PITCH;
+    static __device__ __forceinline__ uint32_t twist(uint32_t r) {
+        if (DT > 64) return (r & 3) << 2 | (r >> 2 & 3);
+        if (DT > 32) return (r >> 1 & 1) << 2 | (r >> 2 & 3);
+        return r >> 2 & 3;
+    }
+    static __device__ __forceinline__ uint32_t place(uint32_t row, uint32_t chunk) { return row * ROW + ((chunk ^ twist(row)) << 4); }
+    // chunk 2 k + hh of row li (+ 16 n: the twist goes by R mod 16): base ^ 32 k
+    static __device__ __forceinline__ uint32_t row_base(int li, int hh) { return place(li, hh); }
+    // A fragment of the transposed tile: contraction rows row0 + {4 hh .. + 3, 8 + 4 hh ..} (row0 a multiple of 16), output rows = columns 32 q + (lane & 31).
+    // ds_read_b64_tr_b16: in each 16 lanes, lane i receives element i & 3 of the 8 bytes that lanes 4 j + (i >> 2) point at
+    static __device__ __forceinline__ uint32_t tr_base(int lane) {
+        const int row = 4 * (lane >> 5) + ((lane & 15) >> 2), chunk = 2 * (lane >> 4 & 1) + ((lane & 3) >> 1);
+        return place(row, chunk) + 8 * (lane & 1);
+    }
+    static __device__ __forceinline__ bf16x8 tr_frag(uint32_t base, int row0, int q) {
+        const bf16x4 lo = lds_tr((base ^ 64 * q) + row0 * ROW), hi = lds_tr((base ^ 64 * q ^ 32) + (row0 + 8) * ROW);      // twist(R + 8) = twist(R) ^ 2
+        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+};
 
 // v_max3_f32 without the operand canonicalisation that fmaxf() carries under IEEE mode
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -145,7 +165,7 @@ __device__ __forceinline__ long row_offset(const Args &a, const View &t, int b, 
 // ROWS rows into registers (CH 16-byte chunks a thread), then into a row-major LDS tile; a row whose bit is clear arrives as zeros
 template <int DT, int ROWS, int THREADS>
 struct Stage {
-    static constexpr int PER_ROW = DT / 8, CH = (ROWS * PER_ROW + THREADS - 1) / THREADS, P = DT + 8;
+    static constexpr int PER_ROW = DT / 8, CH = (ROWS * PER_ROW + THREADS - 1) / THREADS;
     static constexpr bool EVEN = ROWS * PER_ROW % THREADS == 0;
     uint32_t off[CH];
     uint4 r[CH];
@@ -164,10 +184,10 @@ struct Stage {
             for (int c = 0; c < CH; ++c) r[c] = load16(base, off[c]);
         }
     }
-    __device__ __forceinline__ void store(short *tile) const {
+    __device__ __forceinline__ void store(uint32_t tile) const {
 #pragma unroll
         for (int c = 0; c < CH; ++c)
-            if (EVEN || row(c) < ROWS) *reinterpret_cast<uint4 *>(tile + row(c) * P + col(c)) = r[c];
+            if (EVEN || row(c) < ROWS) *(lds_ptr<u32x4>)(uintptr_t)(tile + Tile<DT>::place(row(c), col(c) / 8)) = __builtin_bit_cast(u32x4, r[c]);
     }
 };
 
@@ -225,15 +245,16 @@ __device__ __forceinline__ void share(int n, int part, int parts, int &from, int
 // ---------------------------------------------------------------------------------------------------------------------------------------------
 template <int DT, bool SPLIT>
 __global__ __launch_bounds__(256, 2) void xattn_fwd_kernel(Args a) {
-    constexpr int P = DT + 8, KS = DT / 16, OT = DT / 32;
-    __shared__ __attribute__((aligned(16))) short Ks[2][64 * P];
-    __shared__ __attribute__((aligned(16))) short Vs[2][64 * P];
+    typedef Tile<DT> T;
+    constexpr int KS = DT / 16, OT = DT / 32, BYTES = 64 * T::ROW;
+    __shared__ __attribute__((aligned(256))) char tiles[4 * BYTES];         // K 0, K 1, V 0, V 1
+    const uint32_t Ks = lds_address(tiles), Vs = Ks + 2 * BYTES;
     int g, i;
     if (!map_block(a, g, i)) return;
     const int split = SPLIT ? i % a.splits : 0, rb = SPLIT ? i / a.splits : i;
     const int b = g / a.Hk, hk = g - b * a.Hk;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 31, hh = lane >> 5;
-    const int trp = (4 * hh + ((lane & 15) >> 2)) * P + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+    const uint32_t row_at = T::row_base(li, hh), tr_at = T::tr_base(lane);
     const int len = keys_of(a, b);
     const short *kb = a.k.p + b * a.k.sb + hk * a.k.sh, *vb = a.v.p + b * a.v.sb + hk * a.v.sh;
     const float c = a.scale * LOG2E;
@@ -267,8 +288,8 @@ __global__ __launch_bounds__(256, 2) void xattn_fwd_kernel(Args a) {
         sk.load(kb + t0 * 64L * a.k.sn, bits);
         sv.load(vb + t0 * 64L * a.v.sn, bits);
         keys.fetch(t0 * 64 + 64);
-        sk.store(Ks[0]);
-        sv.store(Vs[0]);
+        sk.store(Ks);
+        sv.store(Vs);
     }
     __syncthreads();
     for (int t = t0; t < t1; ++t) {
@@ -280,7 +301,7 @@ __global__ __launch_bounds__(256, 2) void xattn_fwd_kernel(Args a) {
             keys.fetch(t * 64 + 128);
         }
         if (wave_live && bits) {
-            const short *K = Ks[cur] + li * P + 8 * hh, *V = Vs[cur] + trp;
+            const uint32_t K = Ks + cur * BYTES + row_at, V = Vs + cur * BYTES + tr_at;
             const bool wide = (bits >> 32) != 0;           // the second 32 keys of the tile hold one at least
             f32x16 s[2];
 #pragma unroll
@@ -288,7 +309,7 @@ __global__ __launch_bounds__(256, 2) void xattn_fwd_kernel(Args a) {
                 s[h] = zero16;
                 if (h == 1 && !wide) continue;
 #pragma unroll
-                for (int k = 0; k < KS; ++k) s[h] = XA_MFMA(*reinterpret_cast<const bf16x8 *>(K + 32 * h * P + 16 * k), qf[k], s[h]);
+                for (int k = 0; k < KS; ++k) s[h] = XA_MFMA(lds_16((K ^ 32 * k) + 32 * h * T::ROW), qf[k], s[h]);
             }
             if (~bits) {
 #pragma unroll
@@ -330,15 +351,15 @@ __global__ __launch_bounds__(256, 2) void xattn_fwd_kernel(Args a) {
                 for (int k = 0; k < 2; ++k) {
                     const bf16x8 pk = pack8(p + 8 * k);
 #pragma unroll
-                    for (int q = 0; q < OT; ++q) o[q] = XA_MFMA(tr_frag<P>(V, 32 * h + 16 * k, 32 * q), pk, o[q]);
+                    for (int q = 0; q < OT; ++q) o[q] = XA_MFMA(T::tr_frag(V, 32 * h + 16 * k, q), pk, o[q]);
                     ls = XA_MFMA(ones, pk, ls);
                 }
             }
             l += ls[0];            // every row of ones x P^T is the sum over the tile's keys of this lane's row
         }
         if (t + 1 < t1) {
-            sk.store(Ks[cur ^ 1]);
-            sv.store(Vs[cur ^ 1]);
+            sk.store(Ks + (cur ^ 1) * BYTES);
+            sv.store(Vs + (cur ^ 1) * BYTES);
             bits = next;
         }
         __syncthreads();
@@ -388,15 +409,16 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(Args a, int per_row, un
 // ---------------------------------------------------------------------------------------------------------------------------------------------
 template <int DT, bool SPLIT>
 __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(Args a) {
-    constexpr int P = DT + 8, KS = DT / 16, OT = DT / 32;
-    __shared__ __attribute__((aligned(16))) short Ks[2][64 * P];
-    __shared__ __attribute__((aligned(16))) short Vs[2][64 * P];
+    typedef Tile<DT> T;
+    constexpr int KS = DT / 16, OT = DT / 32, BYTES = 64 * T::ROW;
+    __shared__ __attribute__((aligned(256))) char tiles[4 * BYTES];         // K 0, K 1, V 0, V 1
+    const uint32_t Ks = lds_address(tiles), Vs = Ks + 2 * BYTES;
     int g, i;
     if (!map_block(a, g, i)) return;
     const int split = SPLIT ? i % a.splits : 0, rb = SPLIT ? i / a.splits : i;
     const int b = g / a.Hk, hk = g - b * a.Hk;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 31, hh = lane >> 5;
-    const int trp = (4 * hh + ((lane & 15) >> 2)) * P + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+    const uint32_t row_at = T::row_base(li, hh), tr_at = T::tr_base(lane);
     const int len = keys_of(a, b);
     const short *kb = a.k.p + b * a.k.sb + hk * a.k.sh, *vb = a.v.p + b * a.v.sb + hk * a.v.sh;
     const float c = a.scale * LOG2E;
@@ -444,8 +466,8 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(Args a) {
         sk.load(kb + t0 * 64L * a.k.sn, bits);
         sv.load(vb + t0 * 64L * a.v.sn, bits);
         keys.fetch(t0 * 64 + 64);
-        sk.store(Ks[0]);
-        sv.store(Vs[0]);
+        sk.store(Ks);
+        sv.store(Vs);
     }
     __syncthreads();
     for (int t = t0; t < t1; ++t) {
@@ -457,7 +479,7 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(Args a) {
             keys.fetch(t * 64 + 128);
         }
         if (wave_live && bits) {
-            const short *K = Ks[cur] + li * P + 8 * hh, *V = Vs[cur] + li * P + 8 * hh, *T = Ks[cur] + trp;
+            const uint32_t K = Ks + cur * BYTES + row_at, V = Vs + cur * BYTES + row_at, KT = Ks + cur * BYTES + tr_at;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 if (h == 1 && !(bits >> 32)) continue;         // no valid key among the second 32
@@ -466,8 +488,8 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(Args a) {
                 for (int j = 0; j < 16; ++j) { s[j] = 0.0f; p[j] = 0.0f; }
 #pragma unroll
                 for (int k = 0; k < KS; ++k) {
-                    s = XA_MFMA(*reinterpret_cast<const bf16x8 *>(K + 32 * h * P + 16 * k), qf[k], s);
-                    p = XA_MFMA(*reinterpret_cast<const bf16x8 *>(V + 32 * h * P + 16 * k), df[k], p);
+                    s = XA_MFMA(lds_16((K ^ 32 * k) + 32 * h * T::ROW), qf[k], s);
+                    p = XA_MFMA(lds_16((V ^ 32 * k) + 32 * h * T::ROW), df[k], p);
                 }
                 const uint32_t w = (uint32_t)(bits >> (32 * h)) >> (4 * hh);
                 float d[16];
@@ -482,13 +504,13 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(Args a) {
                 for (int k = 0; k < 2; ++k) {
                     const bf16x8 dk = pack8(d + 8 * k);
 #pragma unroll
-                    for (int q = 0; q < OT; ++q) acc[q] = XA_MFMA(tr_frag<P>(T, 32 * h + 16 * k, 32 * q), dk, acc[q]);
+                    for (int q = 0; q < OT; ++q) acc[q] = XA_MFMA(T::tr_frag(KT, 32 * h + 16 * k, q), dk, acc[q]);
                 }
             }
         }
         if (t + 1 < t1) {
-            sk.store(Ks[cur ^ 1]);
-            sv.store(Vs[cur ^ 1]);
+            sk.store(Ks + (cur ^ 1) * BYTES);
+            sv.store(Vs + (cur ^ 1) * BYTES);
             bits = next;
         }
         __syncthreads();
@@ -506,20 +528,21 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(Args a) {
 // ---------------------------------------------------------------------------------------------------------------------------------------------
 template <int DT, int W, bool SPLIT>
 __global__ __launch_bounds__(64 * W, DT > 64 ? 2 : 3) void xattn_dkdv_kernel(Args a) {
-    constexpr int QT = 32, P = DT + 8, KS = DT / 16, OT = DT / 32;
-    __shared__ __attribute__((aligned(16))) short Qs[2][QT * P];
-    __shared__ __attribute__((aligned(16))) short Os[2][QT * P];
-    // a wave's own 32 rows of V: at 128 columns its fragments do not fit beside the accumulators in 256 registers (two waves a SIMD)
+    typedef Tile<DT> T;
+    // 64 rows a tile where eight waves fill the CU by themselves: half of the meetings (1140 us instead of 1169)
+    constexpr int QT = W == 8 ? 64 : 32, KS = DT / 16, OT = DT / 32, BYTES = QT * T::ROW;
+    // a wave's own 32 rows of V: only at 96 columns do its fragments stay in registers beside the accumulators (elsewhere that would cost a wave a SIMD)
     constexpr bool V_IN_LDS = DT != 96;
-    __shared__ __attribute__((aligned(16))) short Vs[V_IN_LDS ? 32 * W * P : 8];
+    __shared__ __attribute__((aligned(256))) char tiles[4 * BYTES + (V_IN_LDS ? 32 * W * T::ROW : 0)];      // q 0, q 1, dO 0, dO 1, v
     __shared__ __attribute__((aligned(16))) float Ls[2][QT];
     __shared__ __attribute__((aligned(16))) float Ds[2][QT];
+    const uint32_t Qs = lds_address(tiles), Os = Qs + 2 * BYTES, Vs = Qs + 4 * BYTES;
     int g, i;
     if (!map_block(a, g, i)) return;
     const int split = SPLIT ? i % a.splits : 0, kbk = SPLIT ? i / a.splits : i;
     const int b = g / a.Hk, hk = g - b * a.Hk;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, li = lane & 31, hh = lane >> 5;
-    const int trp = (4 * hh + ((lane & 15) >> 2)) * P + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+    const uint32_t row_at = T::row_base(li, hh), tr_at = T::tr_base(lane);
     const int len = keys_of(a, b);
     const float c = a.scale * LOG2E;
     const float *lse = a.lse + (long)g * a.R, *dlt = a.delta + (long)g * a.R;
@@ -533,7 +556,7 @@ __global__ __launch_bounds__(64 * W, DT > 64 ? 2 : 3) void xattn_dkdv_kernel(Arg
     load_row<DT>(a.v.p + b * a.v.sb + hk * a.v.sh + (long)nc * a.v.sn, a.D, hh, vf);
     if (V_IN_LDS) {
 #pragma unroll
-        for (int k = 0; k < KS; ++k) *reinterpret_cast<bf16x8 *>(Vs + (wave * 32 + li) * P + 8 * hh + 16 * k) = vf[k];
+        for (int k = 0; k < KS; ++k) *(lds_ptr<bf16x8>)(uintptr_t)(Vs + wave * 32 * T::ROW + (row_at ^ 32 * k)) = vf[k];
     }
 
     f32x16 dk[OT], dv[OT];
@@ -569,8 +592,8 @@ __global__ __launch_bounds__(64 * W, DT > 64 ? 2 : 3) void xattn_dkdv_kernel(Arg
         }
     };
     auto store = [&](int buf) {
-        sq.store(Qs[buf]);
-        so.store(Os[buf]);
+        sq.store(Qs + buf * BYTES);
+        so.store(Os + buf * BYTES);
         if (tid < QT) Ls[buf][tid] = rl;
         else if (tid < 2 * QT) Ds[buf][tid - QT] = rl;
     };
@@ -586,17 +609,17 @@ __global__ __launch_bounds__(64 * W, DT > 64 ? 2 : 3) void xattn_dkdv_kernel(Arg
         const int cur = (t - t0) & 1;
         if (t + 1 < t1) load(t * QT + QT);
         if (wave_live) {
-#pragma unroll
+#pragma unroll 1
         for (int h = 0; h < QT / 32; ++h) {
             if (h && t * QT + 32 * h >= a.R) break;
-            const short *Q = Qs[cur] + (32 * h + li) * P + 8 * hh, *O = Os[cur] + (32 * h + li) * P + 8 * hh, *Vw = Vs + (V_IN_LDS ? (wave * 32 + li) * P + 8 * hh : 0);
+            const uint32_t Qh = Qs + cur * BYTES + 32 * h * T::ROW, Oh = Qh + 2 * BYTES, Q = Qh + row_at, O = Oh + row_at, Vw = Vs + wave * 32 * T::ROW + row_at;
             f32x16 s, p;
 #pragma unroll
             for (int j = 0; j < 16; ++j) { s[j] = 0.0f; p[j] = 0.0f; }
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
-                s = XA_MFMA(*reinterpret_cast<const bf16x8 *>(Q + 16 * k), kf[k], s);
-                p = XA_MFMA(*reinterpret_cast<const bf16x8 *>(O + 16 * k), V_IN_LDS ? *reinterpret_cast<const bf16x8 *>(Vw + 16 * k) : vf[k], p);
+                s = XA_MFMA(lds_16(Q ^ 32 * k), kf[k], s);
+                p = XA_MFMA(lds_16(O ^ 32 * k), V_IN_LDS ? lds_16(Vw ^ 32 * k) : vf[k], p);
             }
             // register j <-> row (j & 3) + 8 (j >> 2) + 4 hh of the tile; rows behind the last have q = dO = 0 and lse = delta = 0: P is 1 there, dS 0
             float e[16], d[16];
@@ -611,14 +634,14 @@ __global__ __launch_bounds__(64 * W, DT > 64 ? 2 : 3) void xattn_dkdv_kernel(Arg
                     d[4 * q + j] = e[4 * q + j] * (p[4 * q + j] - dl[j]);
                 }
             }
-            const short *ot = Os[cur] + trp, *qt = Qs[cur] + trp;
+            const uint32_t ot = Oh + tr_at, qt = Qh + tr_at;
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 const bf16x8 pb = pack8(e + 8 * k), db = pack8(d + 8 * k);
 #pragma unroll
                 for (int q = 0; q < OT; ++q) {
-                    dv[q] = XA_MFMA(tr_frag<P>(ot, 32 * h + 16 * k, 32 * q), pb, dv[q]);
-                    dk[q] = XA_MFMA(tr_frag<P>(qt, 32 * h + 16 * k, 32 * q), db, dk[q]);
+                    dv[q] = XA_MFMA(T::tr_frag(ot, 16 * k, q), pb, dv[q]);
+                    dk[q] = XA_MFMA(T::tr_frag(qt, 16 * k, q), db, dk[q]);
                 }
             }
         }
