@@ -304,6 +304,7 @@ __global__ __launch_bounds__(256, 2) void xattn_fwd_kernel(Args a) {
             const uint32_t K = Ks + cur * BYTES + row_at, V = Vs + cur * BYTES + tr_at;
             const bool wide = (bits >> 32) != 0;           // the second 32 keys of the tile hold one at least
             f32x16 s[2];
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 s[h] = zero16;
@@ -311,6 +312,7 @@ __global__ __launch_bounds__(256, 2) void xattn_fwd_kernel(Args a) {
 #pragma unroll
                 for (int k = 0; k < KS; ++k) s[h] = XA_MFMA(lds_16((K ^ 32 * k) + 32 * h * T::ROW), qf[k], s[h]);
             }
+            __builtin_amdgcn_s_setprio(0);
             if (~bits) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {

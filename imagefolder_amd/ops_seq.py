@@ -3,6 +3,7 @@
 nn_ops.embedding and nn_ops.cross_attention; everything here takes tensors that live on an MI355X.  Every call enqueues on the current stream of its
 tensors' device and allocates its outputs and workspace there."""
 import ctypes
+import functools
 
 import torch
 
@@ -29,6 +30,11 @@ def _launch(name, device, *args):
 
 def _at(t):
     return None if t is None else t.data_ptr()
+
+
+def _wants_grad(*tensors):
+    """whether autograd has to see the call (an autograd node costs a small call as much as its kernel)"""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def _same_device(name, first, *others):
@@ -109,10 +115,22 @@ def dropout(x, p, key=None, residual=None):
     elif key.dtype != torch.int64 or tuple(key.shape) != (2,) or not key.is_contiguous():
         raise XqError(f"dropout: key is an int64 tensor of two values (got {key.dtype}, shape {tuple(key.shape)})")
     _same_device("dropout", x, residual, key)
+    if not _wants_grad(x, residual):
+        xd = x if _dense(x) else x.contiguous()
+        rd = None if residual is None else _like(residual, xd)
+        return _dropout(xd, rd, float(p), key, x.dtype if rd is None else rd.dtype)
     return DropoutFn.apply(x, residual, float(p), key)
 
 
 # ---- embedding -----------------------------------------------------------------------------------------------------------------------------
+
+def _embedding(ic, w, scale, dtype):
+    V, D = w.shape
+    y = torch.empty(*ic.shape, D, dtype=dtype, device=w.device)
+    _launch("xq_embedding_forward", w.device, ic.data_ptr(), ic.dtype == torch.int64, w.data_ptr(), w.dtype == torch.bfloat16, ic.numel(), V, D, scale,
+            y.data_ptr(), dtype == torch.bfloat16)
+    return y
+
 
 class EmbeddingFn(torch.autograd.Function):
     """y = scale * weight[idx] (xq_embedding_forward); the gradient of the table from the tokens sorted by row (xq_embedding_backward)."""
@@ -120,14 +138,9 @@ class EmbeddingFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, idx, weight, scale, skip, dtype):
         ic, w = idx.contiguous(), weight.detach().contiguous()
-        V, D = w.shape
-        y = torch.empty(*idx.shape, D, dtype=dtype, device=w.device)
-        _launch("xq_embedding_forward", w.device, ic.data_ptr(), ic.dtype == torch.int64, w.data_ptr(), w.dtype == torch.bfloat16, ic.numel(), V, D, scale,
-                y.data_ptr(), dtype == torch.bfloat16)
-        if ctx.needs_input_grad[1]:
-            ctx.save_for_backward(ic)
-            ctx.cfg = (V, D, scale, skip, w.dtype)
-        return y
+        ctx.save_for_backward(ic)
+        ctx.cfg = (*w.shape, scale, skip, w.dtype)
+        return _embedding(ic, w, scale, dtype)
 
     @staticmethod
     def backward(ctx, g):
@@ -157,6 +170,8 @@ def embedding(idx, weight, scale=1.0, padding_idx=None, dtype=None):
             raise XqError(f"embedding: padding_idx = {padding_idx} outside the table of {weight.shape[0]} rows")
         skip = padding_idx % weight.shape[0]
     _same_device("embedding", weight, idx)
+    if not _wants_grad(weight):
+        return _embedding(idx.contiguous(), weight.contiguous(), float(scale), dtype)
     return EmbeddingFn.apply(idx, weight, float(scale), skip, dtype)
 
 
@@ -171,35 +186,40 @@ def _rows(t):
     if (s[3] == 1 or t.shape[3] == 1) and not (s[0] | s[1] | s[2]) & 7 and not t.data_ptr() & 15 and s[1] <= 1 << 23 and s[2] <= 1 << 22:
         return t
     if t.is_contiguous() and not t.data_ptr() & 15:
-        return t                                       # (strides of dimensions of one element may be anything: see _strides)
+        return t                                       # (strides of dimensions of one element may be anything: _nine leaves them out)
     return t.clone(memory_format=torch.contiguous_format)
 
 
-def _strides(*views):
-    return _NINE(*[0 if n == 1 else st for t in views for n, st in zip(t.shape[:3], t.stride()[:3])])
+def _nine(shapes, strides):
+    return _NINE(*[0 if n == 1 else st for shape, stride in zip(shapes, strides) for n, st in zip(shape[:3], stride[:3])])
+
+
+@functools.lru_cache(maxsize=4096)
+def _xattn_plan(q, k, sq, sk, sv, sdq, sdk, sdv):
+    """by shapes and strides alone: the sizes and stride arrays of the C calls, and their workspaces' bytes"""
+    sizes = (q[0], q[1], k[1], q[2], k[2], q[3])
+    l = _lib.lib()
+    return (sizes, _nine((q, k, k), (sq, sk, sv)), l.xq_xattn_forward_workspace_bytes(*sizes),
+            l.xq_xattn_backward_workspace_bytes(*sizes) if sdq else 0, _nine((q, k, k), (sdq, sdk, sdv)) if sdq else None)
 
 
 def _xattn_forward(q, k, v, lens, mask, scale, want_lse):
-    B, Nq, H, D = q.shape
-    Nk, Hk = k.shape[1], k.shape[2]
-    out = torch.empty(B, Nq, H, D, dtype=q.dtype, device=q.device)
-    lse = torch.empty(B, Hk, Nq * (H // Hk), dtype=torch.float32, device=q.device) if want_lse else None
-    nbytes = _lib.lib().xq_xattn_forward_workspace_bytes(B, Nq, Nk, H, Hk, D)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    _launch("xq_xattn_forward", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), B, Nq, Nk, H, Hk, D, _strides(q, k, v), _at(lens),
-            lens is not None and lens.dtype == torch.int64, _at(mask), scale, out.data_ptr(), _at(lse), _at(ws), nbytes)
+    sizes, strides, nbytes, _, _ = _xattn_plan(q.shape, k.shape, q.stride(), k.stride(), v.stride(), None, None, None)
+    out = q.new_empty(q.shape)
+    lse = q.new_empty((sizes[0], sizes[4], sizes[1] * (sizes[3] // sizes[4])), dtype=torch.float32) if want_lse else None
+    ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    _launch("xq_xattn_forward", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), *sizes, strides, _at(lens), lens is not None and lens.dtype == torch.int64,
+            _at(mask), scale, out.data_ptr(), _at(lse), _at(ws), nbytes)
     return out, lse
 
 
 def _xattn_backward(q, k, v, out, g, lse, lens, mask, scale, dq, dk, dv):
-    B, Nq, H, D = q.shape
-    Nk, Hk = k.shape[1], k.shape[2]
-    g = _rows(g) if g.is_contiguous() else g.contiguous()
-    nbytes = _lib.lib().xq_xattn_backward_workspace_bytes(B, Nq, Nk, H, Hk, D)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    _launch("xq_xattn_backward", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), g.data_ptr(), lse.data_ptr(), B, Nq, Nk, H, Hk, D,
-            _strides(q, k, v), _at(lens), lens is not None and lens.dtype == torch.int64, _at(mask), scale, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-            _strides(dq, dk, dv), _at(ws), nbytes)
+    if not g.is_contiguous() or g.data_ptr() & 15:
+        g = g.clone(memory_format=torch.contiguous_format)
+    sizes, strides, _, nbytes, grad_strides = _xattn_plan(q.shape, k.shape, q.stride(), k.stride(), v.stride(), dq.stride(), dk.stride(), dv.stride())
+    ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    _launch("xq_xattn_backward", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), g.data_ptr(), lse.data_ptr(), *sizes, strides, _at(lens),
+            lens is not None and lens.dtype == torch.int64, _at(mask), scale, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), grad_strides, _at(ws), nbytes)
 
 
 class CrossAttentionFn(torch.autograd.Function):
@@ -208,18 +228,16 @@ class CrossAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, lens, mask, scale):
         q, k, v = _rows(q.detach()), _rows(k.detach()), _rows(v.detach())
-        grad = any(ctx.needs_input_grad)
-        out, lse = _xattn_forward(q, k, v, lens, mask, scale, grad)
-        if grad:
-            ctx.save_for_backward(q, k, v, out, lse, lens, mask)
-            ctx.scale = scale
+        out, lse = _xattn_forward(q, k, v, lens, mask, scale, True)
+        ctx.save_for_backward(q, k, v, out, lse, lens, mask)
+        ctx.scale = scale
         return out
 
     @staticmethod
     def backward(ctx, g):
         q, k, v, out, lse, lens, mask = ctx.saved_tensors
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        _xattn_backward(q, k, v, out, g.detach(), lse, lens, mask, ctx.scale, dq, dk, dv)
+        dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+        _xattn_backward(q, k, v, out, g, lse, lens, mask, ctx.scale, dq, dk, dv)
         return dq, dk, dv, None, None, None
 
 
@@ -284,4 +302,8 @@ def cross_attention(q, k, v, kv_lens=None, key_mask=None, scale=None):
     if q.shape[3] % 8 or q.shape[3] > 128:
         raise XqError(f"cross_attention: head dim {q.shape[3]} is not a multiple of 8 up to 128")
     _same_device("cross_attention", q, k, v, kv_lens, key_mask)
-    return CrossAttentionFn.apply(q, k, v, None if kv_lens is None else kv_lens.contiguous(), None if key_mask is None else key_mask.contiguous(), scale)
+    kv_lens = None if kv_lens is None else kv_lens.contiguous()
+    key_mask = None if key_mask is None else key_mask.contiguous()
+    if not _wants_grad(q, k, v):
+        return _xattn_forward(_rows(q), _rows(k), _rows(v), kv_lens, key_mask, scale, False)[0]
+    return CrossAttentionFn.apply(q, k, v, kv_lens, key_mask, scale)
