@@ -357,15 +357,15 @@ __device__ __forceinline__ void sum_rows(const TG *__restrict__ g, const uint32_
 #undef XQ_PIECE
 }
 
-// Groups of `lanes` threads.  Blocks [0, row_blocks): one row of at most `chunk` tokens each; the others: pieces of longer rows, piece 2 b (+ 1) being the
-// head (tail) of chunk b of the sorted positions -> part[piece][D].
+// Groups of `lanes` threads.  Blocks [0, piece_blocks): pieces of long rows (the longest work: begun first), piece 2 b (+ 1) being the head (tail) of chunk b of
+// the sorted positions -> part[piece][D]; the others: one row of at most `chunk` tokens each.
 template <typename TG, typename TW, int VEC>
 __global__ __launch_bounds__(256) void embed_sum_kernel(const TG *__restrict__ g, const uint32_t *__restrict__ order, const uint32_t *__restrict__ row_start,
                                                         const uint32_t *__restrict__ edge, long V, int D, int lanes, float scale, uint32_t chunk, long chunks,
-                                                        long row_blocks, TW *__restrict__ dw, float *__restrict__ part) {
+                                                        long piece_blocks, TW *__restrict__ dw, float *__restrict__ part) {
     const int lane = threadIdx.x % lanes, sub = threadIdx.x / lanes, groups = 256 / lanes;
-    if ((long)blockIdx.x >= row_blocks) {
-        const long id = ((long)blockIdx.x - row_blocks) * groups + sub, b = id >> 1;
+    if ((long)blockIdx.x < piece_blocks) {
+        const long id = (long)blockIdx.x * groups + sub, b = id >> 1;
         if (b >= chunks) return;
         const uint32_t valid = row_start[V];
         const uint64_t p0_ = (uint64_t)b * chunk;
@@ -386,7 +386,7 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const TG *__restrict__ g
         }
         return;
     }
-    const long v = (long)blockIdx.x * groups + sub;
+    const long v = ((long)blockIdx.x - piece_blocks) * groups + sub;
     if (v >= V) return;
     const uint32_t lo = row_start[v], hi = row_start[v + 1];
     if (hi - lo > chunk) return;
@@ -399,31 +399,46 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const TG *__restrict__ g
     }
 }
 
-// block b: the long row that begins in chunk b (there is at most one: it goes on behind the chunk's end).  Its pieces are shared out over the waves in order
-// (each a chain of its own), the waves' sums meet in order.
+// Chunks 8 b .. 8 b + 7, one a wave: the long row that begins in it (there is at most one: it goes on behind the chunk's end), its pieces added in order.  A row of
+// more than 16 pieces is shared out over the block's waves (runs of pieces in order, a chain each; the waves' sums meet in order); of those, eight chunks hold
+// the beginning of one at most.
 template <typename TW>
 __global__ __launch_bounds__(512) void embed_long_kernel(const float *__restrict__ part, const uint32_t *__restrict__ row_start,
-                                                         const uint32_t *__restrict__ edge, long V, int D, float scale, uint32_t chunk,
+                                                         const uint32_t *__restrict__ edge, long V, int D, float scale, uint32_t chunk, long chunks,
                                                          TW *__restrict__ dw) {
     __shared__ float sums[8][64];
-    const uint32_t valid = row_start[V];
-    const uint64_t p0 = (uint64_t)blockIdx.x * chunk;
-    if (p0 + chunk >= valid) return;             // nothing goes on behind the last chunk
-    const long v = edge[2 * (long)blockIdx.x + 1];
-    const uint32_t s = row_start[v], e = row_start[v + 1];
-    if (!(e - s > chunk && s >= p0)) return;
+    __shared__ int heavy;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    // piece 0: the tail of this chunk; piece k: the head of chunk blockIdx.x + k
-    const long b0 = blockIdx.x, pieces = (long)((e - 1) / chunk) - b0 + 1, per = (pieces + 7) / 8;
-    const long k0 = wave * per, k1 = min(pieces, k0 + per);
+    if (threadIdx.x == 0) heavy = -1;
+    __syncthreads();
+    // piece 0: the tail of chunk b; piece k: the head of chunk b + k
+    auto add = [&](long b, long k0, long k1, int c) {
+        float acc = 0.0f;
+#pragma unroll 8
+        for (long k = k0; k < k1; ++k) acc += part[(2 * (b + k) + (k == 0)) * (long)D + c];
+        return acc;
+    };
+    auto pieces_of = [&](long b, long &v) -> long {
+        const uint64_t p0 = (uint64_t)b * chunk;
+        if (b >= chunks || p0 + chunk >= row_start[V]) return 0;         // nothing goes on behind the last chunk
+        v = edge[2 * b + 1];
+        const uint32_t s = row_start[v], e = row_start[v + 1];
+        return e - s > chunk && s >= p0 ? (long)((e - 1) / chunk) - b + 1 : 0;
+    };
+    const long mine = (long)blockIdx.x * 8 + wave;
+    long v = 0;
+    const long pieces = pieces_of(mine, v);
+    if (pieces > 16) {
+        if (lane == 0) heavy = wave;
+    } else if (pieces > 0) {
+        for (int c = blockIdx.y * 64 + lane; c < D; c += 64 * gridDim.y) dw[v * D + c] = from_f<TW>(add(mine, 0, pieces, c) * scale);
+    }
+    __syncthreads();
+    if (heavy < 0) return;
+    const long b = (long)blockIdx.x * 8 + heavy, all = pieces_of(b, v), per = (all + 7) / 8, k0 = wave * per, k1 = min(all, k0 + per);
     for (int c0 = blockIdx.y * 64; c0 < D; c0 += 64 * gridDim.y) {
         const int c = c0 + lane;
-        float acc = 0.0f;
-        if (c < D) {
-#pragma unroll 8
-            for (long k = k0; k < k1; ++k) acc += part[(2 * (b0 + k) + (k == 0)) * (long)D + c];
-        }
-        sums[wave][lane] = acc;
+        sums[wave][lane] = c < D ? add(b, k0, k1, c) : 0.0f;
         __syncthreads();
         if (wave == 0 && c < D) {
             float t = 0.0f;
@@ -515,14 +530,14 @@ void launch_sums(const void *g, long V, int D, float scale, const Plan &p, const
         const int lanes = pow2_lanes(D, VEC), groups = 256 / lanes;                                                                          \
         const long rb = (V + groups - 1) / groups, pb = (2 * p.chunks + groups - 1) / groups;                                                \
         hipLaunchKernelGGL((embed_sum_kernel<TG, TW, VEC>), dim3((unsigned)(rb + pb)), dim3(256), 0, s, (const TG *)g, order, rows, edge, V, D, \
-                           lanes, scale, 1u << p.chunk_bits, p.chunks, rb, (TW *)dw, part);                                                  \
+                           lanes, scale, 1u << p.chunk_bits, p.chunks, pb, (TW *)dw, part);                                                  \
     }
     if (a16 && D % 8 == 0 && sizeof(TG) == 2) XQ_SUM(8)
     else if (a16 && D % 4 == 0 && sizeof(TG) == 4) XQ_SUM(4)
     else XQ_SUM(1)
 #undef XQ_SUM
-    hipLaunchKernelGGL((embed_long_kernel<TW>), dim3((unsigned)p.chunks, (unsigned)std::min(8, (D + 63) / 64)), dim3(512), 0, s, part, rows, edge, V, D,
-                       scale, 1u << p.chunk_bits, (TW *)dw);
+    hipLaunchKernelGGL((embed_long_kernel<TW>), dim3((unsigned)((p.chunks + 7) / 8), (unsigned)std::min(8, (D + 63) / 64)), dim3(512), 0, s, part, rows, edge,
+                       V, D, scale, 1u << p.chunk_bits, p.chunks, (TW *)dw);
 }
 
 template <typename TW>

@@ -78,10 +78,8 @@ class DropoutFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, residual, p, key):
-        xd = x.detach()
-        if not _dense(xd):
-            xd = xd.contiguous()
-        rd = None if residual is None else _like(residual.detach(), xd)
+        xd = x if _dense(x) else x.contiguous()
+        rd = None if residual is None else _like(residual, xd)
         ctx.save_for_backward(key)
         ctx.cfg = (p, xd.dtype, xd.stride())
         return _dropout(xd, rd, p, key, xd.dtype if rd is None else rd.dtype)
@@ -92,9 +90,9 @@ class DropoutFn(torch.autograd.Function):
         p, dtype, stride = ctx.cfg
         dx = None
         if ctx.needs_input_grad[0]:
-            gd = g.detach()
+            gd = g
             if gd.stride() != stride:                  # the mask belongs to places in memory: the gradient has to lie as x did
-                gd = torch.empty_strided(g.shape, stride, dtype=g.dtype, device=g.device).copy_(gd)
+                gd = torch.empty_strided(g.shape, stride, dtype=g.dtype, device=g.device).copy_(g)
             dx = _dropout(gd, None, p, key, dtype)
         return dx, (g if ctx.needs_input_grad[1] else None), None, None
 
@@ -126,10 +124,15 @@ def dropout(x, p, key=None, residual=None):
 
 def _embedding(ic, w, scale, dtype):
     V, D = w.shape
-    y = torch.empty(*ic.shape, D, dtype=dtype, device=w.device)
+    y = w.new_empty((*ic.shape, D), dtype=dtype)
     _launch("xq_embedding_forward", w.device, ic.data_ptr(), ic.dtype == torch.int64, w.data_ptr(), w.dtype == torch.bfloat16, ic.numel(), V, D, scale,
             y.data_ptr(), dtype == torch.bfloat16)
     return y
+
+
+@functools.lru_cache(maxsize=4096)
+def _embedding_workspace(N, V, D):
+    return _lib.lib().xq_embedding_backward_workspace_bytes(N, V, D)
 
 
 class EmbeddingFn(torch.autograd.Function):
@@ -137,7 +140,7 @@ class EmbeddingFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, idx, weight, scale, skip, dtype):
-        ic, w = idx.contiguous(), weight.detach().contiguous()
+        ic, w = idx.contiguous(), weight.contiguous()
         ctx.save_for_backward(ic)
         ctx.cfg = (*w.shape, scale, skip, w.dtype)
         return _embedding(ic, w, scale, dtype)
@@ -146,11 +149,11 @@ class EmbeddingFn(torch.autograd.Function):
     def backward(ctx, g):
         (ic,) = ctx.saved_tensors
         V, D, scale, skip, wdtype = ctx.cfg
-        gc = g.detach().contiguous()
-        dw = torch.empty(V, D, dtype=wdtype, device=g.device)
+        gc = g.contiguous()
+        dw = gc.new_empty((V, D), dtype=wdtype)
         N = ic.numel()
-        nbytes = _lib.lib().xq_embedding_backward_workspace_bytes(N, V, D)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=g.device) if nbytes else None
+        nbytes = _embedding_workspace(N, V, D)
+        ws = gc.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
         _launch("xq_embedding_backward", gc.device, ic.data_ptr(), ic.dtype == torch.int64, gc.data_ptr(), gc.dtype == torch.bfloat16, N, V, D, scale, skip,
                 dw.data_ptr(), wdtype == torch.bfloat16, _at(ws), nbytes)
         return None, dw, None, None, None
@@ -227,7 +230,7 @@ class CrossAttentionFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, lens, mask, scale):
-        q, k, v = _rows(q.detach()), _rows(k.detach()), _rows(v.detach())
+        q, k, v = _rows(q), _rows(k), _rows(v)
         out, lse = _xattn_forward(q, k, v, lens, mask, scale, True)
         ctx.save_for_backward(q, k, v, out, lse, lens, mask)
         ctx.scale = scale
