@@ -379,6 +379,160 @@ __global__ __launch_bounds__(256, 2) void xattn_fwd_kernel(Args a) {
     }
 }
 
+// ---------------------------------------------------------------------------------------------------------------------------------------------
+// forward of at most 32 rows a kv head over at most 1024 keys (serving: one token, its heads, one image's or text's states): the four waves share out the keys,
+// each with its own 32-key tiles and no meeting with the others until their results are joined.  K and V go through LDS tiles of the wave's own (loads of whole
+// rows), fetched a tile ahead.  Bound by latency: one token over 257 keys, 12 heads of 64, takes 6.9 us (in the tiles of the many-row kernel, where one
+// wave of four has rows, 8.8).  Over more keys the many-row kernel with its keys split over blocks reads as fast (16 samples over 4056 .. 8111 keys: 82 us, here
+// 84) and a block's share is no longer one wave's chain.
+// ---------------------------------------------------------------------------------------------------------------------------------------------
+template <int DT>
+__global__ __launch_bounds__(256, 2) void xattn_few_rows_kernel(Args a) {
+    typedef Tile<DT> T;
+    constexpr int KS = DT / 16, OT = DT / 32, PER_ROW = DT / 8, CH = 32 * PER_ROW / 64, BYTES = 32 * T::ROW, PITCH = DT + 4;
+    constexpr int JOIN = 4 * 32 * PITCH * 4;
+    __shared__ __attribute__((aligned(256))) char mem[JOIN > 8 * BYTES ? JOIN : 8 * BYTES];       // the waves' K and V tiles, then their results
+    __shared__ float2 stat[4][32];
+    const int g = blockIdx.x;
+    const int b = g / a.Hk, hk = g - b * a.Hk;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 31, hh = lane >> 5;
+    const uint32_t Kw = lds_address(mem) + 2 * wave * BYTES, Vw = Kw + BYTES, row_at = Kw + T::row_base(li, hh), tr_at = Vw + T::tr_base(lane);
+    const int len = keys_of(a, b);
+    const short *kb = a.k.p + b * a.k.sb + hk * a.k.sh, *vb = a.v.p + b * a.v.sb + hk * a.v.sh;
+    const float c = a.scale * LOG2E;
+    bf16x8 qf[KS];
+    load_row<DT>(a.q.p + row_offset(a, a.q, b, hk, li < a.R ? li : a.R - 1), a.D, hh, qf);
+
+    uint32_t k_at[CH], v_at[CH];
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+        const int id = lane + 64 * i, row = id / PER_ROW, col = id % PER_ROW * 8;
+        k_at[i] = col < a.D ? (uint32_t)(row * (int)a.k.sn + col) * 2 : FAR;
+        v_at[i] = col < a.D ? (uint32_t)(row * (int)a.v.sn + col) * 2 : FAR;
+    }
+    KeyBits keys = {a.mask ? a.mask + (long)b * a.Nk : nullptr, len, 0};
+    uint4 kr[CH], vr[CH];
+    auto load = [&](int t, uint32_t bits) {
+        const short *K = kb + t * 32L * a.k.sn, *V = vb + t * 32L * a.v.sn;
+        if (~bits) {
+#pragma unroll
+            for (int i = 0; i < CH; ++i) {
+                const bool on = (bits >> ((lane + 64 * i) / PER_ROW)) & 1;
+                kr[i] = load16(K, on ? k_at[i] : FAR);
+                vr[i] = load16(V, on ? v_at[i] : FAR);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < CH; ++i) kr[i] = load16(K, k_at[i]);
+#pragma unroll
+            for (int i = 0; i < CH; ++i) vr[i] = load16(V, v_at[i]);
+        }
+    };
+
+    f32x16 o[OT];
+#pragma unroll
+    for (int t = 0; t < OT; ++t)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[t][j] = 0.0f;
+    float m = -INFINITY, l = 0.0f;
+    const bf16x8 ones = {0x3F80, 0x3F80, 0x3F80, 0x3F80, 0x3F80, 0x3F80, 0x3F80, 0x3F80};
+    const f32x16 zero16 = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    const int t0 = wave, t1 = (len + 31) / 32;
+    uint32_t bits = 0, next = 0;
+    if (t0 < t1) {
+        keys.fetch(t0 * 32);
+        bits = (uint32_t)keys.take(t0 * 32);
+        load(t0, bits);
+        keys.fetch(t0 * 32 + 128);
+    }
+    for (int t = t0; t < t1; t += 4) {
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+            const int id = lane + 64 * i;
+            const uint32_t at = T::place(id / PER_ROW, id % PER_ROW);
+            *(lds_ptr<u32x4>)(uintptr_t)(Kw + at) = __builtin_bit_cast(u32x4, kr[i]);
+            *(lds_ptr<u32x4>)(uintptr_t)(Vw + at) = __builtin_bit_cast(u32x4, vr[i]);
+        }
+        if (t + 4 < t1) {
+            next = (uint32_t)keys.take(t * 32 + 128);
+            load(t + 4, next);
+            keys.fetch(t * 32 + 256);
+        }
+        f32x16 s = zero16;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) s = XA_MFMA(lds_16(row_at ^ 32 * k), qf[k], s);
+        if (~bits) {
+            const uint32_t w = bits >> (4 * hh);
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+                if (!((w >> ((j & 3) + 8 * (j >> 2))) & 1u)) s[j] = -INFINITY;
+        }
+        float mx = max3(s[0], s[1], s[2]);
+#pragma unroll
+        for (int j = 3; j < 15; j += 2) mx = max3(mx, s[j], s[j + 1]);
+        mx = max3(mx, s[15], s[15]);
+        mx = max3(mx, __shfl_xor(mx, 32), mx);
+        const float cand = mx * c;
+        if (__any(cand > m + 8.0f)) {
+            const float mn = fmaxf(m, cand);
+            const float alpha = m == mn ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= alpha;
+#pragma unroll
+            for (int q = 0; q < OT; ++q)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) o[q][j] *= alpha;
+        }
+        const float mref = m == -INFINITY ? 0.0f : m;
+        float p[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) p[j] = __builtin_amdgcn_exp2f(fmaf(s[j], c, -mref));
+        f32x16 ls = zero16;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const bf16x8 pk = pack8(p + 8 * k);
+#pragma unroll
+            for (int q = 0; q < OT; ++q) o[q] = XA_MFMA(T::tr_frag(tr_at, 16 * k, q), pk, o[q]);
+            ls = XA_MFMA(ones, pk, ls);
+        }
+        l += ls[0];
+        bits = next;
+    }
+    __syncthreads();
+    float *sum = reinterpret_cast<float *>(mem);
+    if (li < a.R) {
+        float *row = sum + (wave * 32 + li) * PITCH;
+#pragma unroll
+        for (int t = 0; t < OT; ++t)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                *reinterpret_cast<float4 *>(row + 32 * t + 8 * q + 4 * hh) = make_float4(o[t][4 * q], o[t][4 * q + 1], o[t][4 * q + 2], o[t][4 * q + 3]);
+        if (hh == 0) stat[wave][li] = make_float2(m, l);
+    }
+    __syncthreads();
+    const int per_row = a.D / 4;
+    for (int id = threadIdx.x; id < a.R * per_row; id += 256) {
+        const int r = id / per_row, col = (id - r * per_row) * 4;
+        float M = -INFINITY, L = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) M = fmaxf(M, stat[w][r].x);
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float2 ml = stat[w][r];
+            const float f = ml.x == M ? 1.0f : __builtin_amdgcn_exp2f(ml.x - M);
+            const float4 y = *reinterpret_cast<const float4 *>(sum + (w * 32 + r) * PITCH + col);
+            L = fmaf(ml.y, f, L);
+            x.x = fmaf(y.x, f, x.x); x.y = fmaf(y.y, f, x.y); x.z = fmaf(y.z, f, x.z); x.w = fmaf(y.w, f, x.w);
+        }
+        const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+        const uint32_t tok = quotient((uint32_t)r, a.g_reciprocal), gg = (uint32_t)r - tok * a.G;
+        *reinterpret_cast<uint2 *>(a.out + (((long)b * a.Nq + tok) * a.H + hk * a.G + gg) * a.D + col) =
+            make_uint2(pack_bf16(x.x * inv, x.y * inv), pack_bf16(x.z * inv, x.w * inv));
+        if (a.lse && col == 0) a.lse[(long)g * a.R + r] = L == 0.0f ? -INFINITY : (M + __builtin_amdgcn_logf(L)) * LN2;
+    }
+}
+
 // the slabs of a split over keys: O = sum_s w_s O_s / sum_s w_s l_s, w_s = 2^(m_s - max m); four columns a thread
 __global__ __launch_bounds__(256) void xattn_join_kernel(Args a, int per_row, unsigned long long row_reciprocal, long total) {
     const long id = (long)blockIdx.x * 256 + threadIdx.x;
@@ -716,6 +870,7 @@ int splits_for(long blocks, long steps, int least) {
 struct Sizes {
     long groups, R;
     int fwd_splits, dq_splits, kv_splits, kv_waves;
+    bool few_rows;
     size_t fwd_part, fwd_bytes, delta_bytes, bwd_bytes;
 };
 
@@ -725,7 +880,8 @@ Sizes sizes_of(int B, int Nq, int Nk, int H, int Hk, int D) {
     z.R = (long)Nq * (H / Hk);
     z.kv_waves = D > 96 && Nk > 128 ? 8 : 4;
     const long rb = z.groups * tiles_of(z.R, 128), kb = z.groups * tiles_of(Nk, 32 * z.kv_waves);
-    z.fwd_splits = splits_for(rb, tiles_of(Nk, 64), 4);
+    z.few_rows = z.R <= 32 && Nk <= 1024;
+    z.fwd_splits = z.few_rows ? 1 : splits_for(rb, tiles_of(Nk, 64), 4);
     z.dq_splits = splits_for(rb, tiles_of(Nk, 64), 4);
     z.kv_splits = splits_for(kb, tiles_of(z.R, 32), 8);
     const size_t rows = (size_t)z.groups * z.R;
@@ -815,16 +971,22 @@ extern "C" int xq_xattn_forward(const void *q, const void *k, const void *v, int
     a.part = (float *)workspace; a.stat = (float *)((char *)workspace + z.fwd_part);
     unsigned blocks;
     plan_blocks(a, tiles_of(z.R, 128), z.fwd_splits, blocks);
-    if (z.fwd_splits > 1) {
-#define XA_CALL(DT) hipLaunchKernelGGL((xattn_fwd_kernel<DT, true>), dim3(blocks), dim3(256), 0, s, a)
+    if (z.few_rows) {
+#define XA_CALL(DT) hipLaunchKernelGGL((xattn_few_rows_kernel<DT>), dim3((unsigned)z.groups), dim3(256), 0, s, a)
         XA_BY_WIDTH(D, XA_CALL);
 #undef XA_CALL
+    } else {
+#define XA_CALL(DT)                                                                                                              \
+        do {                                                                                                                     \
+            if (z.fwd_splits > 1) hipLaunchKernelGGL((xattn_fwd_kernel<DT, true>), dim3(blocks), dim3(256), 0, s, a);            \
+            else hipLaunchKernelGGL((xattn_fwd_kernel<DT, false>), dim3(blocks), dim3(256), 0, s, a);                            \
+        } while (0)
+        XA_BY_WIDTH(D, XA_CALL);
+#undef XA_CALL
+    }
+    if (z.fwd_splits > 1) {
         const long total = z.groups * z.R * (D / 4);
         hipLaunchKernelGGL(xattn_join_kernel, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, s, a, D / 4, reciprocal_of(D / 4), total);
-    } else {
-#define XA_CALL(DT) hipLaunchKernelGGL((xattn_fwd_kernel<DT, false>), dim3(blocks), dim3(256), 0, s, a)
-        XA_BY_WIDTH(D, XA_CALL);
-#undef XA_CALL
     }
     return xq_check_launch(fn);
 }
