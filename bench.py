@@ -35,6 +35,7 @@ import argparse
 import ctypes
 import json
 import os
+import subprocess
 import sys
 import time
 
@@ -431,7 +432,8 @@ def main():
                 # the eager step that follows dies with hipErrorStreamCaptureInvalidated) — start over in a fresh process, eagerly
                 sys.stderr.write(f"bench.py: hipGraph capture failed ({type(e).__name__}: {str(e)[:300]}); re-running with --graph off\n")
                 sys.stderr.flush()
-                os.execv(sys.executable, [sys.executable] + sys.argv + ["--graph", "off"])
+                # as a child, not by exec: this process has initialised the GPU
+                sys.exit(subprocess.run([sys.executable] + sys.argv + ["--graph", "off"]).returncode)
     run = captured.replay if captured is not None else step
     torch.cuda.synchronize()
     if use_dist:
