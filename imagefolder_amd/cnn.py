@@ -45,7 +45,7 @@ class ResnetBlock(nn.Module):
 
     def forward(self, x):
         h = _conv(self.conv1, _norm_act(self.norm1, x))
-        h = _conv(self.conv2, self.dropout(_norm_act(self.norm2, h)))
+        h = _conv(self.conv2, nn_ops.module_dropout(self.dropout, _norm_act(self.norm2, h)))
         if self.in_channels != self.out_channels:
             x = _conv(self.conv_shortcut if self.use_conv_shortcut else self.nin_shortcut, x)
         return x + h

@@ -45,6 +45,9 @@ FUSED_BLOCKS = True
 # and the choice is logged once.
 F32_TRAIN_LINEAR = __import__("os").environ.get("XQ_F32_TRAIN_LINEAR", "0") == "1"
 _f32_train_logged = False
+# the nn.Dropout of a training CNN block (dropout_p > 0) through nn_ops.dropout: no stored mask, and a mask of its own at every replay of a captured step.
+# OFF by default: the masks differ from ATen's for the same torch.manual_seed (same distribution, p to a multiple of 2^-16).  XQ_COUNTER_DROPOUT=1 selects it.
+COUNTER_DROPOUT = __import__("os").environ.get("XQ_COUNTER_DROPOUT", "0") == "1"
 
 
 def _f32_train_note():
@@ -340,6 +343,13 @@ def dropout(x, p=0.5, training=True, key=None, residual=None):
         return y if residual is None else y + residual
     IMPL["dropout"] = "hip"
     return ops_seq.dropout(x, p, key, residual)
+
+
+def module_dropout(module, x):
+    """an nn.Dropout inside a model: the module itself, or nn_ops.dropout where COUNTER_DROPOUT is on and it would drop something on the GPU"""
+    if COUNTER_DROPOUT and module.training and module.p > 0 and x.is_cuda and x.dtype in (torch.bfloat16, torch.float32):
+        return dropout(x, module.p)
+    return module(x)
 
 
 def embedding(idx, weight, scale=1.0, padding_idx=None, dtype=None):

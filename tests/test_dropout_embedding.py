@@ -461,3 +461,73 @@ def test_on_the_cpu_they_are_the_plain_operators():
     assert torch.equal(y, w[idx] * 2)
     (dw,) = torch.autograd.grad(y.sum(), [w])
     assert torch.equal(dw, torch.tensor([0., 4., 2., 0., 0., 0.])[:, None].expand(6, 4))
+
+
+# ---- the framework's own paths -------------------------------------------------------------------------------------------------------------
+
+@gpu
+def test_cnn_block_with_the_counter_based_dropout(monkeypatch):
+    """ResnetBlock(dropout > 0): off by default (the module's own dropout); on, a bf16 training step runs on the kernel, channels-last, and its gradient is that of the same
+    block with the mask as a constant factor (what the block computes is the same operators on the same values: equal bits)"""
+    from imagefolder_amd import nn_ops
+    from imagefolder_amd.cnn import ResnetBlock
+    torch.manual_seed(4)
+    block = ResnetBlock(128, 128, dropout=0.25).cuda().train()
+    x = torch.randn(2, 128, 16, 16, device="cuda").to(BF).contiguous(memory_format=torch.channels_last).requires_grad_(True)
+    nn_ops.IMPL.pop("dropout", None)
+    with torch.autocast("cuda", torch.bfloat16):
+        block(x)
+    assert "dropout" not in nn_ops.IMPL
+    monkeypatch.setattr(nn_ops, "COUNTER_DROPOUT", True)
+    seen = {}
+    own = nn_ops.dropout
+
+    def spy(t, p, *a, **k):
+        seen["key"] = torch.tensor([3, 4], device="cuda")
+        seen["like"] = t.detach()
+        return own(t, p, key=seen["key"])
+
+    monkeypatch.setattr(nn_ops, "dropout", spy)
+    with torch.autocast("cuda", torch.bfloat16):
+        y = block(x)
+    assert nn_ops.IMPL["dropout"] == "hip"
+    g = torch.randn_like(y)
+    got = torch.autograd.grad(y, [x, block.conv1.weight, block.conv2.weight], g)
+    keep = own(torch.ones_like(seen["like"], dtype=F32), 0.25, key=seen["key"])
+    assert seen["like"].stride() == keep.stride() and 0.2 < float((keep == 0).float().mean()) < 0.3
+
+    class Fixed(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, t):
+            return (t.float() * keep).to(t.dtype)
+
+        @staticmethod
+        def backward(ctx, d):
+            return (d.float() * keep).to(d.dtype)
+
+    monkeypatch.setattr(nn_ops, "module_dropout", lambda m, t: Fixed.apply(t))
+    with torch.autocast("cuda", torch.bfloat16):
+        z = block(x)
+    want = torch.autograd.grad(z, [x, block.conv1.weight, block.conv2.weight], g)
+    assert torch.equal(y, z) and all(torch.equal(a, b) for a, b in zip(got, want))
+    block.eval()
+    nn_ops.IMPL.pop("dropout", None)
+    with torch.no_grad(), torch.autocast("cuda", torch.bfloat16):
+        block(x)
+    assert "dropout" not in nn_ops.IMPL
+
+
+@gpu
+def test_level_embedding_of_the_tokenizer_runs_on_the_lookup():
+    from imagefolder_amd import nn_ops
+    from imagefolder_amd.dino_enc.dinov2 import DINOv2Encoder
+    torch.manual_seed(0)
+    enc = DINOv2Encoder(in_channels=3, num_latent_tokens=16, product_quant=1, model_name="vit_base_patch14_dinov2.lvd142m", pretrained=False, abs_pos_embed=True,
+                        tuning_method="full",
+                        model_kwargs={'img_size': 64, 'patch_size': 8, 'drop_path_rate': 0.0, 'embed_dim': 64, 'depth': 2, 'num_heads': 1}).cuda()
+    nn_ops.IMPL.pop("embedding", None)
+    seq = enc._assemble(torch.randn(2, 64, 64, device="cuda"))
+    assert nn_ops.IMPL["embedding"] == "hip"
+    g = torch.randn_like(seq)
+    (dw,) = torch.autograd.grad(seq, [enc.lvl_embed.weight], g)
+    check_gradient(enc.lvl1LC, g.sum(0, keepdim=True), enc.lvl_embed.weight.shape[0], 1.0, dw)
