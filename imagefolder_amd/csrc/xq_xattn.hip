@@ -689,6 +689,9 @@ __global__ __launch_bounds__(64 * W, DT > 64 ? 2 : 3) void xattn_dkdv_kernel(Arg
     constexpr int QT = W == 8 ? 64 : 32, KS = DT / 16, OT = DT / 32, BYTES = QT * T::ROW;
     // a wave's own 32 rows of V: only at 96 columns do its fragments stay in registers beside the accumulators (elsewhere that would cost a wave a SIMD)
     constexpr bool V_IN_LDS = DT != 96;
+    // at 128 columns the products begin at -lse / scale and -delta instead of zero (two operations a score less: 1135 -> 1082 us at 4 x 4096 x 4352 x 16); at 64 the
+    // wait for the two before the first product costs more than that (121 -> 140 us at 128 x 256 x 257 x 12)
+    constexpr bool BEGIN = DT > 96;
     __shared__ __attribute__((aligned(256))) char tiles[4 * BYTES + (V_IN_LDS ? 32 * W * T::ROW : 0)];      // q 0, q 1, dO 0, dO 1, v
     __shared__ __attribute__((aligned(16))) float Ls[2][QT];
     __shared__ __attribute__((aligned(16))) float Ds[2][QT];
@@ -701,6 +704,7 @@ __global__ __launch_bounds__(64 * W, DT > 64 ? 2 : 3) void xattn_dkdv_kernel(Arg
     const uint32_t row_at = T::row_base(li, hh), tr_at = T::tr_base(lane);
     const int len = keys_of(a, b);
     const float c = a.scale * LOG2E;
+    const float lse_factor = BEGIN ? -1.0f / c : 1.0f;
     const float *lse = a.lse + (long)g * a.R, *dlt = a.delta + (long)g * a.R;
 
     const int n = (kbk * W + wave) * 32 + li, nc = n < a.Nk ? n : a.Nk - 1;
@@ -744,7 +748,7 @@ __global__ __launch_bounds__(64 * W, DT > 64 ? 2 : 3) void xattn_dkdv_kernel(Arg
         so.load(a.dout + ((long)b * a.Nq + tok0) * on + (long)hk * a.G * oh, bits);
         if (tid < 2 * QT) {
             const int r = r0 + tid % QT;
-            rl = r < a.R ? (tid < QT ? log2_of(lse[r]) : dlt[r]) : 0.0f;
+            rl = r < a.R ? (tid < QT ? log2_of(lse[r]) * lse_factor : BEGIN ? -dlt[r] : dlt[r]) : 0.0f;
         }
     };
     auto store = [&](int buf) {
@@ -769,25 +773,29 @@ __global__ __launch_bounds__(64 * W, DT > 64 ? 2 : 3) void xattn_dkdv_kernel(Arg
         for (int h = 0; h < QT / 32; ++h) {
             if (h && t * QT + 32 * h >= a.R) break;
             const uint32_t Qh = Qs + cur * BYTES + 32 * h * T::ROW, Oh = Qh + 2 * BYTES, Q = Qh + row_at, O = Oh + row_at, Vw = Vs + wave * 32 * T::ROW + row_at;
+            // register j <-> row (j & 3) + 8 (j >> 2) + 4 hh of the tile; rows behind the last have q = dO = 0 and lse = delta = 0: P is 1 there, dS 0
             f32x16 s, p;
 #pragma unroll
-            for (int j = 0; j < 16; ++j) { s[j] = 0.0f; p[j] = 0.0f; }
+            for (int q = 0; q < 4; ++q) {
+                const f32x4 l4 = *reinterpret_cast<const f32x4 *>(&Ls[cur][32 * h + 8 * q + 4 * hh]);
+                const f32x4 d4 = *reinterpret_cast<const f32x4 *>(&Ds[cur][32 * h + 8 * q + 4 * hh]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) { s[4 * q + j] = BEGIN ? l4[j] : 0.0f; p[4 * q + j] = BEGIN ? d4[j] : 0.0f; }
+            }
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
                 s = XA_MFMA(lds_16(Q ^ 32 * k), kf[k], s);
                 p = XA_MFMA(lds_16(O ^ 32 * k), V_IN_LDS ? lds_16(Vw ^ 32 * k) : vf[k], p);
             }
-            // register j <-> row (j & 3) + 8 (j >> 2) + 4 hh of the tile; rows behind the last have q = dO = 0 and lse = delta = 0: P is 1 there, dS 0
             float e[16], d[16];
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                const float4 l4 = *reinterpret_cast<const float4 *>(&Ls[cur][32 * h + 8 * q + 4 * hh]);
-                const float4 d4 = *reinterpret_cast<const float4 *>(&Ds[cur][32 * h + 8 * q + 4 * hh]);
-                const float lv[4] = {l4.x, l4.y, l4.z, l4.w}, dl[4] = {d4.x, d4.y, d4.z, d4.w};
+                const f32x4 l4 = *reinterpret_cast<const f32x4 *>(&Ls[cur][32 * h + 8 * q + 4 * hh]);
+                const f32x4 d4 = *reinterpret_cast<const f32x4 *>(&Ds[cur][32 * h + 8 * q + 4 * hh]);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    e[4 * q + j] = __builtin_amdgcn_exp2f(fmaf(s[4 * q + j], c, -lv[j]));
-                    d[4 * q + j] = e[4 * q + j] * (p[4 * q + j] - dl[j]);
+                    e[4 * q + j] = __builtin_amdgcn_exp2f(BEGIN ? s[4 * q + j] * c : fmaf(s[4 * q + j], c, -l4[j]));
+                    d[4 * q + j] = e[4 * q + j] * (BEGIN ? p[4 * q + j] : p[4 * q + j] - d4[j]);
                 }
             }
             const uint32_t ot = Oh + tr_at, qt = Qh + tr_at;
