@@ -4,10 +4,12 @@
 // gradient: dw[v] = scale * sum of g[n] over the tokens n with idx[n] = v — no floating-point atomics: the tokens are sorted by row (stable: ascending n
 // inside a row) and every row of dw is one fp32 chain, written once (rows without a token with zeros: no clearing pass).
 //
-// The sort is two launches, not a radix sort's pass per digit: (1) `embed_bin_kernel` — every block sorts its slice of the tokens by the row's high
-// bits (the bucket: 256 or up to 1024 buckets of 2^shift rows) in LDS and writes the slice's sorted list and its bucket starts; (2) `embed_sort_kernel` —
-// one block per bucket gathers its pieces of every slice's list (they follow each other in token order) and places them by the row's low bits.  The
-// position of a bucket in the sorted whole needs no scan over buckets: it is the sum of the slices' starts of that bucket.
+// The sort is two launches, not a radix sort's pass per digit: (1) `embed_bin_kernel` — every block sorts a slice of 2048 tokens by row in LDS and writes the
+// sorted list and where each bucket (256 or up to 1024 buckets of 2^shift rows) begins in it; (2) `embed_sort_kernel` — one block per bucket gathers its pieces of
+// every slice's list (they follow each other in token order).  The position of a bucket in the sorted whole needs no scan over buckets: it is the sum of the slices'
+// starts of that bucket.  A slice is sorted by row whole, and not by bucket alone, for 4 us more of the first launch (11 us instead of 7): it leaves the second
+// one no ranking, so that a bucket with a frequent row (14000 of 100000 tokens) takes it 22 us instead of 40, a table read at one row only 104 instead of 250 (100000
+// tokens), and 6 to 7 as before where no row is frequent.
 // The sums are two more: (3) `embed_sum_kernel` — rows of up to `chunk` tokens whole, and of the longer ones (a frequent word, a padding id) the pieces
 // that lie in each `chunk` of sorted positions, so that one row's tokens are read by many blocks; (4) `embed_long_kernel` adds a long row's pieces in order.
 #include "xq_common.hpp"
@@ -19,8 +21,6 @@
 namespace {
 
 constexpr int TILE = 2048;                               // tokens that a block of the first launch ranks at once
-constexpr int BIN_THREADS = 512;
-constexpr int MAX_BUCKETS = 1024;                        // of 1024 rows at most: rows <= 2^20
 
 // ---- forward ------------------------------------------------------------------------------------------------------------------------------
 
@@ -106,19 +106,17 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t *count, int n, uint32_t 
     return total;
 }
 
-// A stable counting sort of one tile by a whole block.  Every wave holds `rounds` x 64 items that follow each other in token order, round r's digit in
-// digit[r] (NONE: no item); seen[wave][digit] counts what a wave has met (no two waves share a counter, and the additions of one wave are in order).
+// A stable counting sort of one tile by a whole block.  Every wave holds ROUNDS x 64 items that follow each other in token order, round r's digit in
+// digit[r] (NONE: no item); at[digit] counts what the wave has met (no two waves share a counter, and the additions of one wave are in order).
 constexpr uint32_t NONE = 0xffffffffu;
 
-template <int ROUNDS, int DIGITS>
-__device__ __forceinline__ void tile_ranks(const uint32_t (&digit)[ROUNDS], int rounds, int bits, int digits, uint32_t (*seen)[DIGITS], uint32_t (&rank)[ROUNDS]) {
+template <int ROUNDS>
+__device__ __forceinline__ void tile_ranks(const uint32_t (&digit)[ROUNDS], int bits, int digits, uint32_t *at, uint32_t (&rank)[ROUNDS]) {
     const int lane = threadIdx.x & 63;
-    uint32_t *at = seen[threadIdx.x >> 6];
     for (int i = lane; i < digits; i += 64) at[i] = 0;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
     for (int r = 0; r < ROUNDS; ++r) {
-        if (r >= rounds) break;
         const bool live = digit[r] != NONE;
         const uint64_t same = same_digit(digit[r], bits, live);
         const uint32_t before = (uint32_t)__popcll(same & ((1ull << lane) - 1));
@@ -160,151 +158,183 @@ __device__ __forceinline__ void tile_places(uint32_t *seen, int pitch, int digit
     __syncthreads();
 }
 
-// slices of `tiles` tiles; list (row low bits, token) in bucket order, starts[slice][bucket] relative to the slice, buckets + 1 entries
-template <typename TI>
+// A slice is one tile.  Its tokens are sorted by row in LDS — by the row's low bits, then, stable, by its bucket — and written with what the second launch needs to
+// place them without ranking them again: low bits | place in the slice's run of the row << 10 | last of the run << 21, token.  starts[slice][bucket], buckets + 1.
+template <typename TI, int BIN_THREADS>
 __global__ __launch_bounds__(BIN_THREADS) void embed_bin_kernel(const TI *__restrict__ idx, long N, long V, long skip, int shift, int buckets, int bits,
-                                                                int tiles, uint2 *__restrict__ list, uint32_t *__restrict__ starts) {
+                                                                int pitch, uint2 *__restrict__ list, uint32_t *__restrict__ starts) {
     constexpr int WAVES = BIN_THREADS / 64, ROUNDS = TILE / BIN_THREADS;
-    __shared__ uint32_t seen[WAVES][MAX_BUCKETS];
-    __shared__ uint32_t base[MAX_BUCKETS];
+    extern __shared__ uint32_t lds[];             // the waves' counters, and the block's: pitch each
+    uint32_t *seen = lds, *base = seen + WAVES * pitch;
     __shared__ uint32_t part[WAVES];
+    __shared__ uint32_t sorted[TILE + 1];         // row << 11 | token's place in the tile
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const long first = (long)blockIdx.x * tiles * TILE, end = min(N, first + (long)tiles * TILE);
-    uint32_t *st = starts + (long)blockIdx.x * (buckets + 1);
-    auto publish = [&] {
-        const uint32_t total = block_scan<BIN_THREADS>(base, buckets, part);
-        for (int i = tid; i < buckets; i += BIN_THREADS) st[i] = base[i];
-        if (tid == 0) st[buckets] = total;
-    };
-    if (tiles > 1) {            // the slice's counts first; a slice of one tile has them from its ranks
-        for (int i = tid; i < buckets; i += BIN_THREADS) base[i] = 0;
-        __syncthreads();
-        for (long n0 = first + wave * 64; n0 < end; n0 += BIN_THREADS) {
-            long v = -1;
-            if (n0 + lane < end) v = (long)idx[n0 + lane];
-            const bool live = v >= 0 && v < V && v != skip;
-            const uint64_t same = same_digit((uint32_t)(v >> shift), bits, live);
-            if (live && (same & ((1ull << lane) - 1)) == 0) atomicAdd(&base[v >> shift], (uint32_t)__popcll(same));   // whole numbers: any order
-        }
-        __syncthreads();
-        publish();
-        __syncthreads();
-    }
-    for (long t0 = first; t0 < end; t0 += TILE) {
-        uint32_t digit[ROUNDS], low[ROUNDS], rank[ROUNDS];
-        const long n0 = t0 + wave * (64 * ROUNDS) + lane;
+    const long first = (long)blockIdx.x * TILE;
+    const uint32_t at0 = wave * (64 * ROUNDS) + lane;        // this thread's places: at0 + 64 r
+    uint32_t x[ROUNDS], digit[ROUNDS], rank[ROUNDS], total = 0;
 #pragma unroll
-        for (int r = 0; r < ROUNDS; ++r) {
-            const long n = n0 + r * 64;
-            long v = -1;
-            if (n < end) v = (long)idx[n];
-            const bool live = v >= 0 && v < V && v != skip;
-            digit[r] = live ? (uint32_t)(v >> shift) : NONE;
-            low[r] = (uint32_t)v & ((1u << shift) - 1);
+    for (int r = 0; r < ROUNDS; ++r) {
+        const long n = first + at0 + 64 * r;
+        long v = -1;
+        if (n < N) v = (long)idx[n];
+        x[r] = v >= 0 && v < V && v != skip ? (uint32_t)v << 11 | (at0 + 64 * r) : NONE;
+    }
+    auto pass = [&](int digits, int nbits, bool publish) {
+        tile_ranks<ROUNDS>(digit, nbits, digits, seen + wave * pitch, rank);
+        tile_counts<WAVES>(seen, pitch, digits, base);
+        total = block_scan<BIN_THREADS>(base, digits, part);
+        if (publish) {
+            uint32_t *st = starts + (long)blockIdx.x * (buckets + 1);
+            for (int i = tid; i < digits; i += BIN_THREADS) st[i] = base[i];
+            if (tid == 0) st[buckets] = total;
         }
-        tile_ranks<ROUNDS, MAX_BUCKETS>(digit, ROUNDS, bits, buckets, seen, rank);
-        if (tiles == 1) {
-            tile_counts<WAVES>(seen[0], MAX_BUCKETS, buckets, base);
-            publish();
-        }
-        tile_places<WAVES>(seen[0], MAX_BUCKETS, buckets, base);
+        tile_places<WAVES>(seen, pitch, digits, base);
 #pragma unroll
         for (int r = 0; r < ROUNDS; ++r)
-            if (digit[r] != NONE) list[first + seen[wave][digit[r]] + rank[r]] = make_uint2(low[r], (uint32_t)(n0 + r * 64));
+            if (digit[r] != NONE) sorted[seen[wave * pitch + digit[r]] + rank[r]] = x[r];
         __syncthreads();
+    };
+    if (shift > 0) {
+#pragma unroll
+        for (int r = 0; r < ROUNDS; ++r) digit[r] = x[r] == NONE ? NONE : x[r] >> 11 & ((1u << shift) - 1);
+        pass(1 << shift, shift, false);
+#pragma unroll
+        for (int r = 0; r < ROUNDS; ++r) x[r] = at0 + 64 * r < total ? sorted[at0 + 64 * r] : NONE;
+    }
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) digit[r] = x[r] == NONE ? NONE : x[r] >> (11 + shift);
+    pass(buckets, bits, true);
+    // where the run of the same row begins: the first place not below row << 11
+    uint32_t lo[ROUNDS], key[ROUNDS];
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+        x[r] = at0 + 64 * r < total ? sorted[at0 + 64 * r] : NONE;
+        key[r] = x[r] & ~2047u;
+        lo[r] = 0;
+    }
+    for (int h = TILE / 2; h > 0; h >>= 1) {
+#pragma unroll
+        for (int r = 0; r < ROUNDS; ++r)
+            if (lo[r] + h <= total && sorted[lo[r] + h - 1] < key[r]) lo[r] += h;
+    }
+#pragma unroll
+    for (int r = 0; r < ROUNDS; ++r) {
+        const uint32_t at = at0 + 64 * r;
+        if (at >= total) continue;
+        const bool last = at + 1 == total || (sorted[at + 1] & ~2047u) != key[r];
+        const uint32_t low = x[r] >> 11 & ((1u << shift) - 1);
+        list[first + at] = make_uint2(low | (at - lo[r]) << 10 | (last ? 1u << 21 : 0u), (uint32_t)first + (x[r] & 2047u));
     }
 }
 
-// One block per bucket: row starts of the bucket's rows, its tokens in row order, and the rows of every chunk's first and last position.  Every wave
-// counts the rows of its own eighth of the bucket, then places it: nothing but two meetings of the block between them, so that a bucket that one frequent
-// row fills (14000 of 100000 tokens) costs 40 us (in tiles that the whole block ranked: 100); 7 us where no row is frequent.
+// One block per bucket: row starts of the bucket's rows, its tokens in row order, and the rows of every chunk's first and last position.  Every wave takes its
+// share of the slices, 64 at a time (their pieces end to end, 64 tokens a round, U rounds' loads abreast): it counts its rows from the runs' last tokens; then, the waves' counts
+// known, a token's position is its row's next one plus its place in the run.  Slices that meet in one round take turns, so that a row's runs stay in order.
 template <int SORT_THREADS>
 __global__ __launch_bounds__(SORT_THREADS) void embed_sort_kernel(const uint2 *__restrict__ list, const uint32_t *__restrict__ starts, long V, int shift,
-                                                                  int buckets, int slices, int half, long slice_tokens, uint32_t *__restrict__ row_start,
+                                                                  int buckets, int slices, uint32_t *__restrict__ row_start,
                                                                   uint32_t *__restrict__ order, int chunk_bits, uint32_t *__restrict__ edge) {
     constexpr int WAVES = SORT_THREADS / 64, U = 4;
     extern __shared__ uint32_t lds[];
-    uint32_t *piece = lds, *from = lds + slices;          // where a slice's piece begins in the bucket, and in the slice's list
-    uint32_t *seen = from + slices, *base = seen + (WAVES << shift);
     __shared__ uint32_t part[WAVES];
     __shared__ uint32_t ahead[WAVES];
+    __shared__ uint32_t pieces[WAVES][64], froms[WAVES][64];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, bucket = blockIdx.x;
     const int rows = 1 << shift;
-    uint32_t *at = seen + (wave << shift);
-    uint32_t mine = 0;
-    for (int s = tid; s < slices; s += SORT_THREADS) {
-        const uint32_t *st = starts + (long)s * (buckets + 1) + bucket;
-        const uint32_t b = st[0];
-        mine += b;
-        from[s] = b;
-        piece[s] = st[1] - b;
-    }
+    uint32_t *seen = lds, *base = seen + (WAVES << shift), *at = seen + (wave << shift);
+    uint32_t *piece = pieces[wave], *from = froms[wave];          // a wave's own: where a slice's piece begins in the 64 slices' tokens, and in the slice's list
+    const int s0 = (int)((long)slices * wave / WAVES), s1 = (int)((long)slices * (wave + 1) / WAVES);
     for (int i = lane; i < rows; i += 64) at[i] = 0;
+    // the pieces of slices s .. s + 63 (below s1) -> their tokens' number; `mine`: this lane's slice's tokens ahead of the bucket
+    auto take = [&](int s, uint32_t &mine) {
+        uint32_t b = 0, n = 0;
+        if (s + lane < s1) {
+            const uint32_t *st = starts + (long)(s + lane) * (buckets + 1) + bucket;
+            b = st[0];
+            n = st[1] - b;
+        }
+        mine = b;
+        uint32_t incl = n;
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) mine += __shfl_xor(mine, o);
-    if (lane == 0) ahead[wave] = mine;
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t up = __shfl_up(incl, o);
+            if (lane >= o) incl += up;
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        piece[lane] = incl - n;
+        from[lane] = b;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        return (uint32_t)__shfl(incl, 63);
+    };
+    // the tokens at places i + 64 r (+ lane) of those pieces, and the slice (0 .. 63) of each; NONE behind the end
+    auto items = [&](int s, uint32_t i, uint32_t total, uint2 (&it)[U], int (&lo)[U]) {
+#pragma unroll
+        for (int r = 0; r < U; ++r) lo[r] = 0;
+#pragma unroll
+        for (int h = 32; h > 0; h >>= 1) {
+#pragma unroll
+            for (int r = 0; r < U; ++r)
+                if (piece[lo[r] + h] <= i + 64 * r + lane) lo[r] += h;          // (lo + h <= 63; the last slice that begins not behind the place: the one that holds it)
+        }
+#pragma unroll
+        for (int r = 0; r < U; ++r) {
+            const uint32_t p = i + 64 * r + lane;
+            it[r] = make_uint2(NONE, 0u);
+            if (p < total) it[r] = list[(long)(s + lo[r]) * TILE + from[lo[r]] + (p - piece[lo[r]])];
+        }
+    };
+    uint32_t tokens = 0, before = 0;
+    uint2 it[U];
+    int lo[U];
+    for (int s = s0; s < s1; s += 64) {
+        uint32_t mine;
+        const uint32_t total = take(s, mine);
+        before += mine;
+        tokens += total;
+        for (uint32_t i = 0; i < total; i += 64 * U) {
+            items(s, i, total, it, lo);
+#pragma unroll
+            for (int r = 0; r < U; ++r)
+                if (it[r].x != NONE && it[r].x >> 21) atomicAdd(&at[it[r].x & 1023u], (it[r].x >> 10 & 2047u) + 1);      // a run's tokens (whole numbers: any order)
+        }
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) before += __shfl_xor(before, o);
+    if (lane == 0) ahead[wave] = before;
     __syncthreads();
-    const uint32_t total = block_scan<SORT_THREADS>(piece, slices, part);
+    tile_counts<WAVES>(seen, rows, rows, base);
+    const uint32_t total_rows = block_scan<SORT_THREADS>(base, rows, part);
     uint32_t start = 0;
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) start += ahead[w];
-    // the items at positions i0 + 64 r of the bucket below `end`: the slice whose piece holds each, by halving, all of them abreast (one after another they
-    // would be six to nine dependent reads each)
-    auto items = [&](uint32_t i0, uint32_t end, uint2 (&it)[U]) {
-        int lo[U];
-#pragma unroll
-        for (int r = 0; r < U; ++r) lo[r] = 0;
-        for (int h = half; h > 0; h >>= 1) {
-#pragma unroll
-            for (int r = 0; r < U; ++r) {
-                const int m = lo[r] + h;
-                if (m < slices && piece[m] <= i0 + 64 * r) lo[r] = m;
-            }
-        }
-#pragma unroll
-        for (int r = 0; r < U; ++r) {
-            it[r] = make_uint2(NONE, 0u);
-            const uint32_t i = i0 + 64 * r;
-            if (i < end) it[r] = list[(long)lo[r] * slice_tokens + from[lo[r]] + (i - piece[lo[r]])];
-        }
-    };
-    const uint32_t per = (total + SORT_THREADS - 1) / SORT_THREADS * 64, first = wave * per, end = min(total, first + per);
-    uint2 it[U];
-    for (uint32_t i = first; i < end; i += 64 * U) {
-        items(i + lane, end, it);
-#pragma unroll
-        for (int r = 0; r < U; ++r) {
-            if (i + 64 * r >= end) break;
-            const uint64_t same = same_digit(it[r].x, shift, it[r].x != NONE);
-            if (it[r].x != NONE && (same >> lane) == 1ull) atomicAdd(&at[it[r].x], (uint32_t)__popcll(same));      // (one lane: nothing waits for it)
-        }
-    }
-    __syncthreads();
-    tile_counts<WAVES>(seen, rows, rows, base);
-    block_scan<SORT_THREADS>(base, rows, part);
     const long v0 = (long)bucket << shift;
     for (int i = tid; i < rows; i += SORT_THREADS)
         if (v0 + i < V) row_start[v0 + i] = start + base[i];
-    if (bucket == buckets - 1 && tid == 0) row_start[V] = start + total;
+    if (bucket == buckets - 1 && tid == 0) row_start[V] = start + total_rows;
     tile_places<WAVES>(seen, rows, rows, base);
-    for (uint32_t i = first; i < end; i += 64 * U) {
-        if (end - first > 64 * U) items(i + lane, end, it);       // up to U rounds are still here
+    const bool here = s1 - s0 <= 64 && tokens <= 64 * U;          // all of the wave's tokens are in registers
+    for (int s = s0; s < s1; s += 64) {
+        uint32_t mine, total = tokens;
+        if (!here) total = take(s, mine);
+        for (uint32_t i = 0; i < total; i += 64 * U) {
+            if (!here) items(s, i, total, it, lo);
 #pragma unroll
-        for (int r = 0; r < U; ++r) {
-            if (i + 64 * r >= end) break;
-            const uint32_t digit = it[r].x;
-            const bool live = digit != NONE;
-            const uint64_t same = same_digit(digit, shift, live);
-            uint32_t met = 0;
-            if (live) met = at[digit];
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            if (live && (same >> lane) == 1ull) at[digit] = met + (uint32_t)__popcll(same);
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            if (live) {
-                const uint32_t pos = start + met + (uint32_t)__popcll(same & ((1ull << lane) - 1)), in = pos & ((1u << chunk_bits) - 1);
-                order[pos] = it[r].y;
-                if (in == 0) edge[2 * (pos >> chunk_bits)] = (uint32_t)v0 + digit;
-                if (in == (1u << chunk_bits) - 1) edge[2 * (pos >> chunk_bits) + 1] = (uint32_t)v0 + digit;
+            for (int r = 0; r < U; ++r) {
+                const uint64_t live = __ballot(it[r].x != NONE);
+                if (!live) break;
+                const uint32_t low = it[r].x & 1023u, place = it[r].x >> 10 & 2047u;
+                const int s_first = __builtin_amdgcn_readlane(lo[r], 0), s_last = __builtin_amdgcn_readlane(lo[r], 63 - __builtin_clzll(live));
+                for (int turn = s_first; turn <= s_last; ++turn) {
+                    if (it[r].x == NONE || lo[r] != turn) continue;
+                    const uint32_t next = at[low];
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");           // every token of the run has read before its last one moves the row on
+                    if (it[r].x >> 21) at[low] = next + place + 1;
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                    const uint32_t pos = start + next + place, in = pos & ((1u << chunk_bits) - 1);
+                    order[pos] = it[r].y;
+                    if (in == 0) edge[2 * (pos >> chunk_bits)] = (uint32_t)v0 + low;
+                    if (in == (1u << chunk_bits) - 1) edge[2 * (pos >> chunk_bits) + 1] = (uint32_t)v0 + low;
+                }
             }
         }
     }
@@ -456,7 +486,7 @@ int log2_up(long x) { int b = 0; while ((1L << b) < x) ++b; return b; }
 int pow2_lanes(int D, int vec) { int l = 1; while (l < 256 && l * vec < D) l <<= 1; return l; }
 
 struct Plan {
-    int shift, buckets, bucket_bits, tiles, slices;
+    int shift, buckets, bucket_bits, slices;
     int chunk_bits;
     long chunks;
     size_t o_list, o_starts, o_rows, o_order, o_edge, o_part, bytes;
@@ -470,9 +500,7 @@ Plan make_plan(long N, long V, int D) {
     p.shift = bits <= 8 ? 0 : bits <= 17 ? bits - 8 : bits - 10;
     p.buckets = (int)((V + (1L << p.shift) - 1) >> p.shift);
     p.bucket_bits = log2_up(p.buckets);
-    const long tiles = (N + TILE - 1) / TILE;
-    p.tiles = (int)((tiles + 511) / 512);
-    p.slices = (int)((tiles + p.tiles - 1) / p.tiles);
+    p.slices = (int)((N + TILE - 1) / TILE);
     // 64 tokens: eight trips to memory for a row or a piece of one, and one fp32 row of partial sums written for 64 read
     p.chunk_bits = std::max(6, log2_up((N + 4095) / 4096));
     p.chunks = (N + (1L << p.chunk_bits) - 1) >> p.chunk_bits;
@@ -594,16 +622,17 @@ extern "C" int xq_embedding_backward(const void *idx, int idx_i64, const void *g
     uint32_t *starts = (uint32_t *)(ws + p.o_starts), *rows = (uint32_t *)(ws + p.o_rows), *order = (uint32_t *)(ws + p.o_order),
              *edge = (uint32_t *)(ws + p.o_edge);
     float *part = (float *)(ws + p.o_part);
-    if (idx_i64)
-        hipLaunchKernelGGL((embed_bin_kernel<int64_t>), dim3(p.slices), dim3(BIN_THREADS), 0, s, (const int64_t *)idx, (long)N, (long)V, (long)skip, p.shift,
-                           p.buckets, p.bucket_bits, p.tiles, list, starts);
-    else
-        hipLaunchKernelGGL((embed_bin_kernel<int32_t>), dim3(p.slices), dim3(BIN_THREADS), 0, s, (const int32_t *)idx, (long)N, (long)V, (long)skip, p.shift,
-                           p.buckets, p.bucket_bits, p.tiles, list, starts);
-#define XQ_SORT(THREADS)                                                                                                                       \
-    hipLaunchKernelGGL((embed_sort_kernel<THREADS>), dim3(p.buckets), dim3(THREADS), (size_t)p.slices * 8 + ((THREADS / 64 + 1) << p.shift) * 4, s, list, \
-                       starts, (long)V, p.shift, p.buckets, p.slices, p.slices > 1 ? 1 << (log2_up(p.slices) - 1) : 0, (long)p.tiles * TILE, rows, order, \
-                       p.chunk_bits, edge)
+    // sixteen waves a block where their counters fit the 64 KB of a launch (up to 512 buckets and rows a bucket), eight otherwise
+    const int pitch = std::max(p.buckets, 1 << p.shift);
+#define XQ_BIN(TI, THREADS)                                                                                                                        \
+    hipLaunchKernelGGL((embed_bin_kernel<TI, THREADS>), dim3(p.slices), dim3(THREADS), (size_t)(THREADS / 64 + 1) * pitch * 4, s, (const TI *)idx, (long)N, (long)V, \
+                       (long)skip, p.shift, p.buckets, p.bucket_bits, pitch, list, starts)
+    if (pitch <= 512) { if (idx_i64) XQ_BIN(int64_t, 1024); else XQ_BIN(int32_t, 1024); }
+    else { if (idx_i64) XQ_BIN(int64_t, 512); else XQ_BIN(int32_t, 512); }
+#undef XQ_BIN
+#define XQ_SORT(THREADS)                                                                                                                              \
+    hipLaunchKernelGGL((embed_sort_kernel<THREADS>), dim3(p.buckets), dim3(THREADS), (size_t)((THREADS / 64 + 1) << p.shift) * 4, s, list, starts, (long)V, \
+                       p.shift, p.buckets, p.slices, rows, order, p.chunk_bits, edge)
     if (p.shift <= 9) XQ_SORT(1024);
     else XQ_SORT(512);           // 1024 rows a bucket: sixteen waves' counters would not fit the 64 KB of a launch
 #undef XQ_SORT
