@@ -69,7 +69,7 @@ __device__ __forceinline__ bf16x4 lds_tr(uint32_t at) { return __builtin_amdgcn_
 
 // A row-major bf16 tile in LDS, rows of 64, 128 or 256 bytes (96 columns lie in 256).  Chunk c (16 bytes) of row R is kept at chunk c ^ twist(R), so that both
 // ways of reading meet all 64 banks: 16 rows at one chunk (the operands over the head dimension) and 4 rows x 4 chunks (the transpose reads).  A pitch of
-// DT + 8 instead serves the first way only: half of the LDS cycles were conflicts (forward at 128 columns 536 us, now 483).
+// DT + 8 instead serves the first way only: half of the LDS cycles were conflicts (dk / dv at 128 columns 1140 us, then 1108).
 template <int DT>
 struct Tile {
     static constexpr int PITCH = DT > 64 ? 128 : DT, ROW = 2 * PITCH;
@@ -91,6 +91,14 @@ struct Tile {
         const bf16x4 lo = lds_tr((base ^ 64 * q) + row0 * ROW), hi = lds_tr((base ^ 64 * q ^ 32) + (row0 + 8) * ROW);      // twist(R + 8) = twist(R) ^ 2
         return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     }
+    // the same for 16x16x32: 32 contraction rows from row0 (a multiple of 32; in an order of their own, the same for both operands), columns 16 q + (lane & 15)
+    static __device__ __forceinline__ uint32_t tr16_base(int lane) {
+        return place(8 * (lane >> 4 & 1) + 4 * (lane >> 5) + ((lane & 15) >> 2), (lane & 3) >> 1) + 8 * (lane & 1);
+    }
+    static __device__ __forceinline__ bf16x8 tr16_frag(uint32_t base, int row0, int q) {
+        const bf16x4 lo = lds_tr((base ^ 32 * q) + row0 * ROW), hi = lds_tr((base ^ 32 * q) + (row0 + 16) * ROW);
+        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
 };
 
 // v_max3_f32 without the operand canonicalisation that fmaxf() carries under IEEE mode
@@ -101,6 +109,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 
 #define XA_MFMA(A, B, C) __builtin_amdgcn_mfma_f32_32x32x16_bf16((A), (B), (C), 0, 0, 0)
+#define XA_MFMA16(A, B, C) __builtin_amdgcn_mfma_f32_16x16x32_bf16((A), (B), (C), 0, 0, 0)
 
 __device__ __forceinline__ uint32_t quotient(uint32_t a, uint64_t reciprocal) { return reciprocal ? (uint32_t)__umul64hi((uint64_t)a, reciprocal) : a; }
 
@@ -150,6 +159,7 @@ __device__ __forceinline__ uint4 zero_unless(uint4 v, bool ok) {
 // 16 bytes at a byte offset of up to 2^31 behind a wave-uniform base; FAR reads zeros (a buffer's bounds check), so that what is masked or behind the head
 // dimension costs an offset and no select on the data, and is never touched
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 constexpr uint32_t FAR = 0x80000000u;
 __device__ __forceinline__ uint4 load16(const short *base, uint32_t off) {
     const auto rs = __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, 0x7fffffff, 0x00020000);
@@ -679,7 +689,7 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(Args a) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------------------------
-// dk, dv: one key per lane, 128 keys of one (sample, kv head) a block; tiles of QT rows of q and dO (and lse, delta) in two LDS buffers
+// dk, dv: one key per lane, 32 W keys of one (sample, kv head) a block; tiles of QT rows of q and dO (and lse, delta) in two LDS buffers
 // ---------------------------------------------------------------------------------------------------------------------------------------------
 template <int DT, int W, bool SPLIT>
 __global__ __launch_bounds__(64 * W, DT > 64 ? 2 : 3) void xattn_dkdv_kernel(Args a) {
@@ -689,7 +699,7 @@ __global__ __launch_bounds__(64 * W, DT > 64 ? 2 : 3) void xattn_dkdv_kernel(Arg
     // a wave's own 32 rows of V: only at 96 columns do its fragments stay in registers beside the accumulators (elsewhere that would cost a wave a SIMD)
     constexpr bool V_IN_LDS = DT != 96;
     // at 128 columns the products begin at -lse / scale and -delta instead of zero (two operations a score less: 1135 -> 1082 us at 4 x 4096 x 4352 x 16); at 64 the
-    // wait for the two before the first product costs more than that (121 -> 140 us at 128 x 256 x 257 x 12)
+    // wait for the two before the first product costs more than that (121 -> 140 us at 128 x 256 x 257 x 12 heads)
     constexpr bool BEGIN = DT > 96;
     __shared__ __attribute__((aligned(256))) char tiles[4 * BYTES + (V_IN_LDS ? 32 * W * T::ROW : 0)];      // q 0, q 1, dO 0, dO 1, v
     __shared__ __attribute__((aligned(16))) float Ls[2][QT];
@@ -831,6 +841,254 @@ __global__ __launch_bounds__(64 * W, DT > 64 ? 2 : 3) void xattn_dkdv_kernel(Arg
     }
 }
 
+// ---------------------------------------------------------------------------------------------------------------------------------------------
+// the whole backward of a (sample, kv head) whose keys fit one block (up to 32 W of them): one key per lane as in the dk / dv kernel; dS also goes to LDS
+// (key-major), and the waves share out dq = dS k of the tile before.  q, dO and out are read once, P and dP computed once: five products instead of seven.
+// 128 x 256 rows x 257 keys x 12 heads of 64 (nine waves): 165 us, 2.4 TB/s of its 400 MB and 350 TFLOP/s.  Bound by what no single unit is: LDS reads take about
+// half of the time, the scores' arithmetic 40 %, the matrix pipe a quarter, and one block a CU leaves nothing beside its first loads and last stores.
+// ---------------------------------------------------------------------------------------------------------------------------------------------
+template <int DT, int W, bool SPLIT>
+__global__ __launch_bounds__(64 * W, DT > 64 ? 2 : 3) void xattn_bwd_kernel(Args a) {
+    typedef Tile<DT> T;
+    typedef Tile<32> TS;
+    constexpr int QT = 32, KS = DT / 16, OT = DT / 32, BYTES = QT * T::ROW, SBYTES = 32 * W * TS::ROW;
+    constexpr int SB = DT > 64 ? 1 : 2;                     // buffers of dS: with one, a second meeting a tile, but two blocks a CU
+    constexpr bool V_IN_LDS = W == 9;                       // (with four waves a block fewer blocks would fit a CU)
+    // dq: NA x NB tiles of 16 columns x 16 rows a wave
+    constexpr int NA = W == 4 ? (DT == 96 ? 3 : DT == 128 ? 2 : 1) : 1, NB = W == 4 && (DT == 64 || DT == 128) ? 2 : 1, FIRST = W == 4 ? 0 : 1;
+    // staging: 16 bytes of dO and out, and of q, a thread; where there are threads enough, other threads take q
+    constexpr int PR = DT > 64 ? 16 : DT / 8, CHUNKS = QT * PR;
+    constexpr bool ROLES = 64 * W >= 2 * CHUNKS;
+    constexpr int CH = ROLES ? 1 : CHUNKS / (64 * W);
+    static_assert(ROLES || CHUNKS % (64 * W) == 0, "whole rounds");
+    __shared__ __attribute__((aligned(256))) char tiles[4 * BYTES + (V_IN_LDS ? 2 : 1) * 32 * W * T::ROW + SB * SBYTES];      // q 0, q 1, dO 0, dO 1, k, dS, v
+    __shared__ __attribute__((aligned(16))) float Ls[2][QT];
+    __shared__ __attribute__((aligned(16))) float Ds[2][QT];
+    const uint32_t Qs = lds_address(tiles), Os = Qs + 2 * BYTES, Kb = Qs + 4 * BYTES, Sb = Kb + 32 * W * T::ROW, Vb = Sb + SB * SBYTES;
+    int g, split;
+    if (!map_block(a, g, split)) return;
+    const int b = g / a.Hk, hk = g - b * a.Hk;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 31, hh = lane >> 5;
+    const uint32_t row_at = T::row_base(li, hh), tr_at = T::tr_base(lane);
+    const int len = keys_of(a, b);
+    const float c = a.scale * LOG2E;
+    const float lse_factor = -1.0f / c;
+    const float *lse = a.lse + (long)g * a.R;
+    const unsigned char *mask = a.mask ? a.mask + (long)b * a.Nk : nullptr;
+    const short *kb = a.k.p + b * a.k.sb + hk * a.k.sh;
+
+    const int n = wave * 32 + li, nc = n < a.Nk ? n : a.Nk - 1;
+    bool valid = n < len;
+    if (mask && valid) valid = mask[n] != 0;
+    const bool wave_live = __any(valid), all_valid = __all(valid);
+    // (the prologue's loads are all in flight before the first is waited for)
+    bf16x8 vf[KS];
+    load_row<DT>(a.v.p + b * a.v.sb + hk * a.v.sh + (long)nc * a.v.sn, a.D, hh, vf);
+    uint4 kr[DT / 16];
+#pragma unroll
+    for (int j = 0; j < DT / 16; ++j) {
+        const int id = tid + 64 * W * j, row = id / (DT / 8), chunk = id % (DT / 8);
+        bool there = row < len && 8 * chunk < a.D;
+        if (mask && there) there = mask[row] != 0;
+        kr[j] = make_uint4(0u, 0u, 0u, 0u);
+        if (there) kr[j] = *reinterpret_cast<const uint4 *>(kb + (long)row * a.k.sn + 8 * chunk);
+    }
+    if (!wave_live) {
+        for (int j = 0; j < SB; ++j)
+            for (int i = lane; i < 32 * TS::ROW / 16; i += 64)
+                *(lds_ptr<u32x4>)(uintptr_t)(Sb + j * SBYTES + wave * 32 * TS::ROW + 16 * i) = __builtin_bit_cast(u32x4, make_uint4(0u, 0u, 0u, 0u));
+    }
+
+    f32x16 dk[OT], dv[OT];
+#pragma unroll
+    for (int t = 0; t < OT; ++t)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) { dk[t][j] = 0.0f; dv[t][j] = 0.0f; }
+
+    const long on = (long)a.H * a.D, oh = a.D;
+    const int role = ROLES ? wave / (CHUNKS / 64) : 0;
+    uint32_t off_q[CH], off_o[CH];
+    uint4 rq[CH], rd[CH], ro[CH];
+    float rl = 0.0f;
+    auto row_of = [&](int ch) { return (ROLES ? tid % CHUNKS : tid + 64 * W * ch) / PR; };
+    auto chunk_of = [&](int ch) { return (ROLES ? tid % CHUNKS : tid + 64 * W * ch) % PR; };
+    // row r0 + i of a tile: token (r0 + i) / G.  Where G divides QT its offset from the tile's first token is the same in every tile
+    auto places = [&](int g0) {
+#pragma unroll
+        for (int ch = 0; ch < CH; ++ch) {
+            const uint32_t rr = g0 + row_of(ch), tok = quotient(rr, a.g_reciprocal), gg = rr - tok * a.G;
+            const int col = 8 * chunk_of(ch);
+            off_q[ch] = col < a.D ? (tok * (uint32_t)a.q.sn + gg * (uint32_t)a.q.sh + col) * 2 : FAR;
+            off_o[ch] = col < a.D ? (tok * (uint32_t)on + gg * (uint32_t)oh + col) * 2 : FAR;
+        }
+    };
+    const bool same_places = QT % a.G == 0;
+    places(0);
+    auto load = [&](int r0) {
+        const int tok0 = (int)quotient((uint32_t)r0, a.g_reciprocal), left = a.R - r0;
+        if (!same_places) places(r0 - tok0 * a.G);
+        const long o = ((long)b * a.Nq + tok0) * on + (long)hk * a.G * oh;
+        if (role == 0) {
+#pragma unroll
+            for (int ch = 0; ch < CH; ++ch) {
+                const uint32_t at = row_of(ch) < left ? off_o[ch] : FAR;
+                rd[ch] = load16(a.dout + o, at);
+                ro[ch] = load16(a.out_in + o, at);
+            }
+        }
+        if (!ROLES || role == 1) {
+#pragma unroll
+            for (int ch = 0; ch < CH; ++ch)
+                rq[ch] = load16(a.q.p + b * a.q.sb + tok0 * a.q.sn + (long)hk * a.G * a.q.sh, row_of(ch) < left ? off_q[ch] : FAR);
+        }
+        if (tid < QT) rl = tid < left ? log2_of(lse[r0 + tid]) * lse_factor : 0.0f;
+    };
+    auto store = [&](int buf) {
+        if (role == 0) {
+#pragma unroll
+            for (int ch = 0; ch < CH; ++ch) {
+                const uint4 x = rd[ch], y = ro[ch];
+                float s = bf_lo(x.x) * bf_lo(y.x);
+                s = fmaf(bf_hi(x.x), bf_hi(y.x), s);
+                s = fmaf(bf_lo(x.y), bf_lo(y.y), s); s = fmaf(bf_hi(x.y), bf_hi(y.y), s);
+                s = fmaf(bf_lo(x.z), bf_lo(y.z), s); s = fmaf(bf_hi(x.z), bf_hi(y.z), s);
+                s = fmaf(bf_lo(x.w), bf_lo(y.w), s); s = fmaf(bf_hi(x.w), bf_hi(y.w), s);
+#pragma unroll
+                for (int o = 1; o < PR; o <<= 1) s += __shfl_xor(s, o);
+                if (chunk_of(ch) == 0) Ds[buf][row_of(ch)] = -s;
+                *(lds_ptr<u32x4>)(uintptr_t)(Os + buf * BYTES + T::place(row_of(ch), chunk_of(ch))) = __builtin_bit_cast(u32x4, x);
+            }
+        }
+        if (!ROLES || role == 1) {
+#pragma unroll
+            for (int ch = 0; ch < CH; ++ch)
+                *(lds_ptr<u32x4>)(uintptr_t)(Qs + buf * BYTES + T::place(row_of(ch), chunk_of(ch))) = __builtin_bit_cast(u32x4, rq[ch]);
+        }
+        if (tid < QT) Ls[buf][tid] = rl;
+    };
+
+    const int unit = wave - FIRST;
+    const int ct = NB == 2 ? NA * unit : NA * (unit >> 1), half = NB == 2 ? 0 : unit & 1;       // the wave's first columns and rows of dq
+    const uint32_t kt16 = Kb + T::tr16_base(lane), st16 = TS::tr16_base(lane);
+    auto dq_tile = [&](int t, uint32_t S) {
+        if (ct * 16 >= DT || unit < 0) return;
+        f32x4 acc[NA][NB];
+#pragma unroll
+        for (int i = 0; i < NA; ++i)
+#pragma unroll
+            for (int j = 0; j < NB; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < W; ++k) {
+            bf16x8 ka[NA], sb[NB];
+#pragma unroll
+            for (int i = 0; i < NA; ++i) ka[i] = T::tr16_frag(kt16, 32 * k, ct + i);
+#pragma unroll
+            for (int j = 0; j < NB; ++j) sb[j] = TS::tr16_frag(S + st16, 32 * k, half + j);
+#pragma unroll
+            for (int i = 0; i < NA; ++i)
+#pragma unroll
+                for (int j = 0; j < NB; ++j) acc[i][j] = XA_MFMA16(ka[i], sb[j], acc[i][j]);
+        }
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+            const int r = t * QT + 16 * (half + j) + (lane & 15);
+            if (r >= a.R) continue;
+            short *row = a.dq.p + row_offset(a, a.dq, b, hk, r);
+#pragma unroll
+            for (int i = 0; i < NA; ++i) {
+                const int col = 16 * (ct + i) + 4 * (lane >> 4);
+                const f32x4 x = acc[i][j];
+                if (col < a.D) *reinterpret_cast<uint2 *>(row + col) = make_uint2(pack_bf16(x[0] * a.scale, x[1] * a.scale), pack_bf16(x[2] * a.scale, x[3] * a.scale));
+            }
+        }
+    };
+
+    int t0, t1;
+    share((a.R + QT - 1) / QT, split, SPLIT ? a.splits : 1, t0, t1);
+    if (t0 < t1) load(t0 * QT);
+    const uint32_t Kw = Kb + wave * 32 * T::ROW + row_at, Vw = Vb + wave * 32 * T::ROW + row_at;
+    if (V_IN_LDS) {
+#pragma unroll
+        for (int k = 0; k < KS; ++k) *(lds_ptr<bf16x8>)(uintptr_t)(Vw ^ 32 * k) = vf[k];
+    }
+    // every key's row of k, zeros for one that is not valid: what dq adds of it is 0 x 0
+#pragma unroll
+    for (int j = 0; j < DT / 16; ++j) {
+        const int id = tid + 64 * W * j;
+        *(lds_ptr<u32x4>)(uintptr_t)(Kb + T::place(id / (DT / 8), id % (DT / 8))) = __builtin_bit_cast(u32x4, kr[j]);
+    }
+    if (t0 < t1) store(0);
+    __syncthreads();
+    for (int t = t0; t < t1; ++t) {
+        const int cur = (t - t0) & 1;
+        if (t + 1 < t1) load(t * QT + QT);
+        if (SB == 2 && t > t0) dq_tile(t - 1, Sb + (cur ^ 1) * SBYTES);
+        if (wave_live) {
+            const uint32_t Qh = Qs + cur * BYTES, Oh = Os + cur * BYTES, Q = Qh + row_at, O = Oh + row_at;
+            // the products begin at -lse / scale and -delta.  Register j <-> row (j & 3) + 8 (j >> 2) + 4 hh of the tile; rows behind the last have q = dO = 0 and lse = delta = 0: P is 1 there, dS 0
+            f32x16 s, p;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const f32x4 l4 = *reinterpret_cast<const f32x4 *>(&Ls[cur][8 * q + 4 * hh]);
+                const f32x4 d4 = *reinterpret_cast<const f32x4 *>(&Ds[cur][8 * q + 4 * hh]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) { s[4 * q + j] = l4[j]; p[4 * q + j] = d4[j]; }
+            }
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                s = XA_MFMA(lds_16(Q ^ 32 * k), lds_16(Kw ^ 32 * k), s);
+                p = XA_MFMA(lds_16(O ^ 32 * k), V_IN_LDS ? lds_16(Vw ^ 32 * k) : vf[k], p);
+            }
+            float e[16], d[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                e[j] = __builtin_amdgcn_exp2f(s[j] * c);
+                d[j] = e[j] * p[j];
+            }
+            const uint32_t ot = Oh + tr_at, qt = Qh + tr_at;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const bf16x8 pb = pack8(e + 8 * k);
+                uint4 db = __builtin_bit_cast(uint4, pack8(d + 8 * k));
+                if (!all_valid) db = zero_unless(db, valid);          // (P of a key that is not valid may be infinite)
+                // rows 16 k + 4 hh .. + 3 and 16 k + 8 + 4 hh .. + 3 of the lane's key
+                const uint32_t at = Sb + (SB == 2 ? cur : 0) * SBYTES + 8 * hh;
+                *(lds_ptr<u32x2>)(uintptr_t)(at + TS::place(n, 2 * k)) = u32x2{db.x, db.y};
+                *(lds_ptr<u32x2>)(uintptr_t)(at + TS::place(n, 2 * k + 1)) = u32x2{db.z, db.w};
+#pragma unroll
+                for (int q = 0; q < OT; ++q) {
+                    dv[q] = XA_MFMA(T::tr_frag(ot, 16 * k, q), pb, dv[q]);
+                    dk[q] = XA_MFMA(T::tr_frag(qt, 16 * k, q), __builtin_bit_cast(bf16x8, db), dk[q]);
+                }
+            }
+        }
+        if (SB == 1) {
+            __syncthreads();
+            dq_tile(t, Sb);
+        }
+        if (t + 1 < t1) store(cur ^ 1);
+        __syncthreads();
+    }
+    if (SB == 2 && t0 < t1) dq_tile(t1 - 1, Sb + ((t1 - 1 - t0) & 1) * SBYTES);
+    // a masked key's column holds what its bytes gave: zero goes out for it
+    if (!valid) {
+#pragma unroll
+        for (int t = 0; t < OT; ++t)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) { dk[t][j] = 0.0f; dv[t][j] = 0.0f; }
+    }
+    const bool ok = n < a.Nk;
+    if (SPLIT) {
+        const long slots = (long)a.groups * a.Nk, slot = (long)g * a.Nk + nc;
+        float *pk = a.part + (2 * split * slots + slot) * a.D, *pv = a.part + ((2 * split + 1) * slots + slot) * a.D;
+        store_part<DT>(pk, a.D, hh, dk, ok);
+        store_part<DT>(pv, a.D, hh, dv, ok);
+    } else {
+        store_row<DT>(a.dk.p + b * a.dk.sb + hk * a.dk.sh + (long)nc * a.dk.sn, a.D, hh, dk, a.scale, ok);
+        store_row<DT>(a.dv.p + b * a.dv.sb + hk * a.dv.sh + (long)nc * a.dv.sn, a.D, hh, dv, 1.0f, ok);
+    }
+}
+
 // slabs of a split gradient, added in order: KIND 0 dq rows (g R + r), 1 dk and dv keys (2 x (g Nk + n)); four columns a thread
 template <int KIND>
 __global__ __launch_bounds__(256) void xattn_sum_kernel(Args a, int per_row, unsigned long long row_reciprocal, long total) {
@@ -877,6 +1135,7 @@ int splits_for(long blocks, long steps, int least) {
 struct Sizes {
     long groups, R;
     int fwd_splits, dq_splits, kv_splits, kv_waves;
+    int one_waves;                 // waves of the one-block backward (0: the two kernels)
     bool few_rows;
     size_t fwd_part, fwd_bytes, delta_bytes, bwd_bytes;
 };
@@ -885,7 +1144,7 @@ Sizes sizes_of(int B, int Nq, int Nk, int H, int Hk, int D) {
     Sizes z;
     z.groups = (long)B * Hk;
     z.R = (long)Nq * (H / Hk);
-    z.kv_waves = D > 96 && Nk > 128 ? 8 : 4;
+    z.kv_waves = D > 96 ? 8 : 4;
     const long rb = z.groups * tiles_of(z.R, 128), kb = z.groups * tiles_of(Nk, 32 * z.kv_waves);
     z.few_rows = z.R <= 32 && Nk <= 1024;
     z.fwd_splits = z.few_rows ? 1 : splits_for(rb, tiles_of(Nk, 64), 4);
@@ -895,6 +1154,16 @@ Sizes sizes_of(int B, int Nq, int Nk, int H, int Hk, int D) {
     z.fwd_part = align_up(z.fwd_splits > 1 ? rows * z.fwd_splits * D * 4 : 0, 256);
     z.fwd_bytes = z.fwd_splits > 1 ? z.fwd_part + rows * z.fwd_splits * 8 : 0;
     z.delta_bytes = align_up(rows * 4, 256);
+    // one block for all keys of a (sample, kv head): nine waves fit a CU's LDS and registers up to 64 columns.  Against the two kernels: 128 x 256 rows x 257
+    // keys x 12 heads of 64 165 us instead of 203, 128 keys 77 instead of 101, 16 x 500 x 200 x 8 35 instead of 45, 24 x 286 x 93 x 16 heads of 96 over 4 46
+    // instead of 60; 64 x 256 x 77 x 16 heads of 128 124 instead of 142, 32 x 256 x 77 x 8 heads of 128 45 as before
+    z.one_waves = Nk < 1 || Nq < 1 ? 0 : Nk <= 128 ? 4 : D <= 64 && Nk <= 288 ? 9 : 0;
+    if (z.one_waves) {
+        // shares of the rows no more than the blocks that two a CU hold (a few over that wait for a second round: 46 us, or 58), of eight tiles at least
+        z.kv_splits = (int)std::max<long>(1, std::min(tiles_of(z.R, 32) / 8, 2L * num_cus() / std::max<long>(1, z.groups)));
+        z.delta_bytes = 0;
+        z.dq_splits = 1;
+    }
     const size_t dq = z.dq_splits > 1 ? rows * z.dq_splits * D * 4 : 0, kv = z.kv_splits > 1 ? 2 * (size_t)z.groups * Nk * z.kv_splits * D * 4 : 0;
     z.bwd_bytes = z.delta_bytes + std::max(dq, kv);
     return z;
@@ -1027,7 +1296,24 @@ extern "C" int xq_xattn_backward(const void *q, const void *k, const void *v, co
     a.scale = scale; a.groups = (int)z.groups;
     a.delta = (float *)workspace; a.part = (float *)((char *)workspace + z.delta_bytes);
     unsigned blocks;
-    if (Nq > 0) {
+    if (z.one_waves) {
+        plan_blocks(a, 1, z.kv_splits, blocks);
+#define XA_GO(DT, W)                                                                                                                  \
+    do {                                                                                                                              \
+        if (z.kv_splits > 1) hipLaunchKernelGGL((xattn_bwd_kernel<DT, W, true>), dim3(blocks), dim3(64 * W), 0, s, a);                \
+        else hipLaunchKernelGGL((xattn_bwd_kernel<DT, W, false>), dim3(blocks), dim3(64 * W), 0, s, a);                               \
+    } while (0)
+        if (z.one_waves == 9) {
+            if (D <= 32) XA_GO(32, 9);
+            else XA_GO(64, 9);
+        } else {
+#define XA_CALL(DT) XA_GO(DT, 4)
+            XA_BY_WIDTH(D, XA_CALL);
+#undef XA_CALL
+        }
+#undef XA_GO
+    }
+    if (Nq > 0 && !z.one_waves) {
         plan_blocks(a, tiles_of(z.R, 128), z.dq_splits, blocks);
         if (z.dq_splits > 1) {
 #define XA_CALL(DT) hipLaunchKernelGGL((xattn_dq_kernel<DT, true>), dim3(blocks), dim3(256), 0, s, a)
@@ -1041,24 +1327,22 @@ extern "C" int xq_xattn_backward(const void *q, const void *k, const void *v, co
 #undef XA_CALL
         }
     }
-    if (Nk > 0) {
+    if (Nk > 0 && !z.one_waves) {
         plan_blocks(a, tiles_of(Nk, 32 * z.kv_waves), z.kv_splits, blocks);
 #define XA_GO(DT, W)                                                                                                                  \
     do {                                                                                                                              \
         if (z.kv_splits > 1) hipLaunchKernelGGL((xattn_dkdv_kernel<DT, W, true>), dim3(blocks), dim3(64 * W), 0, s, a);               \
         else hipLaunchKernelGGL((xattn_dkdv_kernel<DT, W, false>), dim3(blocks), dim3(64 * W), 0, s, a);                              \
     } while (0)
-        if (z.kv_waves == 8) XA_GO(128, 8);
-        else {
-#define XA_CALL(DT) XA_GO(DT, 4)
-            XA_BY_WIDTH(D, XA_CALL);
-#undef XA_CALL
-        }
+        if (D <= 32) XA_GO(32, 4);
+        else if (D <= 64) XA_GO(64, 4);
+        else if (D <= 96) XA_GO(96, 4);
+        else XA_GO(128, 8);
 #undef XA_GO
-        if (z.kv_splits > 1) {
-            const long total = 2 * z.groups * (long)Nk * (D / 4);
-            hipLaunchKernelGGL((xattn_sum_kernel<1>), dim3((unsigned)((total + 255) / 256)), dim3(256), 0, s, a, D / 4, reciprocal_of(D / 4), total);
-        }
+    }
+    if (Nk > 0 && z.kv_splits > 1) {
+        const long total = 2 * z.groups * (long)Nk * (D / 4);
+        hipLaunchKernelGGL((xattn_sum_kernel<1>), dim3((unsigned)((total + 255) / 256)), dim3(256), 0, s, a, D / 4, reciprocal_of(D / 4), total);
     }
     return xq_check_launch(fn);
 }
