@@ -86,7 +86,10 @@ def both(q, k, v, lens=None, mask=None, scale=None, g=None):
 
 SHAPES = [(1, 1, 1, 1, 1, 8), (2, 1, 257, 12, 12, 64), (1, 1, 5000, 8, 2, 128), (3, 5, 63, 4, 4, 32), (2, 130, 65, 6, 2, 96), (2, 129, 300, 4, 1, 80),
           (1, 700, 1000, 2, 2, 128), (2, 33, 64, 3, 3, 40), (1, 2, 9001, 2, 1, 64), (4, 77, 2, 4, 2, 16), (8, 16, 128, 2, 2, 24), (1, 1500, 31, 8, 1, 64),
-          (9, 257, 256, 8, 8, 64), (1, 3, 4097, 16, 1, 128), (2, 1, 1025, 16, 1, 96), (1, 17, 700, 1, 1, 112)]
+          (9, 257, 256, 8, 8, 64), (1, 3, 4097, 16, 1, 128), (2, 1, 1025, 16, 1, 96), (1, 17, 700, 1, 1, 112),
+          # the backward in one block, its rows whole and split, at the ends of its sizes
+          (2, 40, 128, 6, 2, 128), (1, 1000, 127, 2, 1, 120), (1, 700, 100, 5, 1, 56), (3, 31, 1, 2, 2, 128), (2, 65, 288, 4, 4, 64), (1, 900, 289, 2, 2, 64),
+          (1, 800, 281, 3, 1, 32), (2, 33, 129, 3, 3, 8), (1, 2100, 33, 2, 2, 96), (1, 600, 97, 24, 4, 128), (70, 100, 200, 1, 1, 48)]
 
 
 @gpu
@@ -436,8 +439,11 @@ def test_refusals():
         assert call(B=0, q=None, strides=None) == 0
     assert bwd(gstrides=odd) == -1 and "dk has to be" in err()
     assert bwd(lse=None) == -1 and bwd(dq=None) == -1
-    need = l.xq_xattn_backward_workspace_bytes(2, 3, 5, 4, 2, 16)
-    assert need >= 2 * 3 * 4 * 4 and bwd(nbytes=need - 1) == -2 and "too small" in err()
+    need = l.xq_xattn_backward_workspace_bytes(2, 3, 400, 4, 2, 16)
+    assert need >= 2 * 3 * 4 * 4 and bwd(Nk=400, nbytes=need - 1) == -2 and "too small" in err()
+    need = l.xq_xattn_backward_workspace_bytes(2, 900, 5, 4, 2, 16)          # the rows split over blocks
+    assert need >= 2 * 2 * 2 * 2 * 5 * 16 * 4 and bwd(Nq=900, nbytes=need - 1) == -2 and "too small" in err()
+    assert l.xq_xattn_backward_workspace_bytes(2, 3, 5, 4, 2, 16) == 0
     need = l.xq_xattn_forward_workspace_bytes(1, 1, 8192, 8, 8, 128)
     assert need > 0 and fwd(B=1, Nq=1, Nk=8192, H=8, Hk=8, D=128, ws=one, nbytes=need - 1) == -2
     assert l.xq_xattn_forward_workspace_bytes(64, 256, 257, 12, 12, 64) == 0
