@@ -1173,7 +1173,8 @@ int check_sizes(const char *fn, int B, int Nq, int Nk, int H, int Hk, int D, flo
     if (B < 0 || Nq < 0 || Nk < 0 || H < 1 || Hk < 1) return xq_set_error(XQ_EINVAL, "%s: bad sizes (H=%ld, Hk=%ld)", fn, (long)H, (long)Hk);
     if (H % Hk) return xq_set_error(XQ_EINVAL, "%s: %ld query heads do not share %ld kv heads evenly", fn, (long)H, (long)Hk);
     if (D < 8 || D > 128 || D % 8) return xq_set_error(XQ_EINVAL, "%s: head dim %ld is not a multiple of 8 up to 128", fn, (long)D);
-    if (!(scale > 0.0f) || !(scale < INFINITY)) return xq_set_error(XQ_EINVAL, "%s: scale has to be positive and finite", fn);
+    // (the backward begins its products at lse / scale: that has to stay far from fp32's end)
+    if (!(scale >= 0x1p-64f) || !(scale <= 0x1p64f)) return xq_set_error(XQ_EINVAL, "%s: scale has to lie in 2^-64 .. 2^64", fn);
     if ((long)B * Hk * (tiles_of((long)Nq * (H / Hk), 128) + 8) > (1L << 22) || (long)B * Hk * (tiles_of(Nk, 128) + 8) > (1L << 22) ||
         (long)Nq * (H / Hk) > 0x7fffff00L || (long)B * H * Nq > 0x7fffffffL || (long)B * Hk * Nk > 0x3fffffffL)
         return xq_set_error(XQ_EINVAL, "%s: too many rows (%ld) or keys (%ld) for one call", fn, (long)B * H * Nq, (long)B * Hk * Nk);

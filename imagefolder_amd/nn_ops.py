@@ -373,7 +373,7 @@ def cross_attention(q, k, v, kv_lens=None, key_mask=None, scale=None):
          up to 128; any strides (a packed k / v projection is read in place; rows that are not 16-byte aligned are copied first);
       kv_lens: int32 / int64 (B,), how many of a sample's keys are valid (clamped to 0 .. Nk: no host check); key_mask: bool (B, Nk), True = valid.  Both on the
          device; a key is valid where both say so.  What lies in masked places (infinities, NaN) reaches nothing; a sample without a valid key gives zeros;
-      scale: positive; default D ** -0.5.
+      scale: 2^-64 .. 2^64; default D ** -0.5.
     CPU tensors: the same in plain fp32 operations."""
     if q.is_cuda:
         if torch.is_autocast_enabled("cuda"):

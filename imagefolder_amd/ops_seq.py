@@ -293,8 +293,8 @@ def check_cross_attention(q, k, v, kv_lens, key_mask, scale):
     if key_mask is not None and (tuple(key_mask.shape) != (B, Nk) or key_mask.dtype != torch.bool):
         raise XqError(f"cross_attention: key_mask is a bool tensor of shape {(B, Nk)} (got {key_mask.dtype}, shape {tuple(key_mask.shape)})")
     scale = float(D) ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < float("inf"):
-        raise XqError(f"cross_attention: scale = {scale} is not positive and finite")
+    if not 2.0 ** -64 <= scale <= 2.0 ** 64:
+        raise XqError(f"cross_attention: scale = {scale} is not positive, 2^-64 .. 2^64")
     return scale
 
 

@@ -587,7 +587,7 @@ int xq_embedding_backward(const void *idx, int idx_i64, const void *g, int g_bf1
  *   dimension has stride 1, pointers are 16-byte aligned, strides multiples of 8 (0 for a broadcast dimension), 64 tokens within 2^30 elements.  Head h reads kv head h / (H / Hk).
  *   D a multiple of 8, 8 .. 128.  Nq, Nk from 0 on.
  *   kv_lens (nullable): DEVICE int32 or int64 (lens_i64) [B], valid keys of a sample (clamped to 0 .. Nk); key_mask (nullable): DEVICE bytes [B][Nk], 0 = masked.
- *   What lies in masked places reaches nothing.  A sample without a valid key: rows of zeros, lse = -inf, zero gradients.  scale > 0.
+ *   What lies in masked places reaches nothing.  A sample without a valid key: rows of zeros, lse = -inf, zero gradients.  scale in 2^-64 .. 2^64.
  *   out [B][Nq][H][D] bf16 contiguous; lse (nullable) fp32 [B][Hk][Nq * H / Hk] (row = token * (H / Hk) + head of the group), what the backward reads.
  *   workspace: xq_xattn_forward_workspace_bytes (0 where the keys are not split over blocks). */
 size_t xq_xattn_forward_workspace_bytes(int B, int Nq, int Nk, int H, int Hk, int D);

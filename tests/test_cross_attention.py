@@ -119,14 +119,14 @@ def test_against_64_bits(B, Nq, Nk, H, Hk, D, case):
 
 
 @gpu
-@pytest.mark.parametrize("Nq", [1, 200])
+@pytest.mark.parametrize("Nq,Nk,D", [(1, 333, 64), (200, 333, 64), (200, 260, 64), (90, 120, 128), (900, 70, 96)])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf"), torch.finfo(BF).min])
-def test_what_lies_in_masked_places_reaches_nothing(Nq, bad):
+def test_what_lies_in_masked_places_reaches_nothing(Nq, Nk, D, bad):
     from imagefolder_amd import nn_ops
-    B, Nk, H, Hk, D = 3, 333, 4, 2, 64
+    B, H, Hk = 3, 4, 2
     torch.manual_seed(5)
     q, k, v, g = (torch.randn(*s, device="cuda").to(BF) for s in ((B, Nq, H, D), (B, Nk, Hk, D), (B, Nk, Hk, D), (B, Nq, H, D)))
-    lens = torch.tensor([100, 0, 333], device="cuda")
+    lens = torch.tensor([Nk // 3, 0, Nk], device="cuda")
     mask = torch.rand(B, Nk, device="cuda") < 0.5
     ok = valid_keys(B, Nk, lens, mask, "cuda")
     results = []
@@ -196,6 +196,16 @@ def test_extreme_scores(Nq):
 
 
 @gpu
+@pytest.mark.parametrize("Nk,D", [(50, 64), (50, 128), (400, 64), (400, 128)])
+def test_the_smallest_scale(Nk, D):
+    """scores that are all but equal: the mean of the values; lse / scale, where the backward's products begin, is log(Nk) 2^64 then.  An accumulator that begins
+    there loses q k^T beside it, which is 2^-50 of it: P = exp(0) / Nk up to 2^-22, and the gradients are those of the oracle"""
+    torch.manual_seed(Nk + D)
+    q, k, v, g = (torch.randn(2, n, 2, D, device="cuda").to(BF) for n in (70, Nk, Nk, 70))
+    both(q, k, v, scale=2.0 ** -64, g=g)
+
+
+@gpu
 def test_strides_alignment_and_broadcasts():
     from imagefolder_amd import nn_ops
     torch.manual_seed(0)
@@ -221,7 +231,7 @@ def test_strides_alignment_and_broadcasts():
 @gpu
 def test_same_bits_from_run_to_run():
     from imagefolder_amd import nn_ops
-    for B, Nq, Nk, H, Hk, D in ((2, 300, 700, 8, 2, 64), (1, 2, 6000, 8, 8, 128)):
+    for B, Nq, Nk, H, Hk, D in ((2, 300, 700, 8, 2, 64), (1, 2, 6000, 8, 8, 128), (3, 900, 257, 4, 4, 64), (2, 700, 90, 16, 4, 96)):
         q, k, v, g = (torch.randn(B, n, h, D, device="cuda").to(BF).requires_grad_(True) for n, h in ((Nq, H), (Nk, Hk), (Nk, Hk), (Nq, H)))
         runs = []
         for _ in range(3):
@@ -402,7 +412,7 @@ def test_refusals():
                      (dict(q=t(2, 3, 4, 8)), "go together"), (dict(q=t(2, 3, 5, 16)), "evenly"), (dict(k=t(2, 5, 0, 16), v=t(2, 5, 0, 16)), "evenly"),
                      (dict(kv_lens=torch.zeros(3, dtype=torch.int32)), "kv_lens"), (dict(kv_lens=torch.zeros(2)), "kv_lens"),
                      (dict(key_mask=torch.zeros(2, 5)), "key_mask"), (dict(key_mask=torch.zeros(2, 4, dtype=torch.bool)), "key_mask"), (dict(scale=0.0), "scale"),
-                     (dict(scale=-1.0), "scale"), (dict(scale=float("inf")), "scale"), (dict(scale=float("nan")), "scale"),
+                     (dict(scale=-1.0), "scale"), (dict(scale=float("inf")), "scale"), (dict(scale=float("nan")), "scale"), (dict(scale=2.0 ** -65), "scale"), (dict(scale=2.0 ** 65), "scale"),
                      (dict(q=t(2, 3, 4, 16, dt=torch.float32)), "bf16"), (dict(v=t(2, 5, 2, 16, dt=torch.float16)), "bf16"),
                      (dict(kv_lens=torch.zeros(2, dtype=torch.int32, device="meta")), "one device")):
         with pytest.raises(XqError, match=what):
@@ -431,6 +441,7 @@ def test_refusals():
         assert call(D=12) == -1 and "multiple of 8" in err()
         assert call(D=136) == -1 and call(B=-1) == -1 and call(Hk=0) == -1
         assert call(scale=0.0) == -1 and call(scale=float("nan")) == -1 and "scale" in err()
+        assert call(scale=2.0 ** -65) == -1 and call(scale=2.0 ** 65) == -1 and "scale" in err()
         assert call(q=None) == -1 and "null" in err()
         assert call(q=ctypes.c_void_p(8)) == -1 and "q has to be" in err()
         assert call(strides=odd) == -1 and "k has to be" in err()
