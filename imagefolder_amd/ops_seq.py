@@ -253,7 +253,7 @@ class PackedAttentionFn(torch.autograd.Function):
         x = qkv.detach().contiguous()
         if x.data_ptr() & 15:
             x = x.clone()
-        q, k, v = x.view(B, N, 3, num_heads, -1).unbind(2)
+        q, k, v = x.view(B, N, 3, num_heads, C3 // (3 * num_heads)).unbind(2)
         scale = float(q.shape[3]) ** -0.5
         out, lse = _xattn_forward(q, k, v, None, None, scale, True)
         ctx.save_for_backward(x, out, lse)

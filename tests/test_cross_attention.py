@@ -351,6 +351,17 @@ def test_packed_self_attention_of_other_head_widths(N, H, D):
 
 
 @gpu
+def test_packed_self_attention_of_an_empty_batch():
+    from imagefolder_amd import nn_ops
+    for B, N in ((0, 5), (2, 0)):
+        qkv = torch.zeros(B, N, 3 * 2 * 32, device="cuda", dtype=BF, requires_grad=True)
+        y = nn_ops.attention_qkvpacked(qkv, 2)
+        assert y.shape == (B, N, 64)
+        (dx,) = torch.autograd.grad(y, (qkv,), torch.zeros_like(y))
+        assert dx.shape == qkv.shape
+
+
+@gpu
 def test_autocast_casts_fp32():
     from imagefolder_amd import nn_ops
     from imagefolder_amd._lib import XqError
