@@ -86,7 +86,7 @@ class DINOv2Encoder(nn.Module):
                     z_list = z.view(x.size(0), P * H, W, -1).chunk(chunks=P, dim=1)
                     z_list = [m._pos_embed(zz)[:, 1:, ] for zz in z_list]  # cls stripped (:164,171)
                     x = torch.cat([x, ] + z_list, dim=1)
-                    x = x + nn_ops.embedding(self.lvl1LC, self.lvl_embed.weight)  # (1, L, D) broadcast over the batch (upstream expands the index first)
+                    x = x + nn_ops.module_embedding(self.lvl_embed, self.lvl1LC)  # (1, L, D) broadcast over the batch (upstream expands the index first)
                 else:
                     x = torch.cat([x, z + self.latent_pos_embed], dim=1)
         return x
@@ -176,7 +176,7 @@ class DINOv2Decoder(nn.Module):
                 z = z.float() + self.latent_pos_embed
             x = torch.cat([x, z], dim=1)
             if self.abs_pos_embed:
-                x = x + nn_ops.embedding(self.lvl1LC, self.lvl_embed.weight)  # (1, L, D) broadcast over the batch (upstream expands the index first)
+                x = x + nn_ops.module_embedding(self.lvl_embed, self.lvl1LC)  # (1, L, D) broadcast over the batch (upstream expands the index first)
         return x
 
     def forward(self, z):

@@ -366,6 +366,15 @@ def embedding(idx, weight, scale=1.0, padding_idx=None, dtype=None):
     return ops_seq.embedding(idx, weight, scale, padding_idx, dtype)
 
 
+def module_embedding(module, idx):
+    """the lookup of an nn.Embedding inside a model: nn_ops.embedding, or the module itself for what that does not take (other types, a renormalised or sparse
+    table, gradients scaled by frequency)"""
+    w = module.weight
+    if w.is_cuda and w.dtype in (torch.bfloat16, torch.float32) and module.max_norm is None and not (module.sparse or module.scale_grad_by_freq):
+        return embedding(idx, w, padding_idx=module.padding_idx)
+    return module(idx)
+
+
 def cross_attention(q, k, v, kv_lens=None, key_mask=None, scale=None):
     """Attention of one sequence to another: softmax(scale q k^T over the valid keys) v -> (B, Nq, H, D); one token (Nq = 1, serving) to thousands, gradients
     for q, k and v (csrc/xq_xattn.hip; no N x N buffer, no atomics).

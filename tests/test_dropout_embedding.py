@@ -531,3 +531,22 @@ def test_level_embedding_of_the_tokenizer_runs_on_the_lookup():
     g = torch.randn_like(seq)
     (dw,) = torch.autograd.grad(seq, [enc.lvl_embed.weight], g)
     check_gradient(enc.lvl1LC, g.sum(0, keepdim=True), enc.lvl_embed.weight.shape[0], 1.0, dw)
+
+
+@gpu
+def test_an_embedding_module_of_another_kind_runs_as_it_is():
+    from imagefolder_amd import nn_ops
+    torch.manual_seed(4)
+    idx = torch.randint(0, 9, (3, 5), device="cuda")
+    for kw in (dict(dtype=torch.float16), dict(dtype=torch.float64), dict(max_norm=1.0), dict(scale_grad_by_freq=True), dict(sparse=True)):
+        m = torch.nn.Embedding(9, 16, device="cuda", **kw)
+        nn_ops.IMPL.pop("embedding", None)
+        y = nn_ops.module_embedding(m, idx)
+        assert "embedding" not in nn_ops.IMPL and torch.equal(y, m(idx)) and y.dtype == m.weight.dtype
+    m = torch.nn.Embedding(9, 16, padding_idx=2, device="cuda")
+    y = nn_ops.module_embedding(m, idx)
+    assert nn_ops.IMPL["embedding"] == "hip" and torch.equal(y, m(idx))
+    (dw,) = torch.autograd.grad(y, (m.weight,), torch.ones_like(y))
+    want = torch.bincount(idx.reshape(-1), minlength=9).float()
+    want[2] = 0
+    assert torch.equal(dw, want[:, None].expand(9, 16))
