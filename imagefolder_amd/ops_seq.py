@@ -6,6 +6,7 @@ import ctypes
 import functools
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import XqError, check
@@ -41,6 +42,16 @@ def _same_device(name, first, *others):
     for t in others:
         if t is not None and t.device != first.device:
             raise XqError(f"{name}: all tensors have to live on one device (got {first.device} and {t.device})")
+
+
+def _first_order(backward):
+    """a backward pass through a kernel has no graph of its own: differentiating through it is an error, not a zero (the check for it only where a graph is asked for)"""
+    checked = once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        return (checked if torch.is_grad_enabled() else backward)(ctx, *grads)
+    return run
 
 
 # ---- dropout -------------------------------------------------------------------------------------------------------------------------------
@@ -85,6 +96,7 @@ class DropoutFn(torch.autograd.Function):
         return _dropout(xd, rd, p, key, xd.dtype if rd is None else rd.dtype)
 
     @staticmethod
+    @_first_order
     def backward(ctx, g):
         (key,) = ctx.saved_tensors
         p, dtype, stride = ctx.cfg
@@ -146,6 +158,7 @@ class EmbeddingFn(torch.autograd.Function):
         return _embedding(ic, w, scale, dtype)
 
     @staticmethod
+    @_first_order
     def backward(ctx, g):
         (ic,) = ctx.saved_tensors
         V, D, scale, skip, wdtype = ctx.cfg
@@ -237,6 +250,7 @@ class CrossAttentionFn(torch.autograd.Function):
         return out
 
     @staticmethod
+    @_first_order
     def backward(ctx, g):
         q, k, v, out, lse, lens, mask = ctx.saved_tensors
         dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
@@ -261,6 +275,7 @@ class PackedAttentionFn(torch.autograd.Function):
         return out.view(B, N, C3 // 3)
 
     @staticmethod
+    @_first_order
     def backward(ctx, g):
         x, out, lse = ctx.saved_tensors
         B, N, H, D = out.shape

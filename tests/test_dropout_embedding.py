@@ -550,3 +550,22 @@ def test_an_embedding_module_of_another_kind_runs_as_it_is():
     want = torch.bincount(idx.reshape(-1), minlength=9).float()
     want[2] = 0
     assert torch.equal(dw, want[:, None].expand(9, 16))
+
+
+@gpu
+def test_second_derivatives_are_refused():
+    from imagefolder_amd import nn_ops
+    w = torch.randn(9, 16, device="cuda", requires_grad=True)
+    x = torch.randn(4, 16, device="cuda", requires_grad=True)
+    q = torch.randn(1, 4, 2, 8, device="cuda").bfloat16().requires_grad_(True)
+    packed = torch.randn(1, 4, 3 * 2 * 8, device="cuda").bfloat16().requires_grad_(True)
+    key = torch.tensor([1, 2], device="cuda")
+    idx = torch.tensor([1, 1, 3], device="cuda")
+    for leaf, f in ((w, lambda t: nn_ops.embedding(idx, t)), (x, lambda t: nn_ops.dropout(t, 0.5, key=key)), (q, lambda t: nn_ops.cross_attention(t, t, t)),
+                    (packed, lambda t: nn_ops.attention_qkvpacked(t, 2))):
+        y = f(leaf)
+        plain, = torch.autograd.grad(y.float().square().sum(), (leaf,), retain_graph=True)
+        again, = torch.autograd.grad(y.float().square().sum(), (leaf,), create_graph=True)
+        assert torch.equal(plain, again.detach())
+        with pytest.raises(RuntimeError, match="twice|once_differentiable"):
+            torch.autograd.grad(again.float().sum(), (leaf,))
