@@ -4,11 +4,11 @@
 // gradient: dw[v] = scale * sum of g[n] over the tokens n with idx[n] = v — no floating-point atomics: the tokens are sorted by row (stable: ascending n
 // inside a row) and every row of dw is one fp32 chain, written once (rows without a token with zeros: no clearing pass).
 //
-// The sort is two launches, not a radix sort's pass per digit: (1) `embed_bin_kernel` — every block sorts a slice of 2048 tokens by row in LDS and writes the
+// The sort is two launches, not a radix sort's pass per digit: (1) `embed_bin_kernel` — every block sorts a slice of 1024 tokens by row in LDS and writes the
 // sorted list and where each bucket (256 or up to 1024 buckets of 2^shift rows) begins in it; (2) `embed_sort_kernel` — one block per bucket gathers its pieces of
 // every slice's list (they follow each other in token order).  The position of a bucket in the sorted whole needs no scan over buckets: it is the sum of the slices'
-// starts of that bucket.  A slice is sorted by row whole, and not by bucket alone, for 4 us more of the first launch (11 us instead of 7): it leaves the second
-// one no ranking, so that a bucket with a frequent row (14000 of 100000 tokens) takes it 22 us instead of 40, a table read at one row only 104 instead of 250 (100000
+// starts of that bucket.  A slice is sorted by row whole, and not by bucket alone, for 2 us more of the first launch (9 us instead of 7): it leaves the second
+// one no ranking, so that a bucket with a frequent row (14000 of 100000 tokens) takes it 20 us instead of 40, a table read at one row only 96 instead of 250 (100000
 // tokens), and 6 to 7 as before where no row is frequent.
 // The sums are two more: (3) `embed_sum_kernel` — rows of up to `chunk` tokens whole, and of the longer ones (a frequent word, a padding id) the pieces
 // that lie in each `chunk` of sorted positions, so that one row's tokens are read by many blocks; (4) `embed_long_kernel` adds a long row's pieces in order.
@@ -20,7 +20,7 @@
 
 namespace {
 
-constexpr int TILE = 2048;                               // tokens that a block of the first launch ranks at once
+constexpr int TILE = 1024, BIN_THREADS = 512;            // tokens and threads of a block of the first launch (2048 and 1024: 11 us instead of 9)
 
 // ---- forward ------------------------------------------------------------------------------------------------------------------------------
 
@@ -160,7 +160,7 @@ __device__ __forceinline__ void tile_places(uint32_t *seen, int pitch, int digit
 
 // A slice is one tile.  Its tokens are sorted by row in LDS — by the row's low bits, then, stable, by its bucket — and written with what the second launch needs to
 // place them without ranking them again: low bits | place in the slice's run of the row << 10 | last of the run << 21, token.  starts[slice][bucket], buckets + 1.
-template <typename TI, int BIN_THREADS>
+template <typename TI>
 __global__ __launch_bounds__(BIN_THREADS) void embed_bin_kernel(const TI *__restrict__ idx, long N, long V, long skip, int shift, int buckets, int bits,
                                                                 int pitch, uint2 *__restrict__ list, uint32_t *__restrict__ starts) {
     constexpr int WAVES = BIN_THREADS / 64, ROUNDS = TILE / BIN_THREADS;
@@ -622,13 +622,12 @@ extern "C" int xq_embedding_backward(const void *idx, int idx_i64, const void *g
     uint32_t *starts = (uint32_t *)(ws + p.o_starts), *rows = (uint32_t *)(ws + p.o_rows), *order = (uint32_t *)(ws + p.o_order),
              *edge = (uint32_t *)(ws + p.o_edge);
     float *part = (float *)(ws + p.o_part);
-    // sixteen waves a block where their counters fit the 64 KB of a launch (up to 512 buckets and rows a bucket), eight otherwise
     const int pitch = std::max(p.buckets, 1 << p.shift);
-#define XQ_BIN(TI, THREADS)                                                                                                                        \
-    hipLaunchKernelGGL((embed_bin_kernel<TI, THREADS>), dim3(p.slices), dim3(THREADS), (size_t)(THREADS / 64 + 1) * pitch * 4, s, (const TI *)idx, (long)N, (long)V, \
+#define XQ_BIN(TI)                                                                                                                                  \
+    hipLaunchKernelGGL((embed_bin_kernel<TI>), dim3(p.slices), dim3(BIN_THREADS), (size_t)(BIN_THREADS / 64 + 1) * pitch * 4, s, (const TI *)idx, (long)N, (long)V, \
                        (long)skip, p.shift, p.buckets, p.bucket_bits, pitch, list, starts)
-    if (pitch <= 512) { if (idx_i64) XQ_BIN(int64_t, 1024); else XQ_BIN(int32_t, 1024); }
-    else { if (idx_i64) XQ_BIN(int64_t, 512); else XQ_BIN(int32_t, 512); }
+    if (idx_i64) XQ_BIN(int64_t);
+    else XQ_BIN(int32_t);
 #undef XQ_BIN
 #define XQ_SORT(THREADS)                                                                                                                              \
     hipLaunchKernelGGL((embed_sort_kernel<THREADS>), dim3(p.buckets), dim3(THREADS), (size_t)((THREADS / 64 + 1) << p.shift) * 4, s, list, starts, (long)V, \
