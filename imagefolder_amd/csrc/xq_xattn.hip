@@ -12,7 +12,9 @@
 // 8 (r >> 2) + 4 (lane >> 5)): the forward and the dq kernel hold one row per lane (S^T = K Q^T, P stays in registers and is the B operand of O^T = V^T P^T;
 // V^T comes from the row-major LDS tile through ds_read_b64_tr_b16), the dk / dv kernel one key per lane.
 // Masked keys are zero rows in LDS and -inf in S: what lies in memory there (infinities, NaN) reaches nothing.
-// Roundings to bf16: P and dS before their products (they are MFMA operands), the results once; everything else is fp32.
+// Roundings to bf16: P and dS before their products (they are operands of the bf16 matrix instructions; fp16 would not hold the range of the other operand, two
+// bf16 parts would double the products), the results once; everything else is fp32.  Against 64 bits the results are 0.0021 .. 0.0027 off in norm (rounding them
+// alone: 0.0017, the operand's rounding as much again in squares, and for dq / dk what delta takes from the rounded O).
 #include "xq_common.hpp"
 #include "xq_internal.hpp"
 #include "../../include/xq_ops.h"
@@ -844,8 +846,8 @@ __global__ __launch_bounds__(64 * W, DT > 64 ? 2 : 3) void xattn_dkdv_kernel(Arg
 // ---------------------------------------------------------------------------------------------------------------------------------------------
 // the whole backward of a (sample, kv head) whose keys fit one block (up to 32 W of them): one key per lane as in the dk / dv kernel; dS also goes to LDS
 // (key-major), and the waves share out dq = dS k of the tile before.  q, dO and out are read once, P and dP computed once: five products instead of seven.
-// 128 x 256 rows x 257 keys x 12 heads of 64 (nine waves): 165 us, 2.4 TB/s of its 400 MB and 350 TFLOP/s.  Bound by what no single unit is: LDS reads take about
-// half of the time, the scores' arithmetic 40 %, the matrix pipe a quarter, and one block a CU leaves nothing beside its first loads and last stores.
+// 128 x 256 rows x 257 keys x 12 heads of 64 (nine waves): 165 us, 2.4 TB/s of its 400 MB and 390 TFLOP/s.  Bound by latency: the vector units and LDS are busy 32 % of
+// the cycles each, the matrix pipe 20 %, and the waves wait half of theirs (a CU holds one such block: nothing runs beside its first loads and last stores).
 // ---------------------------------------------------------------------------------------------------------------------------------------------
 template <int DT, int W, bool SPLIT>
 __global__ __launch_bounds__(64 * W, DT > 64 ? 2 : 3) void xattn_bwd_kernel(Args a) {
