@@ -885,15 +885,17 @@ __global__ __launch_bounds__(64 * W, DT > 64 ? 2 : 3) void xattn_bwd_kernel(Args
     const bool wave_live = __any(valid), all_valid = __all(valid);
     // (the prologue's loads are all in flight before the first is waited for)
     bf16x8 vf[KS];
-    load_row<DT>(a.v.p + b * a.v.sb + hk * a.v.sh + (long)nc * a.v.sn, a.D, hh, vf);
-    uint4 kr[DT / 16];
+    const short *vb = a.v.p + b * a.v.sb + hk * a.v.sh;
+    if (!V_IN_LDS) load_row<DT>(vb + (long)nc * a.v.sn, a.D, hh, vf);
+    uint4 kr[DT / 16], vr[DT / 16];
 #pragma unroll
     for (int j = 0; j < DT / 16; ++j) {
         const int id = tid + 64 * W * j, row = id / (DT / 8), chunk = id % (DT / 8);
         bool there = row < len && 8 * chunk < a.D;
         if (mask && there) there = mask[row] != 0;
-        kr[j] = make_uint4(0u, 0u, 0u, 0u);
+        kr[j] = vr[j] = make_uint4(0u, 0u, 0u, 0u);
         if (there) kr[j] = *reinterpret_cast<const uint4 *>(kb + (long)row * a.k.sn + 8 * chunk);
+        if (V_IN_LDS && there) vr[j] = *reinterpret_cast<const uint4 *>(vb + (long)row * a.v.sn + 8 * chunk);
     }
     if (!wave_live) {
         for (int j = 0; j < SB; ++j)
@@ -1009,15 +1011,13 @@ __global__ __launch_bounds__(64 * W, DT > 64 ? 2 : 3) void xattn_bwd_kernel(Args
     share((a.R + QT - 1) / QT, split, SPLIT ? a.splits : 1, t0, t1);
     if (t0 < t1) load(t0 * QT);
     const uint32_t Kw = Kb + wave * 32 * T::ROW + row_at, Vw = Vb + wave * 32 * T::ROW + row_at;
-    if (V_IN_LDS) {
-#pragma unroll
-        for (int k = 0; k < KS; ++k) *(lds_ptr<bf16x8>)(uintptr_t)(Vw ^ 32 * k) = vf[k];
-    }
-    // every key's row of k, zeros for one that is not valid: what dq adds of it is 0 x 0
+    // every key's row, zeros for one that is not valid: what dq adds of its k is 0 x 0
 #pragma unroll
     for (int j = 0; j < DT / 16; ++j) {
         const int id = tid + 64 * W * j;
-        *(lds_ptr<u32x4>)(uintptr_t)(Kb + T::place(id / (DT / 8), id % (DT / 8))) = __builtin_bit_cast(u32x4, kr[j]);
+        const uint32_t at = T::place(id / (DT / 8), id % (DT / 8));
+        *(lds_ptr<u32x4>)(uintptr_t)(Kb + at) = __builtin_bit_cast(u32x4, kr[j]);
+        if (V_IN_LDS) *(lds_ptr<u32x4>)(uintptr_t)(Vb + at) = __builtin_bit_cast(u32x4, vr[j]);
     }
     if (t0 < t1) store(0);
     __syncthreads();
