@@ -1283,6 +1283,12 @@ extern "C" int xq_xattn_backward(const void *q, const void *k, const void *v, co
     for (int i = 0; i < 3; ++i) {
         if (int rc = check_view(fn, names[i], in[i], strides + 3 * i, i ? 1 : H / Hk)) return rc;
         if (int rc = check_view(fn, names[3 + i], gr[i], grad_strides + 3 * i, i ? 1 : H / Hk)) return rc;
+        const int64_t extent[3] = {B, i ? Nk : Nq, i ? Hk : H};
+        for (int j = 0; j < 3; ++j)
+            if (extent[j] > 1 && grad_strides[3 * i + j] == 0) {
+                snprintf(g_err, sizeof(g_err), "%s: %s has a stride of 0 (several rows in one place)", fn, names[3 + i]);
+                return XQ_EINVAL;
+            }
     }
     if (((uintptr_t)out | (uintptr_t)dout) & 15) return xq_set_error(XQ_EINVAL, "%s: out and dout have to be 16-byte aligned", fn);
     const Sizes z = sizes_of(B, Nq, Nk, H, Hk, D);

@@ -460,6 +460,9 @@ def test_refusals():
         assert call(Nq=2 ** 30, B=4) == -1 and "too many" in err()
         assert call(B=0, q=None, strides=None) == 0
     assert bwd(gstrides=odd) == -1 and "dk has to be" in err()
+    for i, name in enumerate(("dq", "dq", "dq", "dk", "dk", "dk", "dv", "dv", "dv")):
+        wide = (ctypes.c_int64 * 9)(*[0 if j == i else 64 for j in range(9)])
+        assert bwd(gstrides=wide) == -1 and f"{name} has a stride of 0" in err()
     assert bwd(lse=None) == -1 and bwd(dq=None) == -1
     need = l.xq_xattn_backward_workspace_bytes(2, 3, 400, 4, 2, 16)
     assert need >= 2 * 3 * 4 * 4 and bwd(Nk=400, nbytes=need - 1) == -2 and "too small" in err()
