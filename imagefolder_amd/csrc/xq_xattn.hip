@@ -110,6 +110,25 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return d;
 }
 
+// Order for the scheduler: N matrix instructions with PER LDS reads each, the reads AHEAD of them (left to itself it puts every read right before its use, and
+// the wave waits for LDS once a product: dk / dv 1110 us at 4 x 4096 x 4352 x 16 x 128, so 1087; dq 197 us at 8 x 2048 x 2048 x 12 x 64, so 192)
+template <int N, int PER, int AHEAD>
+__device__ __forceinline__ void reads_ahead() {
+    __builtin_amdgcn_sched_group_barrier(0x100, PER * AHEAD, 0);
+#pragma unroll
+    for (int i = 0; i < N - AHEAD; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, PER, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
+}
+
+// the larger of a lane's value and its partner's in the other half of the wave (through LDS the tile waits for it: 525 us, so 510)
+__device__ __forceinline__ float max_of_halves(float x) {
+    const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return max3(__uint_as_float(both[0]), __uint_as_float(both[1]), x);
+}
+
 #define XA_MFMA(A, B, C) __builtin_amdgcn_mfma_f32_32x32x16_bf16((A), (B), (C), 0, 0, 0)
 #define XA_MFMA16(A, B, C) __builtin_amdgcn_mfma_f32_16x16x32_bf16((A), (B), (C), 0, 0, 0)
 
@@ -283,7 +302,7 @@ __global__ __launch_bounds__(256, 2) void xattn_fwd_kernel(Args a) {
         for (int j = 0; j < 16; ++j) o[t][j] = 0.0f;
     // m is the reference exponent (log2 units), moved only when a tile's maximum passes it by more than 2^8: P <= 2^8 loses nothing in bf16 / fp32, and the
     // rescale becomes a rare branch.  l: the lane's share of the row's sum, in fp32 before P is rounded (a product of ones with P^T instead of the additions is
-    // an eighth more matrix work at 128 columns: 552 us, now 537)
+    // an eighth more matrix work at 128 columns: 552 us instead of 537)
     float m = -INFINITY, l = 0.0f;
     const f32x16 zero16 = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 
@@ -319,8 +338,7 @@ __global__ __launch_bounds__(256, 2) void xattn_fwd_kernel(Args a) {
             __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                s[h] = zero16;
-                if (h == 1 && !wide) continue;
+                s[h] = zero16;                             // (the second half also where none of its keys is valid: the choice would copy both halves at every tile: 545 us, so 525)
 #pragma unroll
                 for (int k = 0; k < KS; ++k) s[h] = XA_MFMA(lds_16((K ^ 32 * k) + 32 * h * T::ROW), qf[k], s[h]);
             }
@@ -334,14 +352,14 @@ __global__ __launch_bounds__(256, 2) void xattn_fwd_kernel(Args a) {
                         if (!((w >> ((j & 3) + 8 * (j >> 2))) & 1u)) s[h][j] = -INFINITY;
                 }
             }
-            float mx = max3(s[0][0], s[0][1], s[0][2]);
+            float mx = max3(s[0][0], s[0][1], s[0][2]), my = max3(s[1][0], s[1][1], s[1][2]);
 #pragma unroll
-            for (int j = 3; j < 15; j += 2) mx = max3(mx, s[0][j], s[0][j + 1]);
-            mx = max3(mx, s[0][15], s[1][0]);
-#pragma unroll
-            for (int j = 1; j < 15; j += 2) mx = max3(mx, s[1][j], s[1][j + 1]);
-            mx = max3(mx, s[1][15], s[1][15]);
-            mx = max3(mx, __shfl_xor(mx, 32), mx);
+            for (int j = 3; j < 15; j += 2) {
+                mx = max3(mx, s[0][j], s[0][j + 1]);
+                my = max3(my, s[1][j], s[1][j + 1]);
+            }
+            mx = max3(mx, s[0][15], max3(my, s[1][15], my));
+            mx = max_of_halves(mx);
             const float cand = mx * c;
             if (__any(cand > m + 8.0f)) {
                 const float mn = fmaxf(m, cand);
@@ -482,7 +500,7 @@ __global__ __launch_bounds__(256, 2) void xattn_few_rows_kernel(Args a) {
 #pragma unroll
         for (int j = 3; j < 15; j += 2) mx = max3(mx, s[j], s[j + 1]);
         mx = max3(mx, s[15], s[15]);
-        mx = max3(mx, __shfl_xor(mx, 32), mx);
+        mx = max_of_halves(mx);
         const float cand = mx * c;
         if (__any(cand > m + 8.0f)) {
             const float mn = fmaxf(m, cand);
@@ -658,6 +676,7 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(Args a) {
                     s = XA_MFMA(lds_16((K ^ 32 * k) + 32 * h * T::ROW), qf[k], s);
                     p = XA_MFMA(lds_16((V ^ 32 * k) + 32 * h * T::ROW), df[k], p);
                 }
+                if (DT <= 96) reads_ahead<2 * KS, 1, 4>();         // (at 128 columns that many registers are not there: 711 us, or 725 with spills)
                 const uint32_t w = (uint32_t)(bits >> (32 * h)) >> (4 * hh);
                 float d[16];
 #pragma unroll
@@ -673,6 +692,7 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(Args a) {
 #pragma unroll
                     for (int q = 0; q < OT; ++q) acc[q] = XA_MFMA(T::tr_frag(KT, 32 * h + 16 * k, q), dk, acc[q]);
                 }
+                if (DT <= 96) reads_ahead<2 * OT, 2, 2>();
             }
         }
         if (t + 1 < t1) {
@@ -798,6 +818,7 @@ __global__ __launch_bounds__(64 * W, DT > 64 ? 2 : 3) void xattn_dkdv_kernel(Arg
                 s = XA_MFMA(lds_16(Q ^ 32 * k), kf[k], s);
                 p = XA_MFMA(lds_16(O ^ 32 * k), V_IN_LDS ? lds_16(Vw ^ 32 * k) : vf[k], p);
             }
+            reads_ahead<2 * KS, V_IN_LDS ? 2 : 1, 2>();
             float e[16], d[16];
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
@@ -819,6 +840,7 @@ __global__ __launch_bounds__(64 * W, DT > 64 ? 2 : 3) void xattn_dkdv_kernel(Arg
                     dk[q] = XA_MFMA(T::tr_frag(qt, 16 * k, q), db, dk[q]);
                 }
             }
+            reads_ahead<4 * OT, 2, 2>();
         }
         }
         if (t + 1 < t1) store(cur ^ 1);
@@ -1041,6 +1063,7 @@ __global__ __launch_bounds__(64 * W, DT > 64 ? 2 : 3) void xattn_bwd_kernel(Args
                 s = XA_MFMA(lds_16(Q ^ 32 * k), lds_16(Kw ^ 32 * k), s);
                 p = XA_MFMA(lds_16(O ^ 32 * k), V_IN_LDS ? lds_16(Vw ^ 32 * k) : vf[k], p);
             }
+            reads_ahead<2 * KS, 2, 2>();
             float e[16], d[16];
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
@@ -1063,6 +1086,7 @@ __global__ __launch_bounds__(64 * W, DT > 64 ? 2 : 3) void xattn_bwd_kernel(Args
                     dk[q] = XA_MFMA(T::tr_frag(qt, 16 * k, q), __builtin_bit_cast(bf16x8, db), dk[q]);
                 }
             }
+            reads_ahead<4 * OT, 2, 2>();
         }
         if (SB == 1) {
             __syncthreads();
