@@ -20,6 +20,7 @@
 #include "../../include/xq_ops.h"
 #include <algorithm>
 #include <math.h>
+#include <type_traits>
 
 using namespace xq;
 
@@ -175,6 +176,17 @@ struct KeyBits {
 __device__ __forceinline__ uint4 zero_unless(uint4 v, bool ok) {
     if (!ok) v = make_uint4(0u, 0u, 0u, 0u);
     return v;
+}
+
+// the sum over aligned groups of N = 4, 8 or 16 lanes, in each of them (lane permutations of the vector unit: through LDS each step would wait for it)
+template <int N>
+__device__ __forceinline__ float sum_of_lanes(float x) {
+    auto moved = [](float y, auto control) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(y), decltype(control)::value, 0xf, 0xf, true)); };
+    x += moved(x, std::integral_constant<int, 0xB1>());                     // lanes 1 0 3 2 of four
+    x += moved(x, std::integral_constant<int, 0x4E>());                     // lanes 2 3 0 1
+    if (N >= 8) x += moved(x, std::integral_constant<int, 0x141>());        // lanes 7 .. 0 of eight
+    if (N >= 16) x += moved(x, std::integral_constant<int, 0x140>());       // lanes 15 .. 0 of sixteen
+    return x;
 }
 
 // 16 bytes at a byte offset of up to 2^31 behind a wave-uniform base; FAR reads zeros (a buffer's bounds check), so that what is masked or behind the head
@@ -760,6 +772,7 @@ __global__ __launch_bounds__(64 * W, DT > 64 ? 2 : 3) void xattn_dkdv_kernel(Arg
     Stage<DT, QT, 64 * W> sq, so;
     const long on = (long)a.H * a.D, oh = a.D;
     float rl = 0.0f;
+    int rows = 0;
     auto places = [&](int g0) {
 #pragma unroll
         for (int ch = 0; ch < sq.CH; ++ch) {
@@ -778,15 +791,16 @@ __global__ __launch_bounds__(64 * W, DT > 64 ? 2 : 3) void xattn_dkdv_kernel(Arg
         sq.load(a.q.p + b * a.q.sb + tok0 * a.q.sn + (long)hk * a.G * a.q.sh, bits);
         so.load(a.dout + ((long)b * a.Nq + tok0) * on + (long)hk * a.G * oh, bits);
         if (tid < 2 * QT) {
-            const int r = r0 + tid % QT;
-            rl = r < a.R ? (tid < QT ? log2_of(lse[r]) * lse_factor : BEGIN ? -dlt[r] : dlt[r]) : 0.0f;
+            const int r = min(r0 + tid % QT, a.R - 1);
+            rl = tid < QT ? lse[r] : dlt[r];              // (what is made of it waits for it: in store)
         }
+        rows = left;
     };
     auto store = [&](int buf) {
         sq.store(Qs + buf * BYTES);
         so.store(Os + buf * BYTES);
-        if (tid < QT) Ls[buf][tid] = rl;
-        else if (tid < 2 * QT) Ds[buf][tid - QT] = rl;
+        if (tid < QT) Ls[buf][tid] = tid < rows ? log2_of(rl) * lse_factor : 0.0f;
+        else if (tid < 2 * QT) Ds[buf][tid - QT] = tid - QT >= rows ? 0.0f : BEGIN ? -rl : rl;
     };
 
     int t0, t1;
@@ -868,7 +882,7 @@ __global__ __launch_bounds__(64 * W, DT > 64 ? 2 : 3) void xattn_dkdv_kernel(Arg
 // ---------------------------------------------------------------------------------------------------------------------------------------------
 // the whole backward of a (sample, kv head) whose keys fit one block (up to 32 W of them): one key per lane as in the dk / dv kernel; dS also goes to LDS
 // (key-major), and the waves share out dq = dS k of the tile before.  q, dO and out are read once, P and dP computed once: five products instead of seven.
-// 128 x 256 rows x 257 keys x 12 heads of 64 (nine waves): 165 us, 2.4 TB/s of its 400 MB and 390 TFLOP/s.  Bound by latency: the vector units and LDS are busy 32 % of
+// 128 x 256 rows x 257 keys x 12 heads of 64 (nine waves): 158 us, 2.5 TB/s of its 400 MB and 410 TFLOP/s.  Bound by latency: the vector units and LDS are busy 32 % of
 // the cycles each, the matrix pipe 20 %, and the waves wait half of theirs (a CU holds one such block: nothing runs beside its first loads and last stores).
 // ---------------------------------------------------------------------------------------------------------------------------------------------
 template <int DT, int W, bool SPLIT>
@@ -936,6 +950,7 @@ __global__ __launch_bounds__(64 * W, DT > 64 ? 2 : 3) void xattn_bwd_kernel(Args
     uint32_t off_q[CH], off_o[CH];
     uint4 rq[CH], rd[CH], ro[CH];
     float rl = 0.0f;
+    int rows = 0;
     auto row_of = [&](int ch) { return (ROLES ? tid % CHUNKS : tid + 64 * W * ch) / PR; };
     auto chunk_of = [&](int ch) { return (ROLES ? tid % CHUNKS : tid + 64 * W * ch) % PR; };
     // row r0 + i of a tile: token (r0 + i) / G.  Where G divides QT its offset from the tile's first token is the same in every tile
@@ -967,7 +982,8 @@ __global__ __launch_bounds__(64 * W, DT > 64 ? 2 : 3) void xattn_bwd_kernel(Args
             for (int ch = 0; ch < CH; ++ch)
                 rq[ch] = load16(a.q.p + b * a.q.sb + tok0 * a.q.sn + (long)hk * a.G * a.q.sh, row_of(ch) < left ? off_q[ch] : FAR);
         }
-        if (tid < QT) rl = tid < left ? log2_of(lse[r0 + tid]) * lse_factor : 0.0f;
+        if (tid < QT) rl = lse[tid < left ? r0 + tid : r0];            // (what is made of it waits for it: in store)
+        rows = left;
     };
     auto store = [&](int buf) {
         if (role == 0) {
@@ -979,8 +995,7 @@ __global__ __launch_bounds__(64 * W, DT > 64 ? 2 : 3) void xattn_bwd_kernel(Args
                 s = fmaf(bf_lo(x.y), bf_lo(y.y), s); s = fmaf(bf_hi(x.y), bf_hi(y.y), s);
                 s = fmaf(bf_lo(x.z), bf_lo(y.z), s); s = fmaf(bf_hi(x.z), bf_hi(y.z), s);
                 s = fmaf(bf_lo(x.w), bf_lo(y.w), s); s = fmaf(bf_hi(x.w), bf_hi(y.w), s);
-#pragma unroll
-                for (int o = 1; o < PR; o <<= 1) s += __shfl_xor(s, o);
+                s = sum_of_lanes<PR>(s);
                 if (chunk_of(ch) == 0) Ds[buf][row_of(ch)] = -s;
                 *(lds_ptr<u32x4>)(uintptr_t)(Os + buf * BYTES + T::place(row_of(ch), chunk_of(ch))) = __builtin_bit_cast(u32x4, x);
             }
@@ -990,7 +1005,7 @@ __global__ __launch_bounds__(64 * W, DT > 64 ? 2 : 3) void xattn_bwd_kernel(Args
             for (int ch = 0; ch < CH; ++ch)
                 *(lds_ptr<u32x4>)(uintptr_t)(Qs + buf * BYTES + T::place(row_of(ch), chunk_of(ch))) = __builtin_bit_cast(u32x4, rq[ch]);
         }
-        if (tid < QT) Ls[buf][tid] = rl;
+        if (tid < QT) Ls[buf][tid] = tid < rows ? log2_of(rl) * lse_factor : 0.0f;
     };
 
     const int unit = wave - FIRST;
@@ -1181,11 +1196,11 @@ Sizes sizes_of(int B, int Nq, int Nk, int H, int Hk, int D) {
     z.fwd_bytes = z.fwd_splits > 1 ? z.fwd_part + rows * z.fwd_splits * 8 : 0;
     z.delta_bytes = align_up(rows * 4, 256);
     // one block for all keys of a (sample, kv head): nine waves fit a CU's LDS and registers up to 64 columns.  Against the two kernels: 128 x 256 rows x 257
-    // keys x 12 heads of 64 165 us instead of 203, 128 keys 77 instead of 101, 16 x 500 x 200 x 8 35 instead of 45, 24 x 286 x 93 x 16 heads of 96 over 4 46
-    // instead of 60; 64 x 256 x 77 x 16 heads of 128 124 instead of 142, 32 x 256 x 77 x 8 heads of 128 45 as before
+    // keys x 12 heads of 64 158 us instead of 203, 128 keys 69 instead of 101, 16 x 500 x 200 x 8 35 instead of 45, 24 x 286 x 93 x 16 heads of 96 over 4 42
+    // instead of 60; 64 x 256 x 77 x 16 heads of 128 111 instead of 142, 32 x 256 x 77 x 8 heads of 128 40 instead of 45
     z.one_waves = Nk < 1 || Nq < 1 ? 0 : Nk <= 128 ? 4 : D <= 64 && Nk <= 288 ? 9 : 0;
     if (z.one_waves) {
-        // shares of the rows no more than the blocks that two a CU hold (a few over that wait for a second round: 46 us, or 58), of eight tiles at least
+        // shares of the rows no more than the blocks that two a CU hold (a few over that wait for a second round: at 24 x 286 x 93 58 us instead of 46), of eight tiles at least
         z.kv_splits = (int)std::max<long>(1, std::min(tiles_of(z.R, 32) / 8, 2L * num_cus() / std::max<long>(1, z.groups)));
         z.delta_bytes = 0;
         z.dq_splits = 1;
