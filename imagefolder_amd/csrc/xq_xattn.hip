@@ -424,7 +424,7 @@ __global__ __launch_bounds__(256, 2) void xattn_fwd_kernel(Args a) {
 // ---------------------------------------------------------------------------------------------------------------------------------------------
 // forward of at most 32 rows a kv head over at most 1024 keys (serving: one token, its heads, one image's or text's states): the four waves share out the keys,
 // each with its own 32-key tiles and no meeting with the others until their results are joined.  K and V go through LDS tiles of the wave's own (loads of whole
-// rows), fetched a tile ahead.  Bound by latency: one token over 257 keys, 12 heads of 64, takes 6.9 us (in the tiles of the many-row kernel, where one
+// rows), fetched a tile ahead.  Bound by latency: one token over 257 keys, 12 heads of 64, takes 6.0 us (in the tiles of the many-row kernel, where one
 // wave of four has rows, 8.8).  Over more keys the many-row kernel with its keys split over blocks reads as fast (16 samples over 4056 .. 8111 keys: 82 us, here
 // 84) and a block's share is no longer one wave's chain.
 // ---------------------------------------------------------------------------------------------------------------------------------------------
@@ -437,7 +437,8 @@ __global__ __launch_bounds__(256, 2) void xattn_few_rows_kernel(Args a) {
     __shared__ float2 stat[4][32];
     const int g = blockIdx.x;
     const int b = g / a.Hk, hk = g - b * a.Hk;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 31, hh = lane >> 5;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 31,
+              hh = lane >> 5;          // (the wave's number is the same in its lanes: the buffers' bases lie in scalar registers, 6.9 -> 6.0 us)
     const uint32_t Kw = lds_address(mem) + 2 * wave * BYTES, Vw = Kw + BYTES, row_at = Kw + T::row_base(li, hh), tr_at = Vw + T::tr_base(lane);
     const int len = keys_of(a, b);
     const short *kb = a.k.p + b * a.k.sb + hk * a.k.sh, *vb = a.v.p + b * a.v.sb + hk * a.v.sh;
@@ -582,6 +583,7 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(Args a, int per_row, un
     const int col = ((uint32_t)id - row * per_row) * 4;
     const long rows = (long)a.groups * a.R;
     float M = -INFINITY;
+#pragma unroll 8
     for (int s = 0; s < a.splits; ++s) M = fmaxf(M, a.stat[2 * (s * rows + row)]);
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     float l = 0.0f;
