@@ -104,15 +104,12 @@ struct Tile {
     }
 };
 
-// v_max3_f32 without the operand canonicalisation that fmaxf() carries under IEEE mode
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float d;
-    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
-    return d;
-}
+// The largest of three, NaN if one is (v_maximum3_f32; fmaxf would make every operand canonical first).  Not inline asm: the wait that a matrix instruction's
+// result needs before it is read is the compiler's, and it does not see into asm.
+__device__ __forceinline__ float max3(float a, float b, float c) { return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c); }
 
 // Order for the scheduler: N matrix instructions with PER LDS reads each, the reads AHEAD of them (left to itself it puts every read right before its use, and
-// the wave waits for LDS once a product: dk / dv 1110 us at 4 x 4096 x 4352 x 16 x 128, so 1087; dq 197 us at 8 x 2048 x 2048 x 12 x 64, so 192)
+// the wave waits for LDS once a product: dk / dv at 4 x 4096 x 4352 x 16 x 128 1110 us instead of 1087, dq at 8 x 2048 x 2048 x 12 x 64 197 instead of 192)
 template <int N, int PER, int AHEAD>
 __device__ __forceinline__ void reads_ahead() {
     __builtin_amdgcn_sched_group_barrier(0x100, PER * AHEAD, 0);
@@ -124,7 +121,7 @@ __device__ __forceinline__ void reads_ahead() {
     __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
 }
 
-// the larger of a lane's value and its partner's in the other half of the wave (through LDS the tile waits for it: 525 us, so 510)
+// the larger of a lane's value and its partner's in the other half of the wave (through LDS the tile waits for it: 525 us instead of 510)
 __device__ __forceinline__ float max_of_halves(float x) {
     const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return max3(__uint_as_float(both[0]), __uint_as_float(both[1]), x);
@@ -350,7 +347,7 @@ __global__ __launch_bounds__(256, 2) void xattn_fwd_kernel(Args a) {
             __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                s[h] = zero16;                             // (the second half also where none of its keys is valid: the choice would copy both halves at every tile: 545 us, so 525)
+                s[h] = zero16;                             // (the second half also where none of its keys is valid: the choice would copy both halves at every tile: 545 us instead of 525)
 #pragma unroll
                 for (int k = 0; k < KS; ++k) s[h] = XA_MFMA(lds_16((K ^ 32 * k) + 32 * h * T::ROW), qf[k], s[h]);
             }
@@ -438,7 +435,7 @@ __global__ __launch_bounds__(256, 2) void xattn_few_rows_kernel(Args a) {
     const int g = blockIdx.x;
     const int b = g / a.Hk, hk = g - b * a.Hk;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 31,
-              hh = lane >> 5;          // (the wave's number is the same in its lanes: the buffers' bases lie in scalar registers, 6.9 -> 6.0 us)
+              hh = lane >> 5;          // (the wave's number is the same in its lanes: the buffers' bases lie in scalar registers: 6.0 us instead of 6.9)
     const uint32_t Kw = lds_address(mem) + 2 * wave * BYTES, Vw = Kw + BYTES, row_at = Kw + T::row_base(li, hh), tr_at = Vw + T::tr_base(lane);
     const int len = keys_of(a, b);
     const short *kb = a.k.p + b * a.k.sb + hk * a.k.sh, *vb = a.v.p + b * a.v.sb + hk * a.v.sh;
@@ -690,7 +687,7 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(Args a) {
                     s = XA_MFMA(lds_16((K ^ 32 * k) + 32 * h * T::ROW), qf[k], s);
                     p = XA_MFMA(lds_16((V ^ 32 * k) + 32 * h * T::ROW), df[k], p);
                 }
-                if (DT <= 96) reads_ahead<2 * KS, 1, 4>();         // (at 128 columns that many registers are not there: 711 us, or 725 with spills)
+                if (DT <= 96) reads_ahead<2 * KS, 1, 4>();         // (at 128 columns that many registers are not there: 725 us instead of 711)
                 const uint32_t w = (uint32_t)(bits >> (32 * h)) >> (4 * hh);
                 float d[16];
 #pragma unroll
