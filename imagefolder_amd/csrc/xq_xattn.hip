@@ -890,6 +890,9 @@ __global__ __launch_bounds__(64 * W, DT > 64 ? 2 : 3) void xattn_bwd_kernel(Args
     typedef Tile<32> TS;
     constexpr int QT = 32, KS = DT / 16, OT = DT / 32, BYTES = QT * T::ROW, SBYTES = 32 * W * TS::ROW;
     constexpr int SB = DT > 64 ? 1 : 2;                     // buffers of dS: with one, a second meeting a tile, but two blocks a CU
+    // at 128 columns the next tile is fetched when the scores are done with: beside them there are no registers for it (8 x 1024 x 128 keys x 32 heads over 8: 124 us
+    // instead of 107; q in one step with the others 109)
+    constexpr bool LATE = DT > 96;
     constexpr bool V_IN_LDS = W == 9;                       // (with four waves a block fewer blocks would fit a CU)
     // dq: NA x NB tiles of 16 columns x 16 rows a wave
     constexpr int NA = W == 4 ? (DT == 96 ? 3 : DT == 128 ? 2 : 1) : 1, NB = W == 4 && (DT == 64 || DT == 128) ? 2 : 1, FIRST = W == 4 ? 0 : 1;
@@ -964,6 +967,14 @@ __global__ __launch_bounds__(64 * W, DT > 64 ? 2 : 3) void xattn_bwd_kernel(Args
     };
     const bool same_places = QT % a.G == 0;
     places(0);
+    auto load_q = [&](int r0) {
+        const int tok0 = (int)quotient((uint32_t)r0, a.g_reciprocal), left = a.R - r0;
+        if (!ROLES || role == 1) {
+#pragma unroll
+            for (int ch = 0; ch < CH; ++ch)
+                rq[ch] = load16(a.q.p + b * a.q.sb + tok0 * a.q.sn + (long)hk * a.G * a.q.sh, row_of(ch) < left ? off_q[ch] : FAR);
+        }
+    };
     auto load = [&](int r0) {
         const int tok0 = (int)quotient((uint32_t)r0, a.g_reciprocal), left = a.R - r0;
         if (!same_places) places(r0 - tok0 * a.G);
@@ -976,11 +987,7 @@ __global__ __launch_bounds__(64 * W, DT > 64 ? 2 : 3) void xattn_bwd_kernel(Args
                 ro[ch] = load16(a.out_in + o, at);
             }
         }
-        if (!ROLES || role == 1) {
-#pragma unroll
-            for (int ch = 0; ch < CH; ++ch)
-                rq[ch] = load16(a.q.p + b * a.q.sb + tok0 * a.q.sn + (long)hk * a.G * a.q.sh, row_of(ch) < left ? off_q[ch] : FAR);
-        }
+        if (!LATE) load_q(r0);
         if (tid < QT) rl = lse[tid < left ? r0 + tid : r0];            // (what is made of it waits for it: in store)
         rows = left;
     };
@@ -1046,6 +1053,7 @@ __global__ __launch_bounds__(64 * W, DT > 64 ? 2 : 3) void xattn_bwd_kernel(Args
     int t0, t1;
     share((a.R + QT - 1) / QT, split, SPLIT ? a.splits : 1, t0, t1);
     if (t0 < t1) load(t0 * QT);
+    if (LATE && t0 < t1) load_q(t0 * QT);
     const uint32_t Kw = Kb + wave * 32 * T::ROW + row_at, Vw = Vb + wave * 32 * T::ROW + row_at;
     // every key's row, zeros for one that is not valid: what dq adds of its k is 0 x 0
 #pragma unroll
@@ -1059,7 +1067,7 @@ __global__ __launch_bounds__(64 * W, DT > 64 ? 2 : 3) void xattn_bwd_kernel(Args
     __syncthreads();
     for (int t = t0; t < t1; ++t) {
         const int cur = (t - t0) & 1;
-        if (t + 1 < t1) load(t * QT + QT);
+        if (t + 1 < t1 && !LATE) load(t * QT + QT);
         if (SB == 2 && t > t0) dq_tile(t - 1, Sb + (cur ^ 1) * SBYTES);
         if (wave_live) {
             const uint32_t Qh = Qs + cur * BYTES, Oh = Os + cur * BYTES, Q = Qh + row_at, O = Oh + row_at;
@@ -1084,6 +1092,7 @@ __global__ __launch_bounds__(64 * W, DT > 64 ? 2 : 3) void xattn_bwd_kernel(Args
                 e[j] = __builtin_amdgcn_exp2f(s[j] * c);
                 d[j] = e[j] * p[j];
             }
+            if (LATE && t + 1 < t1) { load(t * QT + QT); load_q(t * QT + QT); }
             const uint32_t ot = Oh + tr_at, qt = Qh + tr_at;
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
@@ -1102,6 +1111,7 @@ __global__ __launch_bounds__(64 * W, DT > 64 ? 2 : 3) void xattn_bwd_kernel(Args
             }
             reads_ahead<4 * OT, 2, 2>();
         }
+        if (LATE && !wave_live && t + 1 < t1) { load(t * QT + QT); load_q(t * QT + QT); }
         if (SB == 1) {
             __syncthreads();
             dq_tile(t, Sb);
@@ -1196,7 +1206,7 @@ Sizes sizes_of(int B, int Nq, int Nk, int H, int Hk, int D) {
     z.delta_bytes = align_up(rows * 4, 256);
     // one block for all keys of a (sample, kv head): nine waves fit a CU's LDS and registers up to 64 columns.  Against the two kernels: 128 x 256 rows x 257
     // keys x 12 heads of 64 158 us instead of 203, 128 keys 69 instead of 101, 16 x 500 x 200 x 8 35 instead of 45, 24 x 286 x 93 x 16 heads of 96 over 4 42
-    // instead of 60; 64 x 256 x 77 x 16 heads of 128 111 instead of 142, 32 x 256 x 77 x 8 heads of 128 40 instead of 45
+    // instead of 60; 64 x 256 x 77 x 16 heads of 128 108 instead of 142, 32 x 256 x 77 x 8 heads of 128 39 instead of 45
     z.one_waves = Nk < 1 || Nq < 1 ? 0 : Nk <= 128 ? 4 : D <= 64 && Nk <= 288 ? 9 : 0;
     if (z.one_waves) {
         // shares of the rows no more than the blocks that two a CU hold (a few over that wait for a second round: at 24 x 286 x 93 58 us instead of 46), of eight tiles at least
