@@ -281,7 +281,9 @@ __device__ __forceinline__ void share(int n, int part, int parts, int &from, int
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------------------------
-// forward: 128 rows of one (sample, kv head) a block, 32 a wave; 64-key tiles of K and V in two LDS buffers
+// forward: 128 rows of one (sample, kv head) a block, 32 a wave; 64-key tiles of K and V in two LDS buffers.  4 x 4096 x <= 4352 keys x 16 heads of 128: 515 us,
+// 890 TFLOP/s, the matrix pipe busy 48 % of the cycles and the vector units 46 %; 128 x 256 x 257 x 12 heads of 64: 59 us, 3.4 TB/s, the vector units 60 %; one token
+// of 16 samples over 4056 .. 8111 keys, 32 heads over 8 of 128: 82 us, 4.9 TB/s (the keys split over four blocks)
 // ---------------------------------------------------------------------------------------------------------------------------------------------
 template <int DT, bool SPLIT>
 __global__ __launch_bounds__(256, 2) void xattn_fwd_kernel(Args a) {
@@ -601,7 +603,8 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(Args a, int per_row, un
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------------------------
-// dq: one row per lane as the forward; delta in the prologue, written for the dk / dv kernel behind it
+// dq: one row per lane as the forward; delta in the prologue, written for the dk / dv kernel behind it.  4 x 4096 x <= 4352 keys x 16 heads of 128: 720 us,
+// 950 TFLOP/s, the matrix pipe busy half of the cycles
 // ---------------------------------------------------------------------------------------------------------------------------------------------
 template <int DT, bool SPLIT>
 __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(Args a) {
@@ -722,7 +725,8 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(Args a) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------------------------
-// dk, dv: one key per lane, 32 W keys of one (sample, kv head) a block; tiles of QT rows of q and dO (and lse, delta) in two LDS buffers
+// dk, dv: one key per lane, 32 W keys of one (sample, kv head) a block; tiles of QT rows of q and dO (and lse, delta) in two LDS buffers.
+// 4 x 4096 x <= 4352 keys x 16 heads of 128: 1075 us, 850 TFLOP/s, the matrix pipe busy 43 % of the cycles: the waves (two a SIMD, their registers full) wait for LDS
 // ---------------------------------------------------------------------------------------------------------------------------------------------
 template <int DT, int W, bool SPLIT>
 __global__ __launch_bounds__(64 * W, DT > 64 ? 2 : 3) void xattn_dkdv_kernel(Args a) {
@@ -881,8 +885,9 @@ __global__ __launch_bounds__(64 * W, DT > 64 ? 2 : 3) void xattn_dkdv_kernel(Arg
 // ---------------------------------------------------------------------------------------------------------------------------------------------
 // the whole backward of a (sample, kv head) whose keys fit one block (up to 32 W of them): one key per lane as in the dk / dv kernel; dS also goes to LDS
 // (key-major), and the waves share out dq = dS k of the tile before.  q, dO and out are read once, P and dP computed once: five products instead of seven.
-// 128 x 256 rows x 257 keys x 12 heads of 64 (nine waves): 158 us, 2.5 TB/s of its 400 MB and 410 TFLOP/s.  Bound by latency: the vector units and LDS are busy 32 % of
-// the cycles each, the matrix pipe 20 %, and the waves wait half of theirs (a CU holds one such block: nothing runs beside its first loads and last stores).
+// 128 x 256 rows x 257 keys x 12 heads of 64 (nine waves): 158 us, 2.5 TB/s of its 400 MB and 410 TFLOP/s.  Bound by latency: the vector units and LDS are busy 33 % of
+// the cycles each, the matrix pipe 22 %, and the waves wait half of theirs (a CU holds one such block: nothing runs beside its first loads and last stores,
+// 50 us of it).
 // ---------------------------------------------------------------------------------------------------------------------------------------------
 template <int DT, int W, bool SPLIT>
 __global__ __launch_bounds__(64 * W, DT > 64 ? 2 : 3) void xattn_bwd_kernel(Args a) {
