@@ -332,6 +332,72 @@ def test_in_graphs_and_on_another_stream(Nq, Nk):
 
 
 @gpu
+def test_two_streams_at_once():
+    from imagefolder_amd import nn_ops
+    sizes = ((4, 300, 500, 8, 2, 64), (2, 900, 100, 8, 8, 128), (3, 64, 257, 12, 12, 64), (2, 1, 5000, 16, 4, 128))
+    for size in sizes:
+        B, Nq, Nk, H, Hk, D = size
+        jobs = [tuple(torch.randn(B, n, h, D, device="cuda").to(BF).requires_grad_(True) for n, h in ((Nq, H), (Nk, Hk), (Nk, Hk))) for _ in range(2)]
+        g = torch.randn(B, Nq, H, D, device="cuda").to(BF)
+
+        def step(job):
+            y = nn_ops.cross_attention(*job)
+            return (y.detach(),) + torch.autograd.grad(y, job, g)
+
+        want = [step(j) for j in jobs]
+        streams = [torch.cuda.Stream() for _ in jobs]
+        torch.cuda.synchronize()
+        got = [[], []]
+        for _ in range(4):
+            for i, st in enumerate(streams):
+                with torch.cuda.stream(st):
+                    got[i].append(step(jobs[i]))
+        torch.cuda.synchronize()
+        for w, runs in zip(want, got):
+            assert all(torch.equal(a, b) for r in runs for a, b in zip(w, r))
+
+
+@gpu
+def test_some_of_the_gradients_and_views_of_lengths_and_masks():
+    from imagefolder_amd import nn_ops
+    torch.manual_seed(9)
+    B, Nq, Nk, H, D = 3, 40, 90, 2, 64
+    q, k, v, g = (torch.randn(B, n, H, D, device="cuda").to(BF) for n in (Nq, Nk, Nk, Nq))
+    lens = torch.tensor([90, 5, 7, 5, 33, 5], device="cuda", dtype=torch.int32)[::2]
+    mask = (torch.rand(1, Nk, device="cuda") < 0.7).expand(B, Nk)
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    want = torch.autograd.grad(nn_ops.cross_attention(*leaves, kv_lens=lens.contiguous(), key_mask=mask.contiguous()), leaves, g)
+    for i in range(3):
+        args = [t.clone().requires_grad_(i == j) for j, t in enumerate((q, k, v))]
+        (d,) = torch.autograd.grad(nn_ops.cross_attention(*args, kv_lens=lens, key_mask=mask), (args[i],), g)
+        assert torch.equal(d, want[i])
+    one = q.clone().requires_grad_(True)            # one tensor in all three places: its gradients add up
+    y = nn_ops.cross_attention(one, one, one)
+    parts = [t.clone().requires_grad_(True) for t in (q, q, q)]
+    z = nn_ops.cross_attention(*parts)
+    (d,) = torch.autograd.grad(y, (one,), g)
+    a, b, c = (t.double() for t in torch.autograd.grad(z, parts, g))
+    # two additions in bf16, in whatever order: each rounds at most half a step of a sum that is at most the sum of the parts' sizes
+    assert torch.equal(y, z) and bool(((d.double() - (a + b + c)).abs() <= 2.05 * HALF * (a.abs() + b.abs() + c.abs())).all())
+
+
+@gpu
+@pytest.mark.parametrize("Nq", [1, 33])
+def test_more_samples_than_a_grid_dimension_of_16_bits(Nq):
+    B, Nk, D = 70001, 3, 8
+    gen = torch.Generator(device="cuda").manual_seed(Nq)
+    q, k, v, g = (torch.randn(B, n, 1, D, generator=gen, device="cuda").to(BF).requires_grad_(True) for n in (Nq, Nk, Nk, Nq))
+    from imagefolder_amd import nn_ops
+    y = nn_ops.cross_attention(q, k, v)
+    grads = torch.autograd.grad(y, (q, k, v), g.detach())
+    for b in (0, 1, 65535, 65536, 70000):
+        part = [t.detach()[b:b + 1] for t in (q, k, v, g)]
+        want, tol = oracle(*part)
+        for name, a, w, t in zip(("O", "dq", "dk", "dv"), (y.detach(),) + grads, want, tol):
+            within(name, a[b:b + 1], w, t)
+
+
+@gpu
 @pytest.mark.parametrize("N,H,D", [(257, 3, 32), (130, 2, 128), (65, 4, 96), (50, 2, 8)])
 def test_packed_self_attention_of_other_head_widths(N, H, D):
     """nn_ops.attention_qkvpacked and its twin of the fused blocks take head widths other than 64 through these kernels"""

@@ -569,3 +569,31 @@ def test_second_derivatives_are_refused():
         assert torch.equal(plain, again.detach())
         with pytest.raises(RuntimeError, match="twice"):
             again.float().sum().backward()
+
+
+@gpu
+def test_embedding_and_dropout_on_two_streams_at_once():
+    from imagefolder_amd import nn_ops
+    jobs = []
+    for seed in range(2):
+        gen = torch.Generator(device="cuda").manual_seed(seed)
+        idx = torch.randint(0, 5000, (20000,), generator=gen, device="cuda")
+        idx[::3] = 7 + seed                       # a frequent row: its pieces meet in the workspace
+        jobs.append((torch.randn(5000, 64, generator=gen, device="cuda").requires_grad_(True), idx, torch.randn(20000, 64, generator=gen, device="cuda"),
+                     torch.tensor([seed, 5], device="cuda")))
+
+    def step(w, idx, g, key):
+        y = nn_ops.dropout(nn_ops.embedding(idx, w), 0.3, key=key)
+        return (y.detach(),) + torch.autograd.grad(y, (w,), g)
+
+    want = [step(*j) for j in jobs]
+    streams = [torch.cuda.Stream() for _ in jobs]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(step(*jobs[i]))
+    torch.cuda.synchronize()
+    for w, runs in zip(want, got):
+        assert all(torch.equal(a, b) for r in runs for a, b in zip(w, r))
