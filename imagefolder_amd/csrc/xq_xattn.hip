@@ -494,6 +494,7 @@ __global__ __launch_bounds__(256, 2) void xattn_few_rows_kernel(Args a) {
             *(lds_ptr<u32x4>)(uintptr_t)(Kw + at) = __builtin_bit_cast(u32x4, kr[i]);
             *(lds_ptr<u32x4>)(uintptr_t)(Vw + at) = __builtin_bit_cast(u32x4, vr[i]);
         }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");       // the lanes read what other lanes of the wave have written (in order for the hardware, not for the compiler)
         if (t + 4 < t1) {
             next = (uint32_t)keys.take(t * 32 + 128);
             load(t + 4, next);
@@ -536,6 +537,7 @@ __global__ __launch_bounds__(256, 2) void xattn_few_rows_kernel(Args a) {
 #pragma unroll
             for (int q = 0; q < OT; ++q) o[q] = XA_MFMA(T::tr_frag(tr_at, 16 * k, q), pk, o[q]);
         }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         bits = next;
     }
     l += __shfl_xor(l, 32);
