@@ -77,6 +77,8 @@ __device__ __forceinline__ uint4 load16_or_zero(const short *p, bool ok) {
 }
 
 // v_max3_f32 without the operand canonicalisation that fmaxf() carries under IEEE mode (57 -> 16 instructions per tile)
+// (the compiler places no wait in front of asm that reads a matrix instruction's result: 17 states lie between the two here, where it keeps 12 for its own
+// instructions; what moves code between them has to keep that, or take __builtin_elementwise_maximum as xq_xattn.hip does)
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
     asm("v_max3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
