@@ -143,9 +143,9 @@ __device__ __forceinline__ void tile_counts(const uint32_t *seen, int pitch, int
     __syncthreads();
 }
 
-// base: where each digit's next item goes -> seen[wave][digit]: where the wave's first one goes; base moves on behind the tile
+// base: where each digit's first item goes -> seen[wave][digit]: where the wave's first one goes
 template <int WAVES>
-__device__ __forceinline__ void tile_places(uint32_t *seen, int pitch, int digits, uint32_t *base) {
+__device__ __forceinline__ void tile_places(uint32_t *seen, int pitch, int digits, const uint32_t *base) {
     for (int i = threadIdx.x; i < digits; i += WAVES * 64) {
         uint32_t b = base[i];
 #pragma unroll
@@ -154,7 +154,6 @@ __device__ __forceinline__ void tile_places(uint32_t *seen, int pitch, int digit
             seen[w * pitch + i] = b;
             b += c;
         }
-        base[i] = b;
     }
     __syncthreads();
 }
