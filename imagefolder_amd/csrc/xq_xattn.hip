@@ -13,7 +13,7 @@
 // V^T comes from the row-major LDS tile through ds_read_b64_tr_b16), the dk / dv kernel one key per lane.
 // Masked keys are zero rows in LDS and -inf in S: what lies in memory there (infinities, NaN) reaches nothing.
 // Roundings to bf16: P and dS before their products (they are operands of the bf16 matrix instructions; fp16 would not hold the range of the other operand, two
-// bf16 parts would double the products), the results once; everything else is fp32.  Against 64 bits the results are 0.0021 .. 0.0027 off in norm (rounding them
+// bf16 parts would double the products), the results once; everything else is fp32.  Against 64 bits the results are 0.0021 .. 0.0029 off in norm (rounding them
 // alone: 0.0017, the operand's rounding as much again in squares, and for dq / dk what delta takes from the rounded O).
 #include "xq_common.hpp"
 #include "xq_internal.hpp"

@@ -35,7 +35,11 @@ def _at(t):
 
 def _wants_grad(*tensors):
     """whether autograd has to see the call (an autograd node costs a small call as much as its kernel)"""
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _same_device(name, first, *others):
@@ -290,27 +294,34 @@ def packed_attention_supported(qkv, num_heads):
     return qkv.is_cuda and qkv.dtype == torch.bfloat16 and qkv.dim() == 3 and qkv.shape[-1] == 3 * num_heads * D and D % 8 == 0 and 8 <= D <= 128
 
 
-def check_cross_attention(q, k, v, kv_lens, key_mask, scale):
-    """shapes and types, on whatever device -> the scale"""
+@functools.lru_cache(maxsize=4096)
+def _check_shapes(q, k, v, lens, mask, scale):
+    """by shapes and types alone (lens, mask: (shape, type) or None) -> the scale"""
     for name, t in (("q", q), ("k", k), ("v", v)):
-        if t.dim() != 4:
-            raise XqError(f"cross_attention: {name} is (batch, tokens, heads, head dim) (got shape {tuple(t.shape)})")
-    B, Nq, H, D = q.shape
-    Nk, Hk = k.shape[1], k.shape[2]
-    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
-        raise XqError(f"cross_attention: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not go together")
+        if len(t) != 4:
+            raise XqError(f"cross_attention: {name} is (batch, tokens, heads, head dim) (got shape {tuple(t)})")
+    B, Nq, H, D = q
+    Nk, Hk = k[1], k[2]
+    if k != v or k[0] != B or k[3] != D:
+        raise XqError(f"cross_attention: q {tuple(q)}, k {tuple(k)} and v {tuple(v)} do not go together")
     if H < 1 or Hk < 1 or H % Hk:
         raise XqError(f"cross_attention: {H} query heads do not share {Hk} key / value heads evenly")
     if D < 1:
         raise XqError("cross_attention: a head dim of 0")
-    if kv_lens is not None and (tuple(kv_lens.shape) != (B,) or kv_lens.dtype not in (torch.int32, torch.int64)):
-        raise XqError(f"cross_attention: kv_lens is an int32 or int64 tensor of {B} lengths (got {kv_lens.dtype}, shape {tuple(kv_lens.shape)})")
-    if key_mask is not None and (tuple(key_mask.shape) != (B, Nk) or key_mask.dtype != torch.bool):
-        raise XqError(f"cross_attention: key_mask is a bool tensor of shape {(B, Nk)} (got {key_mask.dtype}, shape {tuple(key_mask.shape)})")
-    scale = float(D) ** -0.5 if scale is None else float(scale)
+    if lens is not None and (tuple(lens[0]) != (B,) or lens[1] not in (torch.int32, torch.int64)):
+        raise XqError(f"cross_attention: kv_lens is an int32 or int64 tensor of {B} lengths (got {lens[1]}, shape {tuple(lens[0])})")
+    if mask is not None and (tuple(mask[0]) != (B, Nk) or mask[1] != torch.bool):
+        raise XqError(f"cross_attention: key_mask is a bool tensor of shape {(B, Nk)} (got {mask[1]}, shape {tuple(mask[0])})")
+    scale = float(D) ** -0.5 if scale is None else scale
     if not 2.0 ** -64 <= scale <= 2.0 ** 64:
         raise XqError(f"cross_attention: scale = {scale} is not positive, 2^-64 .. 2^64")
     return scale
+
+
+def check_cross_attention(q, k, v, kv_lens, key_mask, scale):
+    """shapes and types, on whatever device -> the scale"""
+    return _check_shapes(q.shape, k.shape, v.shape, None if kv_lens is None else (kv_lens.shape, kv_lens.dtype),
+                         None if key_mask is None else (key_mask.shape, key_mask.dtype), None if scale is None else float(scale))
 
 
 def cross_attention(q, k, v, kv_lens=None, key_mask=None, scale=None):

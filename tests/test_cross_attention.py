@@ -494,6 +494,12 @@ def test_refusals():
                      (dict(kv_lens=torch.zeros(2, dtype=torch.int32, device="meta")), "one device")):
         with pytest.raises(XqError, match=what):
             ops_seq.cross_attention(**{**good, **kw})
+    # a scale held in a tensor is read at every call
+    t = torch.tensor(0.5)
+    assert ops_seq.check_cross_attention(**good, kv_lens=None, key_mask=None, scale=t) == 0.5
+    t.fill_(0.25)
+    assert ops_seq.check_cross_attention(**good, kv_lens=None, key_mask=None, scale=t) == 0.25
+    t = lambda *s, dt=BF: torch.zeros(*s, dtype=dt)  # noqa: E731
     for D in (12, 136, 0):
         with pytest.raises(XqError, match="head dim"):
             ops_seq.cross_attention(t(2, 3, 4, D), t(2, 5, 2, D), t(2, 5, 2, D))
