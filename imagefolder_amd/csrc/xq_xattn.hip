@@ -1182,10 +1182,11 @@ unsigned long long reciprocal_of(long d) { return d <= 1 ? 0 : ~0ull / (unsigned
 // blocks of `tile` rows (or keys) for each (sample, kv head)
 long tiles_of(long n, int tile) { return (n + tile - 1) / tile; }
 
-// shares of the contracted axis (`steps` tiles long) so that about two blocks run on every CU; a share has at least `least` tiles
+// shares of the contracted axis (`steps` tiles long) so that about two blocks run on every CU; a share has at least `least` tiles.  No blocks (an empty batch, no
+// queries or no keys): one share
 int splits_for(long blocks, long steps, int least) {
     const long want = 2L * num_cus();
-    if (blocks >= want || steps < 2 * least) return 1;
+    if (blocks < 1 || blocks >= want || steps < 2 * least) return 1;
     return (int)std::max<long>(1, std::min(steps / least, (want + blocks - 1) / blocks));
 }
 

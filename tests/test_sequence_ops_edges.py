@@ -1,0 +1,48 @@
+"""Calls at the edges of what nn_ops.cross_attention, dropout, embedding and the packed attention of other head widths take: empty ones, sizes past the kernels' limits,
+transforms of autograd other than reverse mode, modules with hooks."""
+import subprocess
+import sys
+
+import pytest
+import torch
+
+gpu = pytest.mark.gpu
+BF, F32 = torch.bfloat16, torch.float32
+
+# (B, Nq, Nk): nothing on one side, sizes on both sides of where the contracted axis is split over blocks
+EMPTY = [(b, nq, nk) for n in (1, 448, 449, 480, 481, 5000) for b, nq, nk in ((0, 3, n), (0, n, 3), (2, 0, n), (2, n, 0), (0, n, n), (0, 0, n), (0, n, 0))]
+
+
+def test_workspaces_of_empty_calls():
+    """in a process of its own: a division by zero ends the process"""
+    code = ("from imagefolder_amd import _lib\nl = _lib.lib()\n"
+            f"for B, Nq, Nk in {EMPTY!r}:\n"
+            "    for H, Hk, D in ((4, 4, 64), (8, 2, 128), (1, 1, 8)):\n"
+            "        f, b = (fn(B, Nq, Nk, H, Hk, D) for fn in (l.xq_xattn_forward_workspace_bytes, l.xq_xattn_backward_workspace_bytes))\n"
+            "        assert f == 0, (B, Nq, Nk, H, f)\n"
+            "        assert b <= 4 * B * H * Nq + 256, (B, Nq, Nk, H, b)\n"          # delta alone
+            "print('done')")
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True)
+    assert r.returncode == 0 and "done" in r.stdout, (r.returncode, r.stderr[-500:])
+
+
+@gpu
+@pytest.mark.parametrize("B,Nq,Nk", EMPTY)
+def test_attention_of_empty_calls(B, Nq, Nk):
+    from imagefolder_amd import nn_ops
+    q, k, v = (torch.randn(B, n, 4, 64, device="cuda").to(BF).requires_grad_(True) for n in (Nq, Nk, Nk))
+    y = nn_ops.cross_attention(q, k, v)
+    assert y.shape == q.shape and not y.any()
+    for t, d in zip((q, k, v), torch.autograd.grad(y, (q, k, v), torch.ones_like(y))):
+        assert d.shape == t.shape and not d.any()
+
+
+@gpu
+@pytest.mark.parametrize("N", [448, 449, 481, 5000])
+def test_packed_attention_of_an_empty_batch(N):
+    from imagefolder_amd import nn_ops, ops_dense
+    for entry in (nn_ops.attention_qkvpacked, ops_dense.attention_qkvpacked):
+        qkv = torch.zeros(0, N, 3 * 2 * 32, device="cuda", dtype=BF, requires_grad=True)
+        y = entry(qkv, 2)
+        assert y.shape == (0, N, 64)
+        assert torch.autograd.grad(y, (qkv,), torch.zeros_like(y))[0].shape == qkv.shape
