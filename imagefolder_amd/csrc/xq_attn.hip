@@ -76,14 +76,9 @@ __device__ __forceinline__ uint4 load16_or_zero(const short *p, bool ok) {
     return v;
 }
 
-// v_max3_f32 without the operand canonicalisation that fmaxf() carries under IEEE mode (57 -> 16 instructions per tile)
-// (the compiler places no wait in front of asm that reads a matrix instruction's result: 17 states lie between the two here, where it keeps 12 for its own
-// instructions; what moves code between them has to keep that, or take __builtin_elementwise_maximum as xq_xattn.hip does)
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float d;
-    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
-    return d;
-}
+// The largest of three, NaN if one is (v_maximum3_f32), without the operand canonicalisation that fmaxf() carries under IEEE mode (57 -> 16 instructions per
+// tile).  Not inline asm: the wait that a matrix instruction's result needs before it is read is the compiler's, and it does not see into asm.
+__device__ __forceinline__ float max3(float a, float b, float c) { return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c); }
 
 #define AT_MFMA(A, B, C) __builtin_amdgcn_mfma_f32_32x32x16_bf16((A), (B), (C), 0, 0, 0)
 // A (uint2: this lane's 4 bf16 of column group k) and B (group k + 1) -> one 16-byte store per lane: lanes 0-31 columns 8 k .. 8 k + 7, lanes

@@ -46,3 +46,14 @@ def test_packed_attention_of_an_empty_batch(N):
         y = entry(qkv, 2)
         assert y.shape == (0, N, 64)
         assert torch.autograd.grad(y, (qkv,), torch.zeros_like(y))[0].shape == qkv.shape
+
+
+def test_no_vector_arithmetic_in_inline_asm():
+    """The compiler places no wait between a matrix instruction and inline asm that reads its result: what computes on vector registers is written with builtins"""
+    import pathlib
+    import re
+    csrc = pathlib.Path(__file__).resolve().parents[1] / "imagefolder_amd" / "csrc"
+    sources = sorted(csrc.glob("*.hip")) + sorted(csrc.glob("*.hpp"))
+    assert len(sources) > 10
+    found = [f"{p.name}: {m.group(0)[:60]}" for p in sources for m in re.finditer(r'\basm\s*(?:volatile\s*)?\(\s*"[^"]*\bv_\w+', p.read_text())]
+    assert not found, found
