@@ -6,6 +6,7 @@ import ctypes
 import functools
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -14,6 +15,7 @@ from ._lib import XqError, check
 _TYPES = (torch.bfloat16, torch.float32)
 _raw_stream = torch._C._cuda_getCurrentRawStream       # the handle alone: torch.cuda.current_stream builds an object, 4 us of a 5 us call
 _current_device = torch._C._cuda_getDevice
+_is_tracing = torch._C._is_tracing
 
 
 def _launch(name, device, *args):
@@ -33,13 +35,14 @@ def _at(t):
     return None if t is None else t.data_ptr()
 
 
-def _wants_grad(*tensors):
-    """whether autograd has to see the call (an autograd node costs a small call as much as its kernel)"""
+def _wants_node(*tensors):
+    """whether autograd has to see the call (an autograd node costs a small call as much as its kernel): a gradient is wanted, tangents may be on their way (a dual
+    tensor requires no gradient; the node refuses it, the bare kernel would drop its tangent), or a trace records the call (it sees the node, not the kernel)"""
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
                 return True
-    return False
+    return forward_ad._current_level >= 0 or _is_tracing()
 
 
 def _same_device(name, first, *others):
@@ -129,7 +132,7 @@ def dropout(x, p, key=None, residual=None):
     elif key.dtype != torch.int64 or tuple(key.shape) != (2,) or not key.is_contiguous():
         raise XqError(f"dropout: key is an int64 tensor of two values (got {key.dtype}, shape {tuple(key.shape)})")
     _same_device("dropout", x, residual, key)
-    if not _wants_grad(x, residual):
+    if not _wants_node(x, residual):
         xd = x if _dense(x) else x.contiguous()
         rd = None if residual is None else _like(residual, xd)
         return _dropout(xd, rd, float(p), key, x.dtype if rd is None else rd.dtype)
@@ -190,7 +193,7 @@ def embedding(idx, weight, scale=1.0, padding_idx=None, dtype=None):
             raise XqError(f"embedding: padding_idx = {padding_idx} outside the table of {weight.shape[0]} rows")
         skip = padding_idx % weight.shape[0]
     _same_device("embedding", weight, idx)
-    if not _wants_grad(weight):
+    if not _wants_node(weight):
         return _embedding(idx.contiguous(), weight.contiguous(), float(scale), dtype)
     return EmbeddingFn.apply(idx, weight, float(scale), skip, dtype)
 
@@ -333,6 +336,6 @@ def cross_attention(q, k, v, kv_lens=None, key_mask=None, scale=None):
     _same_device("cross_attention", q, k, v, kv_lens, key_mask)
     kv_lens = None if kv_lens is None else kv_lens.contiguous()
     key_mask = None if key_mask is None else key_mask.contiguous()
-    if not _wants_grad(q, k, v):
+    if not _wants_node(q, k, v):
         return _xattn_forward(_rows(q), _rows(k), _rows(v), kv_lens, key_mask, scale, False)[0]
     return CrossAttentionFn.apply(q, k, v, kv_lens, key_mask, scale)

@@ -57,3 +57,83 @@ def test_no_vector_arithmetic_in_inline_asm():
     assert len(sources) > 10
     found = [f"{p.name}: {m.group(0)[:60]}" for p in sources for m in re.finditer(r'\basm\s*(?:volatile\s*)?\(\s*"[^"]*\bv_\w+', p.read_text())]
     assert not found, found
+
+
+# ---- transforms of autograd other than reverse mode -----------------------------------------------------------------------------------------
+
+def copying_launch(monkeypatch):
+    """stands for the kernels on the CPU: the result's memory gets the (first) input's -> the names launched"""
+    import ctypes
+    from imagefolder_amd import ops_seq
+    calls = []
+
+    def launch(name, device, *args):
+        calls.append(name)
+        if name == "xq_dropout":
+            ctypes.memmove(args[6], args[0], 4 * args[3])
+        elif name == "xq_embedding_forward":
+            ctypes.memmove(args[8], args[2], 4 * args[4] * args[6])
+        else:
+            B, Nq, _, H, _, D = args[3:9]
+            ctypes.memmove(args[14], args[0], 2 * B * Nq * H * D)
+
+    monkeypatch.setattr(ops_seq, "_launch", launch)
+    return calls
+
+
+def forward_calls():
+    from imagefolder_amd import ops_seq
+    key, idx = torch.tensor([1, 2]), torch.arange(5)
+    k = torch.randn(1, 7, 2, 8).to(BF)
+    return (("dropout", torch.randn(40), lambda t: ops_seq.dropout(t, 0.5, key=key)),
+            ("dropout + residual", torch.randn(40), lambda t: ops_seq.dropout(t, 0.5, key=key, residual=t)),
+            ("embedding", torch.randn(5, 8), lambda t: ops_seq.embedding(idx, t)),
+            ("cross_attention", torch.randn(1, 3, 2, 8).to(BF), lambda t: ops_seq.cross_attention(t, k, k)))
+
+
+@pytest.mark.parametrize("i", range(4))
+def test_a_tangent_is_refused_not_lost(i, monkeypatch):
+    """forward-mode differentiation: the operators have no formula for it, so that a dual tensor is an error with and without gradients, as long as a level is open"""
+    from torch.autograd import forward_ad
+    calls = copying_launch(monkeypatch)
+    name, x, f = forward_calls()[i]
+    assert torch.equal(f(x), x) and len(calls) == 1, name
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        assert not dual.requires_grad
+        with pytest.raises(RuntimeError, match="jvp"):
+            f(dual)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="jvp"):
+            f(dual)
+        assert torch.equal(f(x), x)                    # no tangent on it
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(f, (x,), (torch.ones_like(x),))
+
+
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning")
+@pytest.mark.parametrize("i", range(4))
+def test_a_trace_records_the_call(i, monkeypatch):
+    calls = copying_launch(monkeypatch)
+    name, x, f = forward_calls()[i]
+    traced = torch.jit.trace(f, (x,), check_trace=False)
+    other = torch.randn(x.shape).to(x.dtype)
+    before = len(calls)
+    assert torch.equal(traced(other), other) and len(calls) == before + 1, name
+
+
+@gpu
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning")
+@pytest.mark.parametrize("grad", [False, True])
+def test_traced_calls(grad):
+    """a traced program computes each call anew, on its own inputs"""
+    from imagefolder_amd import nn_ops
+    key, idx = torch.tensor([1, 2], device="cuda"), torch.arange(5, device="cuda")
+    k = torch.randn(1, 70, 2, 8, device="cuda").to(BF)
+    for x, f in ((torch.randn(4000, device="cuda"), lambda t: nn_ops.dropout(t, 0.5, key=key)),
+                 (torch.randn(5, 8, device="cuda"), lambda t: nn_ops.embedding(idx, t, scale=3.0)),
+                 (torch.randn(1, 3, 2, 8, device="cuda").to(BF), lambda t: nn_ops.cross_attention(t, k, k)),
+                 (torch.randn(2, 9, 3 * 2 * 32, device="cuda").to(BF), lambda t: nn_ops.attention_qkvpacked(t, 2))):
+        traced = torch.jit.trace(f, (x.clone().requires_grad_(grad),), check_trace=False)
+        for _ in range(3):
+            other = torch.randn(x.shape, device="cuda").to(x.dtype)
+            assert torch.equal(traced(other), f(other))
