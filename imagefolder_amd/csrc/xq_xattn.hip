@@ -224,6 +224,11 @@ struct Stage {
             for (int c = 0; c < CH; ++c) r[c] = load16(base, off[c]);
         }
     }
+    // `left` rows, then the row at element offset `first` again
+    __device__ __forceinline__ void load_repeating(const short *base, int left, uint32_t first) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) r[c] = load16(base, row(c) < left || off[c] == FAR ? off[c] : (first + col(c)) * 2);
+    }
     __device__ __forceinline__ void store(uint32_t tile) const {
 #pragma unroll
         for (int c = 0; c < CH; ++c)
@@ -727,6 +732,9 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(Args a) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------------------------
+// REPEATED ROWS: in the last tile of rows of the two kernels below, those behind the last hold q of the tile's first row, dO = 0, lse = inf and delta = 0: P and dS are 0
+// there.  Not q = 0: that times a key that holds an infinity is NaN, where every real row may have P = 0 (a score of -inf) and the key zero gradients; with a real
+// row's q a score is NaN or inf only where it is in that row too.
 // dk, dv: one key per lane, 32 W keys of one (sample, kv head) a block; tiles of QT rows of q and dO (and lse, delta) in two LDS buffers.
 // 4 x 4096 x <= 4352 keys x 16 heads of 128: 1075 us, 850 TFLOP/s, the matrix pipe busy 43 % of the cycles: the waves (two a SIMD, their registers full) wait for LDS
 // ---------------------------------------------------------------------------------------------------------------------------------------------
@@ -793,7 +801,9 @@ __global__ __launch_bounds__(64 * W, DT > 64 ? 2 : 3) void xattn_dkdv_kernel(Arg
         const int tok0 = (int)quotient((uint32_t)r0, a.g_reciprocal), left = a.R - r0;
         if (!same_places) places(r0 - tok0 * a.G);
         const uint64_t bits = left >= QT ? ~0ull : (1ull << left) - 1;
-        sq.load(a.q.p + b * a.q.sb + tok0 * a.q.sn + (long)hk * a.G * a.q.sh, bits);
+        const short *q0 = a.q.p + b * a.q.sb + tok0 * a.q.sn + (long)hk * a.G * a.q.sh;
+        if (left >= QT) sq.load(q0, ~0ull);
+        else sq.load_repeating(q0, left, (uint32_t)(r0 - tok0 * a.G) * (uint32_t)a.q.sh);
         so.load(a.dout + ((long)b * a.Nq + tok0) * on + (long)hk * a.G * oh, bits);
         if (tid < 2 * QT) {
             const int r = min(r0 + tid % QT, a.R - 1);
@@ -804,7 +814,7 @@ __global__ __launch_bounds__(64 * W, DT > 64 ? 2 : 3) void xattn_dkdv_kernel(Arg
     auto store = [&](int buf) {
         sq.store(Qs + buf * BYTES);
         so.store(Os + buf * BYTES);
-        if (tid < QT) Ls[buf][tid] = tid < rows ? log2_of(rl) * lse_factor : 0.0f;
+        if (tid < QT) Ls[buf][tid] = tid < rows ? log2_of(rl) * lse_factor : BEGIN ? -INFINITY : INFINITY;
         else if (tid < 2 * QT) Ds[buf][tid - QT] = tid - QT >= rows ? 0.0f : BEGIN ? -rl : rl;
     };
 
@@ -823,7 +833,7 @@ __global__ __launch_bounds__(64 * W, DT > 64 ? 2 : 3) void xattn_dkdv_kernel(Arg
         for (int h = 0; h < QT / 32; ++h) {
             if (h && t * QT + 32 * h >= a.R) break;
             const uint32_t Qh = Qs + cur * BYTES + 32 * h * T::ROW, Oh = Qh + 2 * BYTES, Q = Qh + row_at, O = Oh + row_at, Vw = Vs + wave * 32 * T::ROW + row_at;
-            // register j <-> row (j & 3) + 8 (j >> 2) + 4 hh of the tile; rows behind the last have q = dO = 0 and lse = delta = 0: P is 1 there, dS 0
+            // register j <-> row (j & 3) + 8 (j >> 2) + 4 hh of the tile; rows behind the last: REPEATED ROWS above
             f32x16 s, p;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
@@ -979,7 +989,8 @@ __global__ __launch_bounds__(64 * W, DT > 64 ? 2 : 3) void xattn_bwd_kernel(Args
         if (!ROLES || role == 1) {
 #pragma unroll
             for (int ch = 0; ch < CH; ++ch)
-                rq[ch] = load16(a.q.p + b * a.q.sb + tok0 * a.q.sn + (long)hk * a.G * a.q.sh, row_of(ch) < left ? off_q[ch] : FAR);
+                rq[ch] = load16(a.q.p + b * a.q.sb + tok0 * a.q.sn + (long)hk * a.G * a.q.sh,
+                                row_of(ch) < left || off_q[ch] == FAR ? off_q[ch] : ((uint32_t)(r0 - tok0 * a.G) * (uint32_t)a.q.sh + 8 * chunk_of(ch)) * 2);
         }
     };
     auto load = [&](int r0) {
@@ -1018,7 +1029,7 @@ __global__ __launch_bounds__(64 * W, DT > 64 ? 2 : 3) void xattn_bwd_kernel(Args
             for (int ch = 0; ch < CH; ++ch)
                 *(lds_ptr<u32x4>)(uintptr_t)(Qs + buf * BYTES + T::place(row_of(ch), chunk_of(ch))) = __builtin_bit_cast(u32x4, rq[ch]);
         }
-        if (tid < QT) Ls[buf][tid] = tid < rows ? log2_of(rl) * lse_factor : 0.0f;
+        if (tid < QT) Ls[buf][tid] = tid < rows ? log2_of(rl) * lse_factor : -INFINITY;
     };
 
     const int unit = wave - FIRST;
@@ -1078,7 +1089,7 @@ __global__ __launch_bounds__(64 * W, DT > 64 ? 2 : 3) void xattn_bwd_kernel(Args
         if (SB == 2 && t > t0) dq_tile(t - 1, Sb + (cur ^ 1) * SBYTES);
         if (wave_live) {
             const uint32_t Qh = Qs + cur * BYTES, Oh = Os + cur * BYTES, Q = Qh + row_at, O = Oh + row_at;
-            // the products begin at -lse / scale and -delta.  Register j <-> row (j & 3) + 8 (j >> 2) + 4 hh of the tile; rows behind the last have q = dO = 0 and lse = delta = 0: P is 1 there, dS 0
+            // the products begin at -lse / scale and -delta.  Register j <-> row (j & 3) + 8 (j >> 2) + 4 hh of the tile; rows behind the last: REPEATED ROWS above
             f32x16 s, p;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {

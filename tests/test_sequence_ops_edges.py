@@ -137,3 +137,29 @@ def test_traced_calls(grad):
         for _ in range(3):
             other = torch.randn(x.shape, device="cuda").to(x.dtype)
             assert torch.equal(traced(other), f(other))
+
+
+# ---- infinities ------------------------------------------------------------------------------------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize("Nk,D", [(50, 32), (50, 64), (50, 96), (50, 128), (200, 32), (200, 64), (300, 64), (300, 96), (300, 128)])
+@pytest.mark.parametrize("Nq,G", [(1, 1), (31, 1), (32, 1), (33, 1), (65, 1), (300, 1), (11, 3), (11, 5), (50, 8), (700, 2)])
+def test_a_key_at_minus_infinity_has_zero_gradients(Nk, D, Nq, G):
+    """its score is -inf and its P 0 in every row, whatever the number of rows: dk and dv are those of a call where it is masked (dq = dS k is 0 x inf there)"""
+    from imagefolder_amd import nn_ops
+    torch.manual_seed(Nq + D)
+    B, Hk = 2, 2
+    q = torch.randn(B, Nq, Hk * G, D, device="cuda").abs().add(0.5).to(BF).requires_grad_(True)
+    k, v = (torch.randn(B, Nk, Hk, D, device="cuda").to(BF).requires_grad_(True) for _ in range(2))
+    g = torch.randn(B, Nq, Hk * G, D, device="cuda").to(BF)
+    bad = k.detach().clone()
+    bad[:, 7] = 0
+    bad[:, 7, :, 0] = float("-inf")
+    bad.requires_grad_(True)
+    there = torch.ones(B, Nk, dtype=torch.bool, device="cuda")
+    there[:, 7] = False
+    y, want = nn_ops.cross_attention(q, bad, v), nn_ops.cross_attention(q, k, v, key_mask=there)
+    assert torch.equal(y, want)
+    got, ref = torch.autograd.grad(y, (bad, v), g), torch.autograd.grad(want, (k, v), g)
+    for a, b in zip(got, ref):
+        assert not a[:, 7].any() and torch.equal(a, b)
