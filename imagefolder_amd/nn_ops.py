@@ -130,7 +130,7 @@ def attention_qkvpacked(qkv, num_heads):
     C = C3 // 3
     q, k, v = qkv.reshape(B, N, 3, num_heads, C // num_heads).permute(2, 0, 3, 1, 4).unbind(0)
     if qkv.is_cuda:
-        _lib_ran("attention_library", "library (SDPA: head_dim no multiple of 8 up to 128, or fp32 training)")
+        _lib_ran("attention_library", "library (SDPA: head_dim no multiple of 8 up to 128, more than the kernels take in one call, or fp32 training)")
     x = F.scaled_dot_product_attention(q, k, v)
     return x.transpose(1, 2).reshape(B, N, C)
 
@@ -382,7 +382,9 @@ def cross_attention(q, k, v, kv_lens=None, key_mask=None, scale=None):
          up to 128; any strides (a packed k / v projection is read in place; rows that are not 16-byte aligned are copied first);
       kv_lens: int32 / int64 (B,), how many of a sample's keys are valid (clamped to 0 .. Nk: no host check); key_mask: bool (B, Nk), True = valid.  Both on the
          device; a key is valid where both say so.  What lies in masked places (infinities, NaN) reaches nothing; a sample without a valid key gives zeros;
-      scale: 2^-64 .. 2^64; default D ** -0.5.
+      scale: 2^-64 .. 2^64; default D ** -0.5;
+      one call takes up to 2^22 blocks of 128 rows or keys, each (sample, kv head) counted with eight more: B Hk (ceil(n / 128) + 8) <= 2^22 for n = Nk and n = Nq H / Hk
+         (466000 pairs of a few tokens); a larger batch is an XqError and is passed in parts.
     CPU tensors: the same in plain fp32 operations."""
     if q.is_cuda:
         if torch.is_autocast_enabled("cuda"):

@@ -570,7 +570,7 @@ def attention_supported(qkv, num_heads):
 
 def attention_qkvpacked(qkv, num_heads):
     """(B, N, 3*C) -> (B, N, C).  bf16 with head_dim 64: the hand-written kernels on the packed projection; bf16 with another multiple of 8 up to 128:
-    the cross-attention kernels on its views; anything else (the fp32 parity path): library SDPA on strided q/k/v views."""
+    the cross-attention kernels on its views (up to what they take in one call); anything else (the fp32 parity path): library SDPA on strided q/k/v views."""
     from . import nn_ops, ops_f32, ops_seq
     if attention_supported(qkv, num_heads):
         nn_ops.IMPL["attention"] = "hip"

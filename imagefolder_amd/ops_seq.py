@@ -293,8 +293,14 @@ class PackedAttentionFn(torch.autograd.Function):
 
 
 def packed_attention_supported(qkv, num_heads):
-    D = qkv.shape[-1] // (3 * num_heads)
-    return qkv.is_cuda and qkv.dtype == torch.bfloat16 and qkv.dim() == 3 and qkv.shape[-1] == 3 * num_heads * D and D % 8 == 0 and 8 <= D <= 128
+    if not (qkv.is_cuda and qkv.dtype == torch.bfloat16 and qkv.dim() == 3):
+        return False
+    B, N, C3 = qkv.shape
+    D = C3 // (3 * num_heads)
+    if C3 != 3 * num_heads * D or D % 8 or not 8 <= D <= 128:
+        return False
+    # xq_xattn_forward's limits on one call (blocks of a launch; 64 tokens of the packed projection within 32 bits of bytes)
+    return B * num_heads * ((N + 127) // 128 + 8) <= 1 << 22 and B * num_heads * N <= 0x3fffffff and C3 <= 1 << 23
 
 
 @functools.lru_cache(maxsize=4096)

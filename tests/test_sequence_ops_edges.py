@@ -163,3 +163,52 @@ def test_a_key_at_minus_infinity_has_zero_gradients(Nk, D, Nq, G):
     got, ref = torch.autograd.grad(y, (bad, v), g), torch.autograd.grad(want, (k, v), g)
     for a, b in zip(got, ref):
         assert not a[:, 7].any() and torch.equal(a, b)
+
+
+# ---- more than one call of the kernels takes ---------------------------------------------------------------------------------------------------
+
+def packed(B, N, H, D, **kw):
+    from types import SimpleNamespace
+    return SimpleNamespace(**{**dict(is_cuda=True, dtype=BF, shape=torch.Size((B, N, 3 * H * D)), dim=lambda: 3), **kw})
+
+
+@pytest.mark.parametrize("B,N,H,D", [(32768, 49, 16, 32), (29127, 128, 16, 32), (29128, 128, 16, 32), (26214, 129, 16, 8), (26215, 129, 16, 8), (466033, 1, 1, 128), (466034, 1, 1, 128),
+                                     (2, 268434432, 1, 8), (2, 268434433, 1, 8), (1, 1, 21845, 128), (1, 1, 21846, 128), (0, 70000, 3, 32), (4, 0, 3, 32)])
+def test_packed_attention_takes_what_its_kernels_take(B, N, H, D):
+    """the dispatch and the C entry's own limits say the same (its workspace query checks them); the library takes the rest"""
+    from imagefolder_amd import _lib, ops_seq
+    l = _lib.lib()
+    assert l.xq_xattn_forward_workspace_bytes(1, 1, 1, 1, 1, 9) == 0 and "head dim 9" in l.xq_last_error().decode()
+    for fn in (l.xq_xattn_forward_workspace_bytes, l.xq_xattn_backward_workspace_bytes):
+        fn(B, N, N, H, H, D)
+    refused = "too many rows" in l.xq_last_error().decode()
+    if 3 * H * D <= 1 << 23:
+        assert ops_seq.packed_attention_supported(packed(B, N, H, D), H) == (not refused)
+    else:
+        assert not ops_seq.packed_attention_supported(packed(B, N, H, D), H)
+
+
+def test_packed_attention_leaves_other_forms_to_the_library():
+    from imagefolder_amd import ops_seq
+    assert ops_seq.packed_attention_supported(packed(2, 50, 4, 32), 4)
+    for t, H in ((packed(2, 50, 4, 32, dtype=torch.float16), 4), (packed(2, 50, 4, 32, is_cuda=False), 4), (packed(2, 50, 4, 32, dim=lambda: 4), 4), (packed(2, 50, 4, 36), 4),
+                 (packed(2, 50, 4, 136), 4), (packed(2, 50, 4, 32), 5), (packed(2, 50, 1, 2), 2)):
+        assert not ops_seq.packed_attention_supported(t, H)
+
+
+@gpu
+def test_packed_attention_of_more_windows_than_one_call_takes():
+    from imagefolder_amd import nn_ops, ops_dense
+    torch.manual_seed(3)
+    B, N, H, D = 32768, 3, 16, 8
+    qkv = torch.randn(B, N, 3 * H * D, device="cuda").to(BF).requires_grad_(True)
+    for entry in (nn_ops.attention_qkvpacked, ops_dense.attention_qkvpacked):
+        y = entry(qkv, H)
+        (dx,) = torch.autograd.grad(y, (qkv,), torch.ones_like(y))
+        assert y.shape == (B, N, H * D) and dx.shape == qkv.shape and bool(dx.isfinite().all())
+        for b in (0, B // 2, B - 1):
+            q, k, v = qkv.detach()[b].double().view(N, 3, H, D).permute(1, 2, 0, 3)
+            p = torch.softmax(q @ k.transpose(1, 2) * D ** -0.5, -1)
+            # P rounded to bf16 where it meets v and in the row sum, the result once
+            tol = 1.05 * (2 * 2.0 ** -8 * (p @ v.abs()) + 2.0 ** -8 * (p @ v).abs()) + 1e-6
+            assert bool(((y.detach()[b].double().view(N, H, D).transpose(0, 1) - p @ v).abs() <= tol).all())
