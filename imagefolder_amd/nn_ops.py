@@ -367,10 +367,11 @@ def embedding(idx, weight, scale=1.0, padding_idx=None, dtype=None):
 
 
 def module_embedding(module, idx):
-    """the lookup of an nn.Embedding inside a model: nn_ops.embedding, or the module itself for what that does not take (other types, a renormalised or sparse
-    table, gradients scaled by frequency)"""
+    """the lookup of an nn.Embedding inside a model: nn_ops.embedding, or the module itself for what that does not take (other types, more than 2^20 rows, a
+    renormalised or sparse table, gradients scaled by frequency)"""
     w = module.weight
-    if w.is_cuda and w.dtype in (torch.bfloat16, torch.float32) and module.max_norm is None and not (module.sparse or module.scale_grad_by_freq):
+    if (w.is_cuda and w.dtype in (torch.bfloat16, torch.float32) and w.shape[0] <= ops_seq.MAX_ROWS and module.max_norm is None
+            and not (module.sparse or module.scale_grad_by_freq)):
         return embedding(idx, w, padding_idx=module.padding_idx)
     return module(idx)
 

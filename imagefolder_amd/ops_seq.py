@@ -141,6 +141,9 @@ def dropout(x, p, key=None, residual=None):
 
 # ---- embedding -----------------------------------------------------------------------------------------------------------------------------
 
+MAX_ROWS = 1 << 20                                     # of a table, csrc/xq_embed.hip
+
+
 def _embedding(ic, w, scale, dtype):
     V, D = w.shape
     y = w.new_empty((*ic.shape, D), dtype=dtype)

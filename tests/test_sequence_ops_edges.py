@@ -212,3 +212,23 @@ def test_packed_attention_of_more_windows_than_one_call_takes():
             # P rounded to bf16 where it meets v and in the row sum, the result once
             tol = 1.05 * (2 * 2.0 ** -8 * (p @ v.abs()) + 2.0 ** -8 * (p @ v).abs()) + 1e-6
             assert bool(((y.detach()[b].double().view(N, H, D).transpose(0, 1) - p @ v).abs() <= tol).all())
+
+
+def test_the_limit_of_table_rows_is_the_kernels():
+    from imagefolder_amd import _lib, ops_seq
+    l = _lib.lib()
+    assert l.xq_embedding_backward_workspace_bytes(5, ops_seq.MAX_ROWS, 8) > 0 and l.xq_embedding_backward_workspace_bytes(5, ops_seq.MAX_ROWS + 1, 8) == 0
+
+
+@gpu
+@pytest.mark.parametrize("more", [0, 1])
+def test_an_embedding_module_of_many_rows(more):
+    from imagefolder_amd import nn_ops, ops_seq
+    V = ops_seq.MAX_ROWS + more
+    m = torch.nn.Embedding(V, 4, device="cuda")
+    idx = torch.tensor([[0, V - 1, 5], [5, 5, 0]], device="cuda")
+    nn_ops.IMPL.pop("embedding", None)
+    y = nn_ops.module_embedding(m, idx)
+    assert ("embedding" in nn_ops.IMPL) == (more == 0) and torch.equal(y, m(idx))
+    (dw,) = torch.autograd.grad(y.sum(), (m.weight,))
+    assert dw[:, 0].nonzero()[:, 0].tolist() == [0, 5, V - 1] and dw[[0, 5, V - 1], 0].tolist() == [2, 3, 1]
