@@ -11,6 +11,7 @@ ATen implementation of the same op (tests/test_dense_ops_gpu.py).
 """
 import torch
 import torch.nn.functional as F
+from torch.nn.modules.module import _has_any_global_hook
 
 from . import ops_seq
 
@@ -345,9 +346,17 @@ def dropout(x, p=0.5, training=True, key=None, residual=None):
     return ops_seq.dropout(x, p, key, residual)
 
 
+def _runs_plainly(module, cls):
+    """whether a call of `module` is cls.forward and nothing beside it: no hooks, no forward of a subclass or of its own"""
+    return (type(module).forward is cls.forward and "forward" not in module.__dict__
+            and not (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks or _has_any_global_hook()))
+
+
 def module_dropout(module, x):
-    """an nn.Dropout inside a model: the module itself, or nn_ops.dropout where COUNTER_DROPOUT is on and it would drop something on the GPU"""
-    if COUNTER_DROPOUT and module.training and module.p > 0 and x.is_cuda and x.dtype in (torch.bfloat16, torch.float32):
+    """an nn.Dropout inside a model: the module itself, or nn_ops.dropout where COUNTER_DROPOUT is on and it would drop something on the GPU (and nothing hangs on the
+    module's call)"""
+    if (COUNTER_DROPOUT and _runs_plainly(module, torch.nn.Dropout) and module.training and module.p > 0 and not module.inplace and x.is_cuda
+            and x.dtype in (torch.bfloat16, torch.float32)):
         return dropout(x, module.p)
     return module(x)
 
@@ -368,11 +377,13 @@ def embedding(idx, weight, scale=1.0, padding_idx=None, dtype=None):
 
 def module_embedding(module, idx):
     """the lookup of an nn.Embedding inside a model: nn_ops.embedding, or the module itself for what that does not take (other types, more than 2^20 rows, a
-    renormalised or sparse table, gradients scaled by frequency)"""
-    w = module.weight
-    if (w.is_cuda and w.dtype in (torch.bfloat16, torch.float32) and w.shape[0] <= ops_seq.MAX_ROWS and module.max_norm is None
-            and not (module.sparse or module.scale_grad_by_freq)):
-        return embedding(idx, w, padding_idx=module.padding_idx)
+    renormalised or sparse table, gradients scaled by frequency, a table of a tensor class of its own) and where something hangs on the module's call (hooks, another
+    forward)"""
+    if _runs_plainly(module, torch.nn.Embedding):
+        w = module.weight
+        if (w.is_cuda and type(w) in (torch.Tensor, torch.nn.Parameter) and w.dtype in (torch.bfloat16, torch.float32) and w.shape[0] <= ops_seq.MAX_ROWS
+                and module.max_norm is None and not (module.sparse or module.scale_grad_by_freq)):
+            return embedding(idx, w, padding_idx=module.padding_idx)
     return module(idx)
 
 

@@ -232,3 +232,102 @@ def test_an_embedding_module_of_many_rows(more):
     assert ("embedding" in nn_ops.IMPL) == (more == 0) and torch.equal(y, m(idx))
     (dw,) = torch.autograd.grad(y.sum(), (m.weight,))
     assert dw[:, 0].nonzero()[:, 0].tolist() == [0, 5, V - 1] and dw[[0, 5, V - 1], 0].tolist() == [2, 3, 1]
+
+
+# ---- modules that something hangs on -----------------------------------------------------------------------------------------------------------
+
+def hung(make, x):
+    """(a module, what its call adds) for each way of hanging something on a module's call; `seen` tells that it ran"""
+    seen = []
+
+    class Own(type(make())):
+        def forward(self, t):
+            seen.append("subclass")
+            return super().forward(t)
+
+    m = make()
+    m.register_forward_hook(lambda *a: seen.append("hook"))
+    yield m, seen
+    m = make()
+    m.register_forward_pre_hook(lambda *a: seen.append("pre"))
+    yield m, seen
+    m = make()
+    m.__class__ = Own
+    yield m, seen
+    m = make()
+    inner = m.forward
+    m.forward = lambda t: (seen.append("own"), inner(t))[1]
+    yield m, seen
+    m = make()
+    handle = torch.nn.modules.module.register_module_forward_hook(lambda *a: seen.append("global"))
+    try:
+        yield m, seen
+    finally:
+        handle.remove()
+
+
+def dropouts_and_lookups(device):
+    idx = torch.randint(0, 9, (3, 5), device=device)
+    x = torch.randn(3, 40, device=device)
+    return ((lambda: torch.nn.Embedding(9, 16, device=device), idx, "module_embedding", "embedding"), (lambda: torch.nn.Dropout(0.5), x, "module_dropout", "dropout"))
+
+
+@pytest.mark.parametrize("which", [0, 1])
+def test_what_hangs_on_a_module_runs(which, monkeypatch):
+    """on the CPU, with the dispatch's own look at the device (x.is_cuda) left out of the way: what is asked is the module"""
+    from imagefolder_amd import nn_ops
+    monkeypatch.setattr(nn_ops, "COUNTER_DROPOUT", True)
+    make, x, entry, _ = dropouts_and_lookups("cpu")[which]
+    assert nn_ops._runs_plainly(make(), type(make()))
+    for m, seen in hung(make, x):
+        assert not nn_ops._runs_plainly(m, type(make()))
+        seen.clear()
+        getattr(nn_ops, entry)(m, x)
+        assert len(seen) == 1
+    assert nn_ops._runs_plainly(make(), type(make()))
+    for kind in ("register_full_backward_hook", "register_full_backward_pre_hook"):
+        m = make()
+        getattr(m, kind)(lambda *a: None)
+        assert not nn_ops._runs_plainly(m, type(make()))
+
+
+@gpu
+@pytest.mark.parametrize("which", [0, 1])
+def test_what_hangs_on_a_module_runs_on_the_gpu(which, monkeypatch):
+    from imagefolder_amd import nn_ops
+    monkeypatch.setattr(nn_ops, "COUNTER_DROPOUT", True)
+    make, x, entry, name = dropouts_and_lookups("cuda")[which]
+    nn_ops.IMPL.pop(name, None)
+    for m, seen in hung(make, x):
+        seen.clear()
+        getattr(nn_ops, entry)(m, x)
+        assert len(seen) == 1 and name not in nn_ops.IMPL
+    getattr(nn_ops, entry)(make(), x)
+    assert nn_ops.IMPL[name] == "hip"
+
+
+@gpu
+def test_a_module_that_is_no_embedding_in_its_place():
+    from imagefolder_amd import nn_ops
+
+    class Sum(torch.nn.Module):                         # a table without `weight`
+        def __init__(self):
+            super().__init__()
+            self.a, self.b = (torch.nn.Embedding(9, 4, device="cuda") for _ in range(2))
+
+        def forward(self, idx):
+            return self.a(idx) + self.b(idx)
+
+    m, idx = Sum(), torch.randint(0, 9, (3, 5), device="cuda")
+    assert torch.equal(nn_ops.module_embedding(m, idx), m(idx))
+
+    class Scaled(torch.Tensor):                         # a weight with a lookup of its own
+        @classmethod
+        def __torch_function__(cls, func, types, args=(), kwargs=None):
+            out = super().__torch_function__(func, types, args, kwargs or {})
+            return out * 2 if func is torch.nn.functional.embedding else out
+
+    e = torch.nn.Embedding(9, 4, device="cuda")
+    del e._parameters["weight"]
+    e.weight = torch.randn(9, 4, device="cuda").as_subclass(Scaled)
+    assert torch.equal(nn_ops.module_embedding(e, idx).as_subclass(torch.Tensor), e(idx).as_subclass(torch.Tensor))
