@@ -354,8 +354,8 @@ def _runs_plainly(module, cls):
 
 def module_dropout(module, x):
     """an nn.Dropout inside a model: the module itself, or nn_ops.dropout where COUNTER_DROPOUT is on and it would drop something on the GPU (and nothing hangs on the
-    module's call)"""
-    if (COUNTER_DROPOUT and _runs_plainly(module, torch.nn.Dropout) and module.training and module.p > 0 and not module.inplace and x.is_cuda
+    module's call, nor looks on that has a formula for the module alone)"""
+    if (COUNTER_DROPOUT and not ops_seq.transformed() and _runs_plainly(module, torch.nn.Dropout) and module.training and module.p > 0 and not module.inplace and x.is_cuda
             and x.dtype in (torch.bfloat16, torch.float32)):
         return dropout(x, module.p)
     return module(x)
@@ -377,9 +377,9 @@ def embedding(idx, weight, scale=1.0, padding_idx=None, dtype=None):
 
 def module_embedding(module, idx):
     """the lookup of an nn.Embedding inside a model: nn_ops.embedding, or the module itself for what that does not take (other types, more than 2^20 rows, a
-    renormalised or sparse table, gradients scaled by frequency, a table of a tensor class of its own) and where something hangs on the module's call (hooks, another
-    forward)"""
-    if _runs_plainly(module, torch.nn.Embedding):
+    renormalised or sparse table, gradients scaled by frequency, a table of a tensor class of its own), where something hangs on the module's call (hooks, another
+    forward) and under traces and transforms that the module has formulas for"""
+    if not (ops_seq.transformed() or torch.jit.is_tracing()) and _runs_plainly(module, torch.nn.Embedding):
         w = module.weight
         if (w.is_cuda and type(w) in (torch.Tensor, torch.nn.Parameter) and w.dtype in (torch.bfloat16, torch.float32) and w.shape[0] <= ops_seq.MAX_ROWS
                 and module.max_norm is None and not (module.sparse or module.scale_grad_by_freq)):

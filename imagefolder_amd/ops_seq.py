@@ -45,6 +45,12 @@ def _wants_node(*tensors):
     return forward_ad._current_level >= 0 or _is_tracing()
 
 
+def transformed():
+    """whether something other than plain autograd looks on (a compiler's tracing, an open forward-mode level, torch.func's transforms): where a kernel stands for a library
+    operator that has formulas for those, the operator runs"""
+    return torch.compiler.is_compiling() or forward_ad._current_level >= 0 or torch._C._are_functorch_transforms_active()
+
+
 def _same_device(name, first, *others):
     for t in others:
         if t is not None and t.device != first.device:
@@ -296,7 +302,7 @@ class PackedAttentionFn(torch.autograd.Function):
 
 
 def packed_attention_supported(qkv, num_heads):
-    if not (qkv.is_cuda and qkv.dtype == torch.bfloat16 and qkv.dim() == 3):
+    if not (qkv.is_cuda and qkv.dtype == torch.bfloat16 and qkv.dim() == 3) or transformed():
         return False
     B, N, C3 = qkv.shape
     D = C3 // (3 * num_heads)

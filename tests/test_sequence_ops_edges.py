@@ -331,3 +331,74 @@ def test_a_module_that_is_no_embedding_in_its_place():
     del e._parameters["weight"]
     e.weight = torch.randn(9, 4, device="cuda").as_subclass(Scaled)
     assert torch.equal(nn_ops.module_embedding(e, idx).as_subclass(torch.Tensor), e(idx).as_subclass(torch.Tensor))
+
+
+# ---- transforms, where a kernel stands for a library operator ------------------------------------------------------------------------------------
+
+def test_transforms_are_seen():
+    from torch.autograd import forward_ad
+    from imagefolder_amd import ops_seq
+    seen = []
+    f = lambda t: (seen.append(ops_seq.transformed()), (t * t).sum())[1]  # noqa: E731
+    x = torch.ones(3, requires_grad=True)
+    f(x).backward()
+    assert seen == [False]
+    torch.func.grad(f)(torch.ones(3))
+    torch.func.jvp(f, (torch.ones(3),), (torch.ones(3),))
+    torch.vmap(f)(torch.ones(2, 3))
+    with forward_ad.dual_level():
+        f(torch.ones(3))
+        assert not ops_seq.packed_attention_supported(packed(2, 50, 4, 32), 4)
+    assert seen == [False] + [True] * 4 and not ops_seq.transformed()
+    assert ops_seq.packed_attention_supported(packed(2, 50, 4, 32), 4)
+
+
+@gpu
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning")
+def test_a_level_table_under_transforms():
+    from torch.autograd import forward_ad
+    from imagefolder_amd import nn_ops
+    m = torch.nn.Embedding(9, 16, device="cuda")
+    idx = torch.randint(0, 9, (3, 5), device="cuda")
+    w, d = torch.randn(9, 16, device="cuda"), torch.randn(9, 16, device="cuda")
+    with forward_ad.dual_level():
+        del m._parameters["weight"]
+        m.weight = forward_ad.make_dual(w, d)
+        y = forward_ad.unpack_dual(nn_ops.module_embedding(m, idx))
+        assert torch.equal(y.primal, w[idx]) and torch.equal(y.tangent, d[idx])
+    m = torch.nn.Embedding(9, 16, device="cuda")
+    call = lambda p, i=idx: torch.func.functional_call(Lookup(m), {"m.weight": p}, (i,))  # noqa: E731
+    got = torch.func.grad(lambda p: (call(p) ** 2).sum())(w)
+    want = torch.zeros(9, 16, device="cuda").index_add_(0, idx.reshape(-1), 2 * w[idx].reshape(-1, 16))
+    assert torch.allclose(got, want, rtol=1e-5, atol=1e-6)
+    assert torch.equal(torch.func.jvp(call, (w,), (d,))[1], d[idx])
+    assert torch.equal(torch.vmap(call)(torch.stack((w, d))), torch.stack((w[idx], d[idx])))
+    traced = torch.jit.trace(Lookup(m), (idx,), check_trace=False)
+    assert "aten::embedding" in str(traced.inlined_graph)
+    other = torch.randint(0, 9, (3, 5), device="cuda")
+    assert torch.equal(traced(other), m(other))
+
+
+class Lookup(torch.nn.Module):
+    def __init__(self, m):
+        super().__init__()
+        self.m = m
+
+    def forward(self, idx):
+        from imagefolder_amd import nn_ops
+        return nn_ops.module_embedding(self.m, idx)
+
+
+@gpu
+def test_packed_attention_under_a_transform():
+    """the gradient of torch.func through the library's operator, against the kernels' own"""
+    from torch.nn.attention import SDPBackend, sdpa_kernel
+    from imagefolder_amd import nn_ops
+    torch.manual_seed(2)
+    x, g = torch.randn(2, 60, 3 * 4 * 32, device="cuda").to(BF), torch.randn(2, 60, 4 * 32, device="cuda").to(BF)
+    leaf = x.clone().requires_grad_(True)
+    (want,) = torch.autograd.grad(nn_ops.attention_qkvpacked(leaf, 4), (leaf,), g)
+    with sdpa_kernel([SDPBackend.FLASH_ATTENTION, SDPBackend.EFFICIENT_ATTENTION]):
+        got = torch.func.grad(lambda t: (nn_ops.attention_qkvpacked(t, 4).float() * g.float()).sum())(x)
+    # each side rounds P, dS, the rounded O in delta and the result to bf16: 4 * 2^-8 in norm, twice
+    assert float((got.double() - want.double()).norm()) <= 8 * 2.0 ** -8 * float(want.double().norm())
