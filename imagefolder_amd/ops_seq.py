@@ -163,6 +163,17 @@ def _embedding_workspace(N, V, D):
     return _lib.lib().xq_embedding_backward_workspace_bytes(N, V, D)
 
 
+def _embedding_gradient(ic, g, V, D, scale, skip, wdtype):
+    gc = g.contiguous()
+    dw = gc.new_empty((V, D), dtype=wdtype)
+    N = ic.numel()
+    nbytes = _embedding_workspace(N, V, D)
+    ws = gc.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    _launch("xq_embedding_backward", gc.device, ic.data_ptr(), ic.dtype == torch.int64, gc.data_ptr(), gc.dtype == torch.bfloat16, N, V, D, scale, skip,
+            dw.data_ptr(), wdtype == torch.bfloat16, _at(ws), nbytes)
+    return dw
+
+
 class EmbeddingFn(torch.autograd.Function):
     """y = scale * weight[idx] (xq_embedding_forward); the gradient of the table from the tokens sorted by row (xq_embedding_backward)."""
 
@@ -176,19 +187,36 @@ class EmbeddingFn(torch.autograd.Function):
     @staticmethod
     @_first_order
     def backward(ctx, g):
+        return None, _embedding_gradient(*ctx.saved_tensors, g, *ctx.cfg), None, None, None
+
+
+class EmbeddingAgainFn(EmbeddingFn):
+    """the lookup of an nn.Embedding, whose gradient can be differentiated again as the module's can"""
+
+    @staticmethod
+    def backward(ctx, g):
+        f = EmbeddingGradientFn.apply if torch.is_grad_enabled() else _embedding_gradient
+        return None, f(*ctx.saved_tensors, g, *ctx.cfg), None, None, None
+
+
+class EmbeddingGradientFn(torch.autograd.Function):
+    """the gradient of the table is linear in g: its own gradient is the lookup of what comes back, zeros where g added nothing"""
+
+    @staticmethod
+    def forward(ctx, ic, g, V, D, scale, skip, wdtype):
+        ctx.save_for_backward(ic)
+        ctx.cfg = (V, scale, skip, g.dtype)
+        return _embedding_gradient(ic, g, V, D, scale, skip, wdtype)
+
+    @staticmethod
+    def backward(ctx, gg):
         (ic,) = ctx.saved_tensors
-        V, D, scale, skip, wdtype = ctx.cfg
-        gc = g.contiguous()
-        dw = gc.new_empty((V, D), dtype=wdtype)
-        N = ic.numel()
-        nbytes = _embedding_workspace(N, V, D)
-        ws = gc.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-        _launch("xq_embedding_backward", gc.device, ic.data_ptr(), ic.dtype == torch.int64, gc.data_ptr(), gc.dtype == torch.bfloat16, N, V, D, scale, skip,
-                dw.data_ptr(), wdtype == torch.bfloat16, _at(ws), nbytes)
-        return None, dw, None, None, None
+        V, scale, skip, dtype = ctx.cfg
+        dg = embedding(ic, gg, scale, None, dtype, again=True)
+        return None, torch.where(((ic >= 0) & (ic < V) & (ic != skip)).unsqueeze(-1), dg, torch.zeros_like(dg)), None, None, None, None, None
 
 
-def embedding(idx, weight, scale=1.0, padding_idx=None, dtype=None):
+def embedding(idx, weight, scale=1.0, padding_idx=None, dtype=None, again=False):
     dtype = weight.dtype if dtype is None else dtype
     if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:
         raise XqError(f"embedding: the table is (rows, width) (got shape {tuple(weight.shape)})")
@@ -204,7 +232,7 @@ def embedding(idx, weight, scale=1.0, padding_idx=None, dtype=None):
     _same_device("embedding", weight, idx)
     if not _wants_node(weight):
         return _embedding(idx.contiguous(), weight.contiguous(), float(scale), dtype)
-    return EmbeddingFn.apply(idx, weight, float(scale), skip, dtype)
+    return (EmbeddingAgainFn if again else EmbeddingFn).apply(idx, weight, float(scale), skip, dtype)
 
 
 # ---- attention to another sequence ---------------------------------------------------------------------------------------------------------

@@ -402,3 +402,28 @@ def test_packed_attention_under_a_transform():
         got = torch.func.grad(lambda t: (nn_ops.attention_qkvpacked(t, 4).float() * g.float()).sum())(x)
     # each side rounds P, dS, the rounded O in delta and the result to bf16: 4 * 2^-8 in norm, twice
     assert float((got.double() - want.double()).norm()) <= 8 * 2.0 ** -8 * float(want.double().norm())
+
+
+@gpu
+@pytest.mark.parametrize("pad", [None, 3])
+def test_second_derivatives_of_a_level_table(pad):
+    """as the module's: y = w[idx], L = sum c y^4, dL/dw, the gradient of its product with d, and of that once more (of fp32 sums of few terms: 2^-18 of their size)"""
+    from imagefolder_amd import nn_ops
+    torch.manual_seed(1)
+    m = torch.nn.Embedding(9, 16, padding_idx=pad, device="cuda")
+    idx = torch.randint(0, 9, (3, 20), device="cuda")
+    c, d = torch.randn(3, 20, 16, device="cuda"), torch.randn(9, 16, device="cuda")
+
+    def derivatives(look):
+        (a,) = torch.autograd.grad((c * look(idx) ** 4).sum(), (m.weight,), create_graph=True)
+        (b,) = torch.autograd.grad((a * d).sum(), (m.weight,), create_graph=True)
+        (e,) = torch.autograd.grad((b * d).sum(), (m.weight,))
+        return a.detach(), b.detach(), e
+
+    nn_ops.IMPL.pop("embedding", None)
+    got = derivatives(lambda i: nn_ops.module_embedding(m, i))
+    assert nn_ops.IMPL["embedding"] == "hip"
+    want = derivatives(m)
+    for a, b in zip(got, want):
+        assert float((a - b).abs().max()) <= 2.0 ** -18 * 24 * float(m.weight.detach().abs().max()) ** 3 * 60 * float(c.abs().max()) * max(1, float(d.abs().max())) ** 2
+        assert float(b.abs().max()) > 1e-2 and (pad is None or not a[pad].any())
