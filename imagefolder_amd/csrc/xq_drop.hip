@@ -47,8 +47,8 @@ __device__ __forceinline__ void load8(const T *p, long left, float (&v)[8]) {
 }
 
 template <typename TX, typename TY, bool RES, bool VEC>
-__global__ __launch_bounds__(256) void dropout_kernel(const TX *__restrict__ x, const TY *__restrict__ residual, long n, uint32_t threshold, float factor,
-                                                      const uint64_t *__restrict__ key, TY *__restrict__ y) {
+__global__ __launch_bounds__(256) void dropout_kernel(const TX *x, const TY *residual, long n, uint32_t threshold, float factor, const uint64_t *__restrict__ key,
+                                                      TY *y) {                  // (no __restrict__: y may be x, a group's loads come before its stores)
     const uint64_t seed = key[0], stream = key[1];
     const long groups = (n + 7) / 8, step = (long)gridDim.x * 256;
     for (long g = (long)blockIdx.x * 256 + threadIdx.x; g < groups; g += step) {

@@ -427,3 +427,23 @@ def test_second_derivatives_of_a_level_table(pad):
     for a, b in zip(got, want):
         assert float((a - b).abs().max()) <= 2.0 ** -18 * 24 * float(m.weight.detach().abs().max()) ** 3 * 60 * float(c.abs().max()) * max(1, float(d.abs().max())) ** 2
         assert float(b.abs().max()) > 1e-2 and (pad is None or not a[pad].any())
+
+
+# ---- dropout in place --------------------------------------------------------------------------------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize("kind", [BF, F32])
+@pytest.mark.parametrize("first", [0, 1])
+@pytest.mark.parametrize("n", [1, 8, 4099, 3000001])
+def test_dropout_in_place(n, first, kind):
+    """xq_dropout with y = x (the C entry's promise), on aligned elements and from an odd one on, with and without a residual"""
+    from imagefolder_amd import _lib
+    key = torch.tensor([5, 7], device="cuda")
+    base = torch.randn(n + first, device="cuda").to(kind)
+    r = torch.randn(n + first, device="cuda").to(kind)[first:]
+    stream = torch.cuda.current_stream().cuda_stream
+    for res in (None, r.data_ptr()):
+        apart, x = torch.zeros_like(base)[first:], base.clone()[first:]
+        for y in (apart, x):
+            assert _lib.lib().xq_dropout(x.data_ptr(), kind == BF, res, n, 0.3, key.data_ptr(), y.data_ptr(), kind == BF, stream) == 0
+        assert torch.equal(apart, x)
