@@ -1358,6 +1358,9 @@ extern "C" int xq_xattn_backward(const void *q, const void *k, const void *v, co
             }
     }
     if (((uintptr_t)out | (uintptr_t)dout) & 15) return xq_set_error(XQ_EINVAL, "%s: out and dout have to be 16-byte aligned", fn);
+    // (out and dout are read like q: a tile's rows at 32-bit byte offsets)
+    if ((Nq > 1 ? 64 * (long)H * D : 0) + (long)(H / Hk) * D > (1L << 30))
+        return xq_set_error(XQ_EINVAL, "%s: rows of out and dout are too wide (64 tokens within 2^30 elements: %ld heads of %ld)", fn, (long)H, (long)D);
     const Sizes z = sizes_of(B, Nq, Nk, H, Hk, D);
     if (z.bwd_bytes && (!workspace || workspace_bytes < z.bwd_bytes))
         return xq_set_error(XQ_ENOSPACE, "%s: workspace too small (need %ld bytes, got %ld)", fn, (long)z.bwd_bytes, (long)workspace_bytes);

@@ -593,7 +593,7 @@ int xq_embedding_backward(const void *idx, int idx_i64, const void *g, int g_bf1
 size_t xq_xattn_forward_workspace_bytes(int B, int Nq, int Nk, int H, int Hk, int D);
 int xq_xattn_forward(const void *q, const void *k, const void *v, int B, int Nq, int Nk, int H, int Hk, int D, const int64_t *strides, const void *kv_lens,
                      int lens_i64, const void *key_mask, float scale, void *out, float *lse, void *workspace, size_t workspace_bytes, xq_stream_t stream);
-/* its gradients: dq, dk, dv bf16 with `grad_strides` (HOST, nine, as above, but none of 0 over more than one row); out, dout contiguous; every row of dq, dk, dv is written (masked keys with zeros).
+/* its gradients: dq, dk, dv bf16 with `grad_strides` (HOST, nine, as above, but none of 0 over more than one row); out, dout contiguous (64 tokens within 2^30 elements); every row of dq, dk, dv is written (masked keys with zeros).
  * No atomics: the same bits from run to run.  workspace: xq_xattn_backward_workspace_bytes. */
 size_t xq_xattn_backward_workspace_bytes(int B, int Nq, int Nk, int H, int Hk, int D);
 int xq_xattn_backward(const void *q, const void *k, const void *v, const void *out, const void *dout, const float *lse, int B, int Nq, int Nk, int H, int Hk,

@@ -447,3 +447,19 @@ def test_dropout_in_place(n, first, kind):
         for y in (apart, x):
             assert _lib.lib().xq_dropout(x.data_ptr(), kind == BF, res, n, 0.3, key.data_ptr(), y.data_ptr(), kind == BF, stream) == 0
         assert torch.equal(apart, x)
+
+
+# ---- offsets -----------------------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("H,Hk,Nq,taken", [(1 << 17, 1 << 17, 64, False), ((1 << 17) - 1, (1 << 17) - 1, 64, True), (1 << 17, 1, 2, False), ((1 << 17) - 2048, 1, 2, True), (1 << 23, 1, 1, True),
+                                           ((1 << 23) + 1, 1, 1, False), (1 << 24, 1, 1, False)])
+def test_rows_of_out_past_32_bits_of_bytes_are_refused(H, Hk, Nq, taken):
+    """the C entry, on head-major q and dq (or broadcast ones): no launch either way, the workspace handed in is too small"""
+    import ctypes
+    from imagefolder_amd import _lib
+    l, one, D, Nk = _lib.lib(), ctypes.c_void_p(16), 128, 300
+    st = (ctypes.c_int64 * 9)(*[0, D, 0] + [64] * 6)
+    grad = (ctypes.c_int64 * 9)(*[64, D, 8] + [64] * 6)
+    rc = l.xq_xattn_backward(one, one, one, one, one, one, 1, Nq, Nk, H, Hk, D, st, None, 0, None, ctypes.c_float(0.1), one, one, one, grad, one, 0, None)
+    assert (rc, "too small" if taken else "too wide") == (-2 if taken else -1, "too small" if taken else "too wide")
+    assert ("too small" if taken else "too wide") in l.xq_last_error().decode()
