@@ -240,10 +240,12 @@ def embedding(idx, weight, scale=1.0, padding_idx=None, dtype=None, again=False)
 _NINE = ctypes.c_int64 * 9
 
 
-def _rows(t):
-    """t (B, N, heads, D) as the kernels read it: elements of a row side by side, rows 16-byte aligned; a copy where it is not"""
+def _rows(t, group=1):
+    """t (B, N, heads, D) as the kernels read it: elements of a row side by side, rows 16-byte aligned, 64 tokens and the `group` heads that share a kv head within
+    2^30 elements; a copy where it is not"""
     s = t.stride()
-    if (s[3] == 1 or t.shape[3] == 1) and not (s[0] | s[1] | s[2]) & 7 and not t.data_ptr() & 15 and s[1] <= 1 << 23 and s[2] <= 1 << 22:
+    if (s[3] == 1 or t.shape[3] == 1) and not (s[0] | s[1] | s[2]) & 7 and not t.data_ptr() & 15 and s[1] <= 1 << 23 and s[2] <= 1 << 22 and (
+            64 * s[1] + group * s[2] <= 1 << 30):
         return t
     if t.is_contiguous() and not t.data_ptr() & 15:
         return t                                       # (strides of dimensions of one element may be anything: _nine leaves them out)
@@ -287,7 +289,7 @@ class CrossAttentionFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, lens, mask, scale):
-        q, k, v = _rows(q), _rows(k), _rows(v)
+        q, k, v = _rows(q, q.shape[2] // k.shape[2]), _rows(k), _rows(v)
         out, lse = _xattn_forward(q, k, v, lens, mask, scale, True)
         ctx.save_for_backward(q, k, v, out, lse, lens, mask)
         ctx.scale = scale
@@ -380,5 +382,5 @@ def cross_attention(q, k, v, kv_lens=None, key_mask=None, scale=None):
     kv_lens = None if kv_lens is None else kv_lens.contiguous()
     key_mask = None if key_mask is None else key_mask.contiguous()
     if not _wants_node(q, k, v):
-        return _xattn_forward(_rows(q), _rows(k), _rows(v), kv_lens, key_mask, scale, False)[0]
+        return _xattn_forward(_rows(q, q.shape[2] // k.shape[2]), _rows(k), _rows(v), kv_lens, key_mask, scale, False)[0]
     return CrossAttentionFn.apply(q, k, v, kv_lens, key_mask, scale)

@@ -463,3 +463,15 @@ def test_rows_of_out_past_32_bits_of_bytes_are_refused(H, Hk, Nq, taken):
     rc = l.xq_xattn_backward(one, one, one, one, one, one, 1, Nq, Nk, H, Hk, D, st, None, 0, None, ctypes.c_float(0.1), one, one, one, grad, one, 0, None)
     assert (rc, "too small" if taken else "too wide") == (-2 if taken else -1, "too small" if taken else "too wide")
     assert ("too small" if taken else "too wide") in l.xq_last_error().decode()
+
+
+def test_views_that_the_kernels_do_not_reach_over_are_copied():
+    """head-major q of long sequences under many shared heads: 64 tokens and the group's heads span more than 2^30 elements (no memory behind meta tensors)"""
+    from imagefolder_amd import ops_seq
+    q = torch.empty(1, 512, 32768, 128, dtype=BF, device="meta").transpose(1, 2)           # heads 2^22 elements apart
+    assert ops_seq._rows(q) is q and ops_seq._rows(q, 254) is q
+    for group in (256, 512):
+        copy = ops_seq._rows(q, group)
+        assert copy.is_contiguous() and copy.shape == q.shape
+    flat = torch.empty(1, 70, 512, 128, dtype=BF, device="meta")
+    assert ops_seq._rows(flat, 512) is flat
