@@ -369,8 +369,9 @@ def embedding(idx, weight, scale=1.0, padding_idx=None, dtype=None):
     if not weight.is_cuda:
         IMPL["embedding"] = "library (CPU)"
         y = F.embedding(idx, weight, padding_idx)
-        y = y if scale == 1.0 else y * scale
-        return y if dtype is None else y.to(dtype)
+        if scale != 1.0:
+            y = y.to(torch.promote_types(y.dtype, torch.float32)) * scale
+        return y.to(weight.dtype if dtype is None else dtype)
     IMPL["embedding"] = "hip"
     return ops_seq.embedding(idx, weight, scale, padding_idx, dtype)
 

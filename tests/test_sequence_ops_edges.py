@@ -475,3 +475,21 @@ def test_views_that_the_kernels_do_not_reach_over_are_copied():
         assert copy.is_contiguous() and copy.shape == q.shape
     flat = torch.empty(1, 70, 512, 128, dtype=BF, device="meta")
     assert ops_seq._rows(flat, 512) is flat
+
+
+# ---- on the CPU --------------------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("wt", [BF, torch.float16, F32, torch.float64])
+@pytest.mark.parametrize("yt", [None, BF, F32, torch.float64])
+def test_a_scaled_lookup_on_the_cpu_is_rounded_once(wt, yt):
+    from imagefolder_amd import nn_ops
+    torch.manual_seed(0)
+    w, idx = torch.randn(50, 8).to(wt).requires_grad_(True), torch.randint(0, 50, (4, 30))
+    y = nn_ops.embedding(idx, w, scale=1.7, dtype=yt)
+    assert y.dtype == (yt or wt)
+    want = w.detach().double()[idx] * 1.7
+    # the product in 32 bits (64 for a 64-bit table), then the result's rounding
+    product = 2.0 ** -52 if wt == torch.float64 else 2.0 ** -23
+    assert bool(((y.detach().double() - want).abs() <= want.abs() * (torch.finfo(y.dtype).eps / 2 * (1 + 2.0 ** -7) + product)).all())
+    (dw,) = torch.autograd.grad(y.sum(), (w,))
+    assert dw.dtype == wt and dw[idx[0, 0], 0] > 0
