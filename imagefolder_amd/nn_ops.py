@@ -333,17 +333,20 @@ def dropout(x, p=0.5, training=True, key=None, residual=None):
            must not change before the backward pass has; None draws one from the device's default generator (torch.manual_seed, graph-safe);
       residual: added in fp32 before the one rounding; x's shape, x's type or fp32 (the result has its type).
     CPU tensors: F.dropout (no key there)."""
+    if training and p != 0 and x.is_cuda:
+        IMPL["dropout"] = "hip"
+        return ops_seq.dropout(x, p, key, residual)
+    ops_seq.check_dropout(x, p, residual)
     if not training or p == 0:
         return x if residual is None else x + residual
-    if not x.is_cuda:
-        if key is not None:
-            from ._lib import XqError
-            raise XqError("dropout: a keyed mask is computed on an MI355X only (x lives on the CPU)")
-        IMPL["dropout"] = "library (CPU)"
-        y = F.dropout(x, p)
-        return y if residual is None else y + residual
-    IMPL["dropout"] = "hip"
-    return ops_seq.dropout(x, p, key, residual)
+    if key is not None:
+        from ._lib import XqError
+        raise XqError("dropout: a keyed mask is computed on an MI355X only (x lives on the CPU)")
+    IMPL["dropout"] = "library (CPU)"
+    if residual is None:
+        return F.dropout(x, p)
+    wide = torch.promote_types(residual.dtype, torch.float32)
+    return (F.dropout(x.to(wide), p) + residual).to(residual.dtype)
 
 
 def _runs_plainly(module, cls):

@@ -122,9 +122,8 @@ class DropoutFn(torch.autograd.Function):
         return dx, (g if ctx.needs_input_grad[1] else None), None, None
 
 
-def dropout(x, p, key=None, residual=None):
-    if x.dtype not in _TYPES:
-        raise XqError(f"dropout: x of type {x.dtype} (bf16 / fp32)")
+def check_dropout(x, p, residual):
+    """what holds on whatever device, training or not"""
     if not 0.0 <= p <= 1.0:
         raise XqError(f"dropout: p = {p} does not lie in [0, 1]")
     if residual is not None:
@@ -132,6 +131,12 @@ def dropout(x, p, key=None, residual=None):
             raise XqError(f"dropout: residual of shape {tuple(residual.shape)} for x of shape {tuple(x.shape)}")
         if residual.dtype != x.dtype and residual.dtype != torch.float32:
             raise XqError(f"dropout: residual of type {residual.dtype} for x of type {x.dtype} (x's own type or fp32)")
+
+
+def dropout(x, p, key=None, residual=None):
+    if x.dtype not in _TYPES:
+        raise XqError(f"dropout: x of type {x.dtype} (bf16 / fp32)")
+    check_dropout(x, p, residual)
     if key is None:
         # from the device's default generator: follows torch.manual_seed, and a captured graph draws anew at every replay
         key = torch.randint(-2 ** 63, 2 ** 63 - 1, (2,), dtype=torch.int64, device=x.device)

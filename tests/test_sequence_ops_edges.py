@@ -493,3 +493,27 @@ def test_a_scaled_lookup_on_the_cpu_is_rounded_once(wt, yt):
     assert bool(((y.detach().double() - want).abs() <= want.abs() * (torch.finfo(y.dtype).eps / 2 * (1 + 2.0 ** -7) + product)).all())
     (dw,) = torch.autograd.grad(y.sum(), (w,))
     assert dw.dtype == wt and dw[idx[0, 0], 0] > 0
+
+
+def test_dropout_checks_its_arguments_on_every_path():
+    """the CPU, evaluation and p = 0 refuse what a training step on the GPU refuses"""
+    from imagefolder_amd import nn_ops
+    from imagefolder_amd._lib import XqError
+    x = torch.randn(6, 8)
+    for training in (True, False):
+        for kw, what in ((dict(p=1.5), r"\[0, 1\]"), (dict(p=float("nan")), r"\[0, 1\]"), (dict(p=-0.1), r"\[0, 1\]"), (dict(residual=torch.zeros(8)), "residual of shape"),
+                         (dict(p=0.0, residual=torch.zeros(1, 8)), "residual of shape"), (dict(residual=x.to(BF)), "residual of type")):
+            with pytest.raises(XqError, match=what):
+                nn_ops.dropout(x, training=training, **{"p": 0.5, **kw})
+        assert nn_ops.dropout(x, 0.5, training, residual=x).dtype == F32
+
+
+@pytest.mark.parametrize("rt", [BF, F32])
+def test_dropout_and_residual_on_the_cpu_are_rounded_once(rt):
+    from imagefolder_amd import nn_ops
+    x, r = torch.randn(5000).to(BF), torch.randn(5000).to(rt)
+    y = nn_ops.dropout(x, 0.3, residual=r)
+    assert y.dtype == rt
+    kept, dropped = x.double() / 0.7 + r.double(), r.double()
+    off = lambda want: (y.double() - want).abs() <= want.abs() * torch.finfo(rt).eps / 2 * (1 + 2.0 ** -7) + x.double().abs() * 2.0 ** -22  # noqa: E731
+    assert bool((off(kept) | off(dropped)).all()) and 0.2 < float((y.double() == dropped).double().mean()) < 0.4
