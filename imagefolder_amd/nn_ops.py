@@ -126,7 +126,7 @@ def attention_qkvpacked(qkv, num_heads):
             return ops_f32.AttentionF32Fn.apply(qkv, num_heads)
         if ops_seq.packed_attention_supported(qkv, num_heads):
             IMPL["attention"] = "hip (xq_xattn_forward / xq_xattn_backward)"
-            return ops_seq.PackedAttentionFn.apply(qkv, num_heads)
+            return ops_seq.packed_attention(qkv, num_heads)
     B, N, C3 = qkv.shape
     C = C3 // 3
     q, k, v = qkv.reshape(B, N, 3, num_heads, C // num_heads).permute(2, 0, 3, 1, 4).unbind(0)

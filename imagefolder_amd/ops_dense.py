@@ -584,7 +584,7 @@ def attention_qkvpacked(qkv, num_heads):
         return ops_f32.AttentionF32Fn.apply(qkv, num_heads)
     if ops_seq.packed_attention_supported(qkv, num_heads):
         nn_ops.IMPL["attention"] = "hip (xq_xattn_forward / xq_xattn_backward)"
-        return ops_seq.PackedAttentionFn.apply(qkv, num_heads)
+        return ops_seq.packed_attention(qkv, num_heads)
     nn_ops.IMPL["attention"] = "library (SDPA)"
     B, N, C3 = qkv.shape
     C = C3 // 3

@@ -309,21 +309,25 @@ class CrossAttentionFn(torch.autograd.Function):
         return dq, dk, dv, None, None, None
 
 
+def _packed_forward(x, num_heads, want_lse):
+    B, N, C3 = x.shape
+    x = x.contiguous()
+    if x.data_ptr() & 15:
+        x = x.clone()
+    q, k, v = x.view(B, N, 3, num_heads, C3 // (3 * num_heads)).unbind(2)
+    scale = float(q.shape[3]) ** -0.5
+    out, lse = _xattn_forward(q, k, v, None, None, scale, want_lse)
+    return x, out, lse, scale
+
+
 class PackedAttentionFn(torch.autograd.Function):
     """self-attention on the packed (B, N, 3, H, D) projection through the same kernels, for the head widths that csrc/xq_attn.hip (64) does not take"""
 
     @staticmethod
     def forward(ctx, qkv, num_heads):
-        B, N, C3 = qkv.shape
-        x = qkv.detach().contiguous()
-        if x.data_ptr() & 15:
-            x = x.clone()
-        q, k, v = x.view(B, N, 3, num_heads, C3 // (3 * num_heads)).unbind(2)
-        scale = float(q.shape[3]) ** -0.5
-        out, lse = _xattn_forward(q, k, v, None, None, scale, True)
+        x, out, lse, ctx.scale = _packed_forward(qkv.detach(), num_heads, True)
         ctx.save_for_backward(x, out, lse)
-        ctx.scale = scale
-        return out.view(B, N, C3 // 3)
+        return out.flatten(2)
 
     @staticmethod
     @_first_order
@@ -334,6 +338,12 @@ class PackedAttentionFn(torch.autograd.Function):
         _xattn_backward(*x.view(B, N, 3, H, D).unbind(2), out, g.detach().to(x.dtype).reshape(B, N, H, D), lse, None, None, ctx.scale,
                         *dx.view(B, N, 3, H, D).unbind(2))
         return dx, None
+
+
+def packed_attention(qkv, num_heads):
+    if _wants_node(qkv):
+        return PackedAttentionFn.apply(qkv, num_heads)
+    return _packed_forward(qkv, num_heads, False)[1].flatten(2)
 
 
 def packed_attention_supported(qkv, num_heads):
