@@ -398,11 +398,13 @@ def cross_attention(q, k, v, kv_lens=None, key_mask=None, scale=None):
       q: (B, Nq, H, D); k, v: (B, Nk, Hk, D) with H a multiple of Hk (head h reads kv head h // (H // Hk)); bf16, or cast to it by bf16 autocast; D a multiple of 8
          up to 128; any strides (a packed k / v projection is read in place; rows that are not 16-byte aligned are copied first);
       kv_lens: int32 / int64 (B,), how many of a sample's keys are valid (clamped to 0 .. Nk: no host check); key_mask: bool (B, Nk), True = valid.  Both on the
-         device; a key is valid where both say so.  What lies in masked places (infinities, NaN) reaches nothing; a sample without a valid key gives zeros;
+         device; a key is valid where both say so.  What lies in masked places (infinities, NaN) reaches nothing; a sample without a valid key gives zeros, as does a
+         row whose valid scores are all -inf (a score of -inf is a key that is not there);
       scale: 2^-64 .. 2^64; default D ** -0.5;
       one call takes up to 2^22 blocks of 128 rows or keys, each (sample, kv head) counted with eight more: B Hk (ceil(n / 128) + 8) <= 2^22 for n = Nk and n = Nq H / Hk
          (466000 pairs of a few tokens); a larger batch is an XqError and is passed in parts.
-    CPU tensors: the same in plain fp32 operations."""
+    The softmax's statistics and all sums are fp32; its weights P and their gradients dS are rounded to bf16, as operands of the matrix instructions (0.002 - 0.003 of a
+    result's norm in all).  CPU tensors: the same in plain fp32 operations."""
     if q.is_cuda:
         if torch.is_autocast_enabled("cuda"):
             act = torch.get_autocast_dtype("cuda")
@@ -419,5 +421,7 @@ def cross_attention(q, k, v, kv_lens=None, key_mask=None, scale=None):
     valid = valid[:, None, None]
     kk, vv = (t.float().repeat_interleave(G, dim=2).transpose(1, 2).masked_fill(~valid.transpose(2, 3), 0.0) for t in (k, v))
     s = (torch.matmul(q.float().transpose(1, 2), kk.transpose(2, 3)) * scale).masked_fill(~valid, float("-inf"))
-    p = torch.softmax(s.masked_fill(~valid.any(-1, keepdim=True), 0.0), dim=-1).masked_fill(~valid, 0.0) if Nk else s
-    return torch.matmul(p, vv).transpose(1, 2).to(q.dtype)
+    if Nk:
+        none = (s == float("-inf")).all(-1, keepdim=True)       # a row without a key, or with scores of -inf alone
+        s = torch.softmax(s.masked_fill(none, 0.0), dim=-1).masked_fill(none | ~valid, 0.0)
+    return torch.matmul(s, vv).transpose(1, 2).to(q.dtype)

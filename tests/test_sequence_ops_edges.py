@@ -517,3 +517,22 @@ def test_dropout_and_residual_on_the_cpu_are_rounded_once(rt):
     kept, dropped = x.double() / 0.7 + r.double(), r.double()
     off = lambda want: (y.double() - want).abs() <= want.abs() * torch.finfo(rt).eps / 2 * (1 + 2.0 ** -7) + x.double().abs() * 2.0 ** -22  # noqa: E731
     assert bool((off(kept) | off(dropped)).all()) and 0.2 < float((y.double() == dropped).double().mean()) < 0.4
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+@pytest.mark.parametrize("Nq,Nk", [(3, 5), (40, 40), (40, 300), (300, 700), (1, 3000)])
+def test_rows_whose_scores_are_all_minus_infinity(device, Nq, Nk):
+    """every second key has a score of -inf: as if it were masked; where those are the only valid ones a row is zero, on every path"""
+    from imagefolder_amd import nn_ops
+    torch.manual_seed(Nq)
+    kind = BF if device == "cuda" else F32
+    k, v = (torch.randn(2, Nk, 2, 16, device=device).to(kind) for _ in range(2))
+    k[..., 0] = 0
+    k[:, ::2] = 0
+    k[:, ::2, :, 0] = float("-inf")
+    q = torch.randn(2, Nq, 2, 16, device=device).to(kind)
+    q[..., 0] = 1
+    there = torch.ones(2, Nk, dtype=torch.bool, device=device)
+    there[:, ::2] = False
+    assert torch.equal(nn_ops.cross_attention(q, k, v), nn_ops.cross_attention(q, k, v, key_mask=there))
+    assert not nn_ops.cross_attention(q, k, v, key_mask=~there).any()
