@@ -2,10 +2,8 @@
 // nn.GELU() (exact, erf) of timm's Mlp (dino_enc/vision_transformer.py:295-339 via timm.layers.Mlp) and the tanh approximation
 // of the DINO-S discriminator trunk.  One definition, so the fused and the stand-alone paths round identically.
 //
-// Round 4: everything works on PAIRS of values in packed fp32 (v_pk_mul_f32 / v_pk_add_f32 / v_pk_fma_f32: two lanes' worth of
-// arithmetic per VALU issue slot).  The fused fc1 / fc2-gradient GEMM epilogues spend ~11 k VALU cycles per 256 x 256 tile and SIMD
-// on this function with the matrix pipe idle (profiles/r03_gemm_where_the_cycles_go.md: +38 % kernel time over the plain product);
-// the packed form issues ~12 instead of ~20 VALU slots per element.
+// Everything works on PAIRS of values.  The pairs were written for packed fp32 arithmetic; the build has those instructions turned off (the Makefile says why), so that
+// a pair is two scalar operations of each kind, about 20 VALU slots per value.  The fused GEMM epilogues take the values from a table in LDS that these functions fill.
 #pragma once
 #include <hip/hip_runtime.h>
 

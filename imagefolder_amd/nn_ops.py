@@ -383,7 +383,7 @@ def module_embedding(module, idx):
     """the lookup of an nn.Embedding inside a model: nn_ops.embedding (its gradient can be differentiated again, as the module's), or the module itself for what that
     does not take (other types, more than 2^20 rows, a renormalised or sparse table, gradients scaled by frequency, a table of a tensor class of its own), where
     something hangs on the module's call (hooks, another forward) and under traces and transforms that the module has formulas for"""
-    if not (ops_seq.transformed() or torch.jit.is_tracing()) and _runs_plainly(module, torch.nn.Embedding):
+    if not (ops_seq.transformed() or ops_seq.is_tracing()) and _runs_plainly(module, torch.nn.Embedding):
         w = module.weight
         if (w.is_cuda and type(w) in (torch.Tensor, torch.nn.Parameter) and w.dtype in (torch.bfloat16, torch.float32) and w.shape[0] <= ops_seq.MAX_ROWS
                 and module.max_norm is None and not (module.sparse or module.scale_grad_by_freq)):

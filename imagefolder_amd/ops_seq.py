@@ -15,7 +15,7 @@ from ._lib import XqError, check
 _TYPES = (torch.bfloat16, torch.float32)
 _raw_stream = torch._C._cuda_getCurrentRawStream       # the handle alone: torch.cuda.current_stream builds an object, 4 us of a 5 us call
 _current_device = torch._C._cuda_getDevice
-_is_tracing = torch._C._is_tracing
+is_tracing = torch._C._is_tracing                        # (torch.jit.is_tracing asks this and more, for half a microsecond)
 
 
 def _launch(name, device, *args):
@@ -42,7 +42,7 @@ def _wants_node(*tensors):
         for t in tensors:
             if t is not None and t.requires_grad:
                 return True
-    return forward_ad._current_level >= 0 or _is_tracing()
+    return forward_ad._current_level >= 0 or is_tracing()
 
 
 def transformed():
